@@ -500,6 +500,69 @@ int plyolo_lnw_act_bwd(int dtype, int N, int H, int W, int C, const void* dout, 
                        const float* gamma, const float* beta, int act, void* dx, int dx_ld, int accumulate_dx, float* dgamma, float* dbeta,
                        int accumulate_params, void* stream);
 
+/* ------------------------------------------------- group norm + activation, channels last
+ * The batch-free normalisation of a BaseConv unit (norm = "gn"; the reference builds bn / ln there, models/layers/normalization.py:4-13,
+ * network_blocks.py:30-37).  x, out, res, dout, dx are [N*HW, ld] pixel rows of C channels; group k holds channels
+ * [k*C/groups, (k+1)*C/groups) of one image.
+ *   forward   xh = (x - mean) * rstd over the HW * C/groups values of (image, group), biased variance, eps inside the root;
+ *             out = act(gamma * xh + beta) + res          (res NULL: no shortcut)
+ *             stats[N][groups][2] = (mean, rstd), fp32, for the backward
+ *   backward  from dout, x, stats: dx (written, or added to when accumulate_dx), dgamma / dbeta [C] fp32 (either may be NULL; added to
+ *             when accumulate_params).  The shortcut's gradient is dout itself.
+ * gamma, beta: fp32 [C], NULL = 1 / 0.  Any C, pitch and element-aligned address; rows of 16-byte-aligned vectors take the wide path.
+ * Statistics and gradient sums are formed in a fixed order (no atomics): results repeat bit for bit.  A NaN or infinity stays inside its
+ * (image, group).  No operand may overlap another, except out == x and dx == dout (same pitch).
+ * Workspace: plyolo_gn_workspace(d) bytes, 16-byte aligned, contents need not survive a call; calls that may run at the same time
+ * (streams, captured graphs) need one each.  C <= 4096, N*HW and every pitch below 2^31. */
+typedef struct plyolo_gn_desc {
+  int dtype, N, HW, C, groups, act;
+  float eps;
+  int x_ld, o_ld, r_ld; /* o_ld: forward only */
+} plyolo_gn_desc;
+size_t plyolo_gn_workspace(const plyolo_gn_desc* d); /* 0 = the descriptor is invalid (plyolo_last_error) */
+int plyolo_gn_act_fwd(const plyolo_gn_desc* d, const void* x, const float* gamma, const float* beta, const void* res, void* out, float* stats,
+                      void* workspace, size_t ws_bytes, void* stream);
+int plyolo_gn_act_bwd(const plyolo_gn_desc* d, const void* dout, int d_ld, const void* x, const float* stats, const float* gamma,
+                      const float* beta, void* dx, int dx_ld, int accumulate_dx, float* dgamma, float* dbeta, int accumulate_params,
+                      void* workspace, size_t ws_bytes, void* stream);
+
+/* ------------------------------------------------- linear layer (1x1 convolution with bias, no normalisation)
+ * nn.Conv2d(K, N, 1, bias=True) / nn.Linear on pixel rows, with what follows it in its epilogue (reference
+ * models/layers/network_blocks.py:18-37 with norm=None): weights in torch's own layout [N][K] (pitch w_ld, type `dtype`), bias fp32.
+ *   forward   z = x . w^T + bias;  y = act(z) + res      (bias, res, z may be NULL; z [M][z_ld] is what the backward reads)
+ *   backward  dz = dy * act'(z)  (z NULL only for PLYOLO_ACT_NONE);  dx = dz . w (written or added to);  dw = dz^T . x  [N][K] dense, in
+ *             dw_dtype (PLYOLO_F32: the masters' type; or `dtype`);  db[n] = sum dz, fp32.  dx, dw, db may each be NULL; dw and db are
+ *             added to when accumulate_params.  The shortcut's gradient is dy itself.
+ * PLYOLO_BF16: bf16 operands, fp32 accumulation (MFMA), dz rounded to bf16 once for the two products (db sums it unrounded);
+ * PLYOLO_F32: fp32 throughout.  y is formed from the unrounded z.  Any M, N, K >= 1, pitches and element-aligned addresses; operands
+ * whose rows start on 16-byte boundaries with K and N multiples of 8 (bf16) take the wide path.  dy rows have pitch y_ld.
+ * Every sum runs in a fixed order: results repeat bit for bit.  No operand may overlap another.
+ * Workspace: plyolo_linear_workspace(d, backward) bytes, 16-byte aligned, one per call that may run at the same time (0 bytes: none
+ * needed, pass NULL). */
+typedef struct plyolo_linear_desc {
+  int dtype, M, N, K, act;
+  int x_ld, w_ld, y_ld, z_ld, r_ld;
+} plyolo_linear_desc;
+size_t plyolo_linear_workspace(const plyolo_linear_desc* d, int backward);
+int plyolo_linear_fwd(const plyolo_linear_desc* d, const void* x, const void* w, const float* bias, const void* res, void* z, void* y,
+                      void* workspace, size_t ws_bytes, void* stream);
+int plyolo_linear_bwd(const plyolo_linear_desc* d, const void* dy, const void* z, const void* x, const void* w, void* dx, int dx_ld,
+                      int accumulate_dx, void* dw, int dw_dtype, float* db, int accumulate_params, void* workspace, size_t ws_bytes, void* stream);
+
+/* ------------------------------------------------- dropout from a counter-based generator
+ * out = (keep ? x / (1 - p) : 0) + res on [M, ld] rows of C channels; the mask is a function of (seed, step, site, element) and is never
+ * stored: the backward forms it again.  Element i = m * C + c (whatever the pitch) takes word i % 4 of Philox4x32 with 7 rounds (Salmon,
+ * Moraes, Dror, Shaw, "Parallel random numbers: as easy as 1, 2, 3", SC 2011: the fewest rounds its authors report as passing BigCrush),
+ * counter = (low and high half of i / 4, low half of step, site), key = the halves of seed; it is kept when word >> 8 >= round(p * 2^24).
+ * rng: device uint64[2] = {seed, step}, read by the launch (so a captured or replayed launch follows the state); `site` tells the
+ * dropouts of one step apart.  0 <= p <= 1 (p = 1: nothing is kept).  A dropped infinity or NaN is 0.  x == out (same pitch) is allowed.
+ * plyolo_rng_next: out[0..1] = state[0..1]; state[1] += 1 -- one launch per step; forward and backward of the step read `out`. */
+int plyolo_rng_next(uint64_t* state, uint64_t* out, void* stream);
+int plyolo_dropout_fwd(int dtype, int M, int C, const void* x, int x_ld, float p, const uint64_t* rng, unsigned site, const void* res, int r_ld,
+                       void* out, int o_ld, void* stream);
+int plyolo_dropout_bwd(int dtype, int M, int C, const void* dout, int d_ld, float p, const uint64_t* rng, unsigned site, void* dx, int dx_ld,
+                       int accumulate, void* stream);
+
 /* -------------------------------------------------- data movement kernels */
 /* Focus space-to-depth (network_blocks.py:50-65): NCHW fp32 image ->
  * NHWC [N,H/2,W/2,Cp] with channel blocks TL,BL,TR,BR (3 each) then zero pad. */

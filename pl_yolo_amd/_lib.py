@@ -149,6 +149,15 @@ class FmtImage(C.Structure):   # plyolo_fmt_image
     _fields_ = [("det", C.c_void_p), ("n", C.c_int), ("ld", C.c_int), ("row0", C.c_int), ("scale", C.c_float)]
 
 
+class GnDesc(C.Structure):     # plyolo_gn_desc
+    _fields_ = [(n, C.c_int) for n in ("dtype", "N", "HW", "C", "groups", "act")] + [("eps", C.c_float)] + \
+               [(n, C.c_int) for n in ("x_ld", "o_ld", "r_ld")]
+
+
+class LinearDesc(C.Structure):     # plyolo_linear_desc
+    _fields_ = [(n, C.c_int) for n in ("dtype", "M", "N", "K", "act", "x_ld", "w_ld", "y_ld", "z_ld", "r_ld")]
+
+
 _vp, _i, _f, _d, _sz = C.c_void_p, C.c_int, C.c_float, C.c_double, C.c_size_t
 _P = C.POINTER
 
@@ -204,6 +213,15 @@ SIGNATURES = {
     "plyolo_reduce_slabs": (_i, [_vp, _i, _sz, _vp]),
     "plyolo_lnw_act_fwd": (_i, [_i, _i, _i, _i, _i, _vp, _i, _vp, _vp, _f, _i, _vp, _i, _vp, _vp]),
     "plyolo_lnw_act_bwd": (_i, [_i, _i, _i, _i, _i, _vp, _i, _vp, _i, _vp, _vp, _vp, _i, _vp, _i, _i, _vp, _vp, _i, _vp]),
+    "plyolo_gn_workspace": (_sz, [_P(GnDesc)]),
+    "plyolo_gn_act_fwd": (_i, [_P(GnDesc), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "plyolo_gn_act_bwd": (_i, [_P(GnDesc), _vp, _i, _vp, _vp, _vp, _vp, _vp, _i, _i, _vp, _vp, _i, _vp, _sz, _vp]),
+    "plyolo_linear_workspace": (_sz, [_P(LinearDesc), _i]),
+    "plyolo_linear_fwd": (_i, [_P(LinearDesc), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "plyolo_linear_bwd": (_i, [_P(LinearDesc), _vp, _vp, _vp, _vp, _vp, _i, _i, _vp, _i, _vp, _i, _vp, _sz, _vp]),
+    "plyolo_rng_next": (_i, [_vp, _vp, _vp]),
+    "plyolo_dropout_fwd": (_i, [_i, _i, _i, _vp, _i, _f, _vp, C.c_uint, _vp, _i, _vp, _i, _vp]),
+    "plyolo_dropout_bwd": (_i, [_i, _i, _i, _vp, _i, _f, _vp, C.c_uint, _vp, _i, _i, _vp]),
     "plyolo_mosaic4": (_i, [_vp, _i, _i, _vp, _vp]),
     "plyolo_warp_affine_u8": (_i, [_vp, _i, _i, _P(_d), _vp, _i, _i, _i, _vp]),
     "plyolo_warp_perspective_u8": (_i, [_vp, _i, _i, _P(_d), _vp, _i, _i, _i, _vp]),
