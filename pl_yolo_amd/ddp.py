@@ -142,6 +142,7 @@ def _op_params(op):
         bn = getattr(op, attr, None)
         if bn is not None:
             ps += [bn.weight, bn.bias]
+    ps += getattr(op, "own_params", [])
     if isinstance(op, G.DwConvUnitOp):
         ps.append(op.w)
     if isinstance(op, G.ImplicitHeadOp):

@@ -21,7 +21,7 @@ import os
 import torch
 
 from . import _lib
-from ._lib import BF16, F32, ACT, STAT_SLOTS, BnStats, Split, BnBwdSplit, BnBwdFuse, BnRed, BN_RED_SEGS, ConvDesc, PackEntry, YoloxDesc, yolov7_desc, call, ptr
+from ._lib import BF16, F32, ACT, STAT_SLOTS, BnStats, Split, BnBwdSplit, BnBwdFuse, BnRed, BN_RED_SEGS, ConvDesc, GnDesc, LinearDesc, PackEntry, YoloxDesc, yolov7_desc, call, ptr
 
 BN_EPS_DEFAULT = 1e-3
 
@@ -97,6 +97,8 @@ class Graph:
         self.scratch_elems = 0  # shared dz scratch (activation dtype)
         self.scratch_f32 = 0    # shared fp32 scratch (maxpool backward)
         self.image_act = None
+        self.root = None        # the module that is traced (rng_state_of: the dropouts' seed and step belong to it)
+        self.rng, self.n_drop = None, 0     # this graph's copy of (seed, step) during one forward -> backward pair; dropouts so far
         self.post_unpack = []   # ops with work that must follow unpack_wgrads
         self.plan = None        # the Plan being recorded (ops use it for lanes / events)
         self.cur_lane, self.cur_lane_fwd = 0, None
@@ -566,11 +568,20 @@ class Graph:
         self.flush_reduce_on_lane()
         if self.use_lanes:
             self.flush_param_grads()
-            self.plan.wait(0, self.plan.record(WGRAD_LANE))
+            if self.plan.lanes() > WGRAD_LANE:      # (a plan without convolutions never used that lane)
+                self.plan.wait(0, self.plan.record(WGRAD_LANE))
 
     def zero_fwd_stats(self):
         if self.training:
             call("plyolo_memset_async", self.stat_arena.data_ptr(), 0, self.stat_arena.numel() * 8, None)
+
+    def next_rng(self):
+        """In front of a forward plan's ops: this step's (seed, step) for its dropouts, and the module's step counter moved on."""
+        if self.rng is not None and self.training:
+            call("plyolo_rng_next", rng_state_of(self.root, self.device).data_ptr(), self.rng.data_ptr(), None)
+
+    def top_is(self, module):
+        return self.root is module
 
     def zero_bwd_stats(self):
         call("plyolo_memset_async", self.bstat_arena.data_ptr(), 0, self.bstat_arena.numel() * 8, None)
@@ -603,9 +614,13 @@ class Graph:
         self.n_pack = n
 
     def pack_weights(self):
+        if self.n_pack == 0:      # a sub-module without convolutions (Dropout, a linear unit)
+            return
         call("plyolo_pack_weights_flat", self.pack_table.data_ptr(), self.n_pack, self.dtype, self.pack_blocks, None)
 
     def unpack_wgrads(self):
+        if self.n_pack == 0:
+            return
         call("plyolo_unpack_wgrads_flat", self.pack_table.data_ptr(), self.n_pack, self.pack_blocks, 0, None)
 
     # ----------------------------------------------------------------- gradients
@@ -706,7 +721,7 @@ def op_io(op):
         return [op.src], [op.dst]
     if isinstance(op, ConvPairOp):
         return [op.x], [op.out_a, op.out_b]
-    if isinstance(op, (ConvUnitOp, DwConvUnitOp, BnOnlyOp)):
+    if isinstance(op, (ConvUnitOp, DwConvUnitOp, BnOnlyOp, LinearOp, DropoutOp)):
         return [op.x] + ([op.res] if op.res is not None else []), [op.out]
     if isinstance(op, (BicubicUpsampleOp, ActOp, LnWidthOp, UpsampleOp, MaxPool2x2Op)):
         return [op.x], [op.out]
@@ -1007,6 +1022,10 @@ class ConvUnitOp:
              g.aptr(self.res) if self.res is not None else None, self.res.ld if self.res is not None else 0,
              g.aptr(self.out), self.out.ld, C.byref(st) if st is not None else None, None, None)
 
+    def form_dz(self, dout, zt, dz):
+        # BaseConv(norm=None): out = act(z)  (ecmnet.py:158 Bottleneck.conv1) -> dz = dout * act'(z)
+        call("plyolo_act_bwd", self.g.dtype, self.out.M, self.Cout, dout, self.out.ld, zt, self.Cout, self.act, dz, self.Cout, 0, None)
+
     def bwd(self):
         g, bn = self.g, self.bn
         if not g.grad_ready(self.out):
@@ -1032,8 +1051,7 @@ class ConvUnitOp:
             if not (res_in_dz or res_in_dgrad):
                 call("plyolo_copy_add", g.dtype, M, Cout, dout, self.out.ld, g.gptr(self.res), self.res.ld, acc_res, None)
         if bn is None:
-            # BaseConv(norm=None): out = act(z)  (ecmnet.py:158 Bottleneck.conv1) -> dz = dout * act'(z)
-            call("plyolo_act_bwd", g.dtype, M, Cout, dout, self.out.ld, zt, Cout, self.act, dz, Cout, 0, None)
+            self.form_dz(dout, zt, dz)
         else:
             bslots = g.bstat_arena.data_ptr() + self.slot_off * 8
             if not (g.diag_skip_r or self.red_done):
@@ -1431,6 +1449,150 @@ class BnOnlyOp:
              g.grad_ptr_of(bn.weight), g.grad_ptr_of(bn.bias), 0, 0, dz, Cc, None, None, None)
         acc = g.grad_mode(x)    # here dz IS the gradient w.r.t. the normalised tensor itself
         call("plyolo_copy_add", g.dtype, M, Cc, dz, Cc, g.gptr(x), x.ld, acc, None)
+
+
+def rng_state_of(module, device=None):
+    """Device tensor (seed, step) of the dropouts of a traced module (layers.dropout_state)."""
+    s = module.__dict__.get("_dropout_state")
+    if device is None:
+        p = next(module.parameters(), None)
+        device = p.device if p is not None else (s.device if s is not None else torch.device("cuda", torch.cuda.current_device()))
+    if s is None:
+        seed = int(torch.randint(0, 1 << 62, (1,)).item())
+        if torch.distributed.is_available() and torch.distributed.is_initialized():
+            seed ^= torch.distributed.get_rank() * 0x1E3779B97F4A7C15 & ((1 << 62) - 1)
+        s = torch.tensor([seed, 0], dtype=torch.int64, device=device)
+        module.__dict__["_dropout_state"] = s
+    elif s.device != device:
+        s = s.to(device)
+        module.__dict__["_dropout_state"] = s
+    return s
+
+
+class GnConvUnitOp(ConvUnitOp):
+    """BaseConv with norm = "gn": conv -> group norm -> activation [+ residual].  z is the convolution's output as it is; one
+    plyolo_gn_act_fwd normalises, activates and adds the shortcut, one plyolo_gn_act_bwd forms dz and the affine gradients."""
+
+    def __init__(self, g, x, conv_w, gn, act, stride, residual=None, need_dgrad=True, cin_pad=None):
+        super().__init__(g, x, conv_w, None, None, stride, residual, need_dgrad, cin_pad)
+        self.gn, self.gn_act = gn, ACT[act]
+        self.own_params = [p for p in (gn.weight, gn.bias) if p is not None]
+
+    def _gn(self):
+        if not hasattr(self, "gn_desc"):
+            d = GnDesc()
+            d.dtype, d.N, d.HW, d.C, d.groups, d.act, d.eps = (self.g.dtype, self.out.N, self.OH * self.OW, self.Cout, self.gn.num_groups, self.gn_act,
+                                                               float(self.gn.eps))
+            d.x_ld, d.o_ld, d.r_ld = self.Cout, self.out.ld, self.res.ld if self.res is not None else 0
+            self.gn_desc = d
+            self.stats = torch.empty(d.N * d.groups * 2, dtype=torch.float32, device=self.g.device)
+            # its own: launches of other lanes may run beside it
+            n = _lib.lib().plyolo_gn_workspace(C.byref(d))
+            if n == 0:
+                _lib.check(-1, "plyolo_gn_workspace")
+            self.ws = torch.empty(n, dtype=torch.uint8, device=self.g.device)
+        return C.byref(self.gn_desc)
+
+    def fwd(self):
+        g, gn = self.g, self.gn
+        self._alloc_small()
+        zt = self.z.tensor.data_ptr()
+        call("plyolo_conv2d_fwd", C.byref(self.desc), self.xptr, self.pc.wp, None, zt, None, None)
+        call("plyolo_gn_act_fwd", self._gn(), zt, ptr(gn.weight), ptr(gn.bias), g.aptr(self.res) if self.res is not None else None, g.aptr(self.out),
+             self.stats.data_ptr(), self.ws.data_ptr(), self.ws.numel(), None)
+
+    def form_dz(self, dout, zt, dz):
+        g, gn = self.g, self.gn
+        call("plyolo_gn_act_bwd", self._gn(), dout, self.out.ld, zt, self.stats.data_ptr(), ptr(gn.weight), ptr(gn.bias), dz, self.Cout, 0,
+             g.grad_ptr_of(gn.weight), g.grad_ptr_of(gn.bias), 0, self.ws.data_ptr(), self.ws.numel(), None)
+
+
+class LinearOp:
+    """BaseConv(1x1, bias=True, norm=None): y = act(x . W^T + b) [+ residual] on the pixel rows (plyolo_linear_fwd / _bwd).  The weights are
+    the masters themselves in fp32, a copy cast by every forward in bf16 (they change with every optimizer step)."""
+
+    def __init__(self, g, x, conv_w, conv_b, act, residual=None, need_dgrad=True):
+        self.g, self.x, self.w, self.b, self.act, self.res, self.need_dgrad = g, x, conv_w, conv_b, ACT[act], residual, need_dgrad
+        N, K = conv_w.shape[0], conv_w.shape[1]
+        assert x.C == K, "linear input channels %d != %d" % (x.C, K)
+        x.needs_tensor = True
+        if residual is not None:
+            residual.needs_tensor = True
+        self.N, self.K = N, K
+        self.own_params = [p for p in (conv_w, conv_b) if p is not None]
+        self.macs = x.M * N * K
+        self.out = g.new_act(x.N, x.H, x.W, N, "lin")
+        self.z = None
+        if g.training and self.act != 0:
+            self.z = Storage(x.N, x.H, x.W, N, "z")
+            g.storages.append(self.z)
+        g.add_op(self)
+
+    def _desc(self):
+        g = self.g
+        if not hasattr(self, "desc"):
+            d = LinearDesc()
+            d.dtype, d.M, d.N, d.K, d.act = g.dtype, self.x.M, self.N, self.K, self.act
+            d.x_ld, d.w_ld, d.y_ld, d.z_ld, d.r_ld = self.x.ld, self.K, self.out.ld, self.N, self.res.ld if self.res is not None else 0
+            self.desc = d
+            lib = _lib.lib()
+            n = max(lib.plyolo_linear_workspace(C.byref(d), 0), lib.plyolo_linear_workspace(C.byref(d), 1) if g.training else 0, 16)
+            self.ws = torch.empty(n, dtype=torch.uint8, device=g.device)
+            self.wt = torch.empty(self.N * self.K, dtype=g.tdtype, device=g.device) if g.dtype == BF16 else self.w
+        return C.byref(self.desc)
+
+    def fwd(self):
+        g = self.g
+        d = self._desc()
+        if g.dtype == BF16:
+            call("plyolo_f32_to_act", g.dtype, self.N, self.K, self.w.data_ptr(), self.wt.data_ptr(), self.K, 0, None)
+        call("plyolo_linear_fwd", d, g.aptr(self.x), self.wt.data_ptr(), ptr(self.b), g.aptr(self.res) if self.res is not None else None,
+             self.z.tensor.data_ptr() if self.z is not None else None, g.aptr(self.out), self.ws.data_ptr(), self.ws.numel(), None)
+
+    def bwd(self):
+        g = self.g
+        if not g.grad_ready(self.out):
+            return
+        dy = g.gptr(self.out)
+        if self.res is not None:
+            call("plyolo_copy_add", g.dtype, self.out.M, self.N, dy, self.out.ld, g.gptr(self.res), self.res.ld, g.grad_mode(self.res), None)
+        dw, db = g.grad_ptr_of(self.w), g.grad_ptr_of(self.b)
+        if not (self.need_dgrad or dw or db):
+            return
+        acc = g.grad_mode(self.x) if self.need_dgrad else 0
+        call("plyolo_linear_bwd", self._desc(), dy, self.z.tensor.data_ptr() if self.z is not None else None, g.aptr(self.x), self.wt.data_ptr(),
+             g.gptr(self.x) if self.need_dgrad else None, self.x.ld, acc, dw, F32, db, 0, self.ws.data_ptr(), self.ws.numel(), None)
+
+
+class DropoutOp:
+    """out = dropout(x, p) [+ residual].  The mask is formed from the graph's (seed, step), this op's number and the element index, forward
+    and backward alike."""
+
+    def __init__(self, g, x, p, residual=None):
+        self.g, self.x, self.p, self.res = g, x, float(p), residual
+        x.needs_tensor = True
+        if residual is not None:
+            residual.needs_tensor = True
+        self.site = g.n_drop
+        g.n_drop += 1
+        if g.rng is None:
+            g.rng = torch.zeros(2, dtype=torch.int64, device=g.device)
+        self.out = g.new_act(x.N, x.H, x.W, x.C, "drop")
+        g.add_op(self)
+
+    def fwd(self):
+        g, x = self.g, self.x
+        call("plyolo_dropout_fwd", g.dtype, x.M, x.C, g.aptr(x), x.ld, self.p, g.rng.data_ptr(), self.site,
+             g.aptr(self.res) if self.res is not None else None, self.res.ld if self.res is not None else 0, g.aptr(self.out), self.out.ld, None)
+
+    def bwd(self):
+        g, x = self.g, self.x
+        if not g.grad_ready(self.out):
+            return
+        dy = g.gptr(self.out)
+        if self.res is not None:
+            call("plyolo_copy_add", g.dtype, x.M, x.C, dy, self.out.ld, g.gptr(self.res), self.res.ld, g.grad_mode(self.res), None)
+        call("plyolo_dropout_bwd", g.dtype, x.M, x.C, dy, self.out.ld, self.p, g.rng.data_ptr(), self.site, g.gptr(x), x.ld, g.grad_mode(x), None)
 
 
 class LnWidthOp:

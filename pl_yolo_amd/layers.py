@@ -5,6 +5,8 @@ nn.BatchNorm2d containers, so checkpoints load unchanged) and describe their
 computation to the HIP launch-plan builder through `emit(g, x)`; they never run
 torch compute kernels themselves.
 """
+import math
+
 import torch
 import torch.nn as nn
 
@@ -27,13 +29,16 @@ def get_activation(name="silu", inplace=True):
 
 
 def get_normalization(name, out_channels):
-    """normalization.py:4-13 (bn = BatchNorm2d(eps=1e-3, momentum=0.03))."""
+    """normalization.py:4-13 (bn = BatchNorm2d(eps=1e-3, momentum=0.03)).  "gn" is this package's own: GroupNorm over gcd(32, C) groups,
+    for batches too small per GPU for batch statistics (csrc/groupnorm.hip; the same in training and inference)."""
     if name is None:
         return None
     if name == "bn":
         return nn.BatchNorm2d(out_channels, eps=1e-3, momentum=0.03)
     if name == "ln":
         return nn.LayerNorm(out_channels)     # over the LAST axis of the NCHW tensor, i.e. the width (G.LnWidthOp)
+    if name == "gn":
+        return nn.GroupNorm(math.gcd(32, out_channels), out_channels)
     raise AttributeError("Unsupported normalization function type: {}".format(name))
 
 
@@ -56,24 +61,38 @@ class HipModule(nn.Module):
 
 
 class BaseConv(HipModule):
-    """A Convolution2d -> Normalization -> Activation (network_blocks.py:7-40)."""
+    """A Convolution2d -> Normalization -> Activation (network_blocks.py:7-40).
 
-    def __init__(self, in_channels, out_channels, ksize, stride, padding=None, groups=1, bias=False, norm="bn", act="silu"):
+    Beyond the reference's argument values: norm="gn" (get_normalization), bias=True on a 1x1 stride-1 unit without normalisation (the
+    linear layer of csrc/linear.hip, trainable, any channel counts), and `drop`: dropout of the activated output with this probability
+    in training, in front of the shortcut where the unit has one (csrc/dropout.hip)."""
+
+    def __init__(self, in_channels, out_channels, ksize, stride, padding=None, groups=1, bias=False, norm="bn", act="silu", drop=0.0):
         super().__init__()
         pad = (ksize - 1) // 2 if padding is None else padding
         # groups: 1 (MFMA kernels) or depthwise 3x3 stride 1 (groups == in == out: the e-yolox Bottleneck, csrc/dwconv.hip)
         self.depthwise = groups != 1 and groups == in_channels == out_channels and ksize == 3 and stride == 1
-        if (groups != 1 and not self.depthwise) or bias or pad != (ksize - 1) // 2 or ksize not in (1, 3) or stride not in (1, 2):
-            raise NotImplementedError("HIP conv supports k in {1,3}, stride in {1,2}, same padding, no bias, groups=1 or depthwise 3x3 stride 1")
+        self.linear = bool(bias) and norm is None and groups == 1 and ksize == 1 and stride == 1
+        if (groups != 1 and not self.depthwise) or (bias and not self.linear) or pad != (ksize - 1) // 2 or ksize not in (1, 3) or stride not in (1, 2):
+            raise NotImplementedError("HIP conv supports k in {1,3}, stride in {1,2}, same padding, no bias (except 1x1 stride 1 with norm=None), "
+                                      "groups=1 or depthwise 3x3 stride 1")
+        if not 0.0 <= drop <= 1.0:
+            raise ValueError("dropout probability has to be between 0 and 1, but got {}".format(drop))
         self.conv = nn.Conv2d(in_channels, out_channels, kernel_size=ksize, stride=stride, padding=pad, groups=groups, bias=bias)
         self.norm = get_normalization(norm, out_channels)
         self.act = get_activation(act, inplace=True)
         self.stride = stride
+        self.drop = float(drop)
 
     def emit(self, g, x, residual=None, need_dgrad=True, cin_pad=None):
+        if getattr(self, "drop", 0.0) > 0.0 and g.training:
+            return G.DropoutOp(g, self._emit_unit(g, x, None, need_dgrad, cin_pad), self.drop, residual).out
+        return self._emit_unit(g, x, residual, need_dgrad, cin_pad)
+
+    def _emit_unit(self, g, x, residual, need_dgrad, cin_pad):
         act = self.act.act_name if self.act is not None else None
         if getattr(self, "depthwise", False):
-            if self.norm is None:
+            if not isinstance(self.norm, nn.BatchNorm2d):
                 raise NotImplementedError("depthwise BaseConv without BatchNorm (fold it back or keep norm='bn')")
             return G.DwConvUnitOp(g, x, self.conv.weight, self.norm, act, residual).out
         if isinstance(self.norm, nn.LayerNorm):
@@ -81,6 +100,10 @@ class BaseConv(HipModule):
                 raise NotImplementedError("a shortcut on a BaseConv with norm='ln'")
             z = G.ConvUnitOp(g, x, self.conv.weight, None, None, self.stride, None, need_dgrad, cin_pad, conv_b=self.conv.bias).out
             return G.LnWidthOp(g, z, self.norm, act).out
+        if isinstance(self.norm, nn.GroupNorm):
+            return G.GnConvUnitOp(g, x, self.conv.weight, self.norm, act, self.stride, residual, need_dgrad, cin_pad).out
+        if getattr(self, "linear", False):
+            return G.LinearOp(g, x, self.conv.weight, self.conv.bias, act, residual, need_dgrad).out
         op = G.ConvUnitOp(g, x, self.conv.weight, self.norm, act, self.stride, residual, need_dgrad, cin_pad, conv_b=self.conv.bias)
         return op.out
 
@@ -89,6 +112,8 @@ class BaseConv(HipModule):
         it, so that forward == the reference's `fuseforward` = act(conv(x)) (network_blocks.py:39-40; the folding rule is
         RepConv.fuse_conv_bn, yolov7_neck.py:265-286).  One HIP launch (plyolo_fold_conv_bn); inference only."""
         if self.norm is None or getattr(self, "depthwise", False):   # depthwise units keep their BatchNorm (no fused deploy kernel)
+            return self
+        if isinstance(self.norm, nn.GroupNorm):      # its statistics are the input's own: nothing to fold
             return self
         if not isinstance(self.norm, nn.BatchNorm2d):
             raise NotImplementedError("only BatchNorm2d folds into a convolution")
@@ -138,12 +163,36 @@ def emit_pair(g, x, unit_a, unit_b):
     act_a = unit_a.act.act_name if unit_a.act is not None else None
     act_b = unit_b.act.act_name if unit_b.act is not None else None
     same = (g.pair_convs and ca.kernel_size == cb.kernel_size and unit_a.stride == unit_b.stride and act_a == act_b
-            and na is not None and nb is not None and na.eps == nb.eps and na.momentum == nb.momentum
+            and isinstance(na, nn.BatchNorm2d) and isinstance(nb, nn.BatchNorm2d) and not (getattr(unit_a, "drop", 0.0) or getattr(unit_b, "drop", 0.0)) and na.eps == nb.eps and na.momentum == nb.momentum
             and ca.out_channels % g.vec == 0 and cb.out_channels % g.vec == 0)
     if not same:
         return unit_a.emit(g, x), unit_b.emit(g, x)
     op = G.ConvPairOp(g, x, ca.weight, na, cb.weight, nb, act_a, unit_a.stride)
     return op.out_a, op.out_b
+
+
+class Dropout(HipModule):
+    """nn.Dropout(p) of a feature map: every element on its own, scaled by 1 / (1 - p), in training; the identity in eval mode.  The mask
+    is a function of (seed, step, place in the network, element) and is never stored (csrc/dropout.hip); see dropout_state()."""
+
+    def __init__(self, p=0.5):
+        super().__init__()
+        if not 0.0 <= p <= 1.0:
+            raise ValueError("dropout probability has to be between 0 and 1, but got {}".format(p))
+        self.p = float(p)
+
+    def emit(self, g, x, residual=None):
+        p = self.p if g.training else 0.0
+        if p == 0.0 and residual is None and not g.top_is(self):
+            return x
+        return G.DropoutOp(g, x, p, residual).out
+
+
+def dropout_state(module):
+    """The state of `module`'s dropouts: a device int64 tensor (seed, step).  Every training forward of the module advances `step` by one;
+    copying a saved tensor back (`dropout_state(m).copy_(saved)`) resumes its masks.  The seed is drawn from torch's default CPU generator
+    when the state is first used (torch.manual_seed makes it repeat), with the rank of the process group mixed in."""
+    return G.rng_state_of(module)
 
 
 class Focus(HipModule):

@@ -82,6 +82,7 @@ class ModuleRunner:
         m = self.m
         g = G.Graph(BF16 if dtype == "bf16" else F32, training, device)
         g.grad_ptr_of = self.grad_ptr_of
+        g.root = m
         s = _Session()
         s.g, s.image, s.stem_kind = g, image, None
         vec = g.vec
@@ -132,6 +133,7 @@ class ModuleRunner:
             g.plan = s.fwd
             g.pack_weights()
             g.zero_fwd_stats()
+            g.next_rng()
             G.record_ops(g, s.fwd, g.ops, "fwd", lanes=False)
         s.bwd = None
         s.used_params = []
@@ -168,6 +170,11 @@ class ModuleRunner:
                         if p is not None and id(p) not in seen:
                             seen.add(id(p))
                             s.used_params.append(p)
+            for op in g.ops:      # affine pairs of group norms, weights of linear layers: their launches write the gradients directly
+                for p in getattr(op, "own_params", ()):
+                    if id(p) not in seen:
+                        seen.add(id(p))
+                        s.used_params.append(p)
             for (_, w, b) in g.pack_entries:
                 for p in (w, b):
                     if p is not None and id(p) not in seen:

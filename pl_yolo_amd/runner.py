@@ -140,6 +140,7 @@ class DetectorRunner:
         training = model.training
         g = G.Graph(self.dtype, training, device)
         g.grad_ptr_of = self.grad_ptr_of
+        g.root = model
         s = _Session()
         s.g, s.mode, s.B, s.H, s.W, s.M = g, mode, B, H, W, M
         s.generation = 0          # bumped by every forward of this session (see _check_generation)
@@ -187,6 +188,7 @@ class DetectorRunner:
             g.plan = s.fwd
             g.pack_weights()
             g.zero_fwd_stats()
+            g.next_rng()
             # PLYOLO_FWD_LANES=0 records the forward on one lane, which then replays as ONE hipGraph: measured 2 %
             # slower than the eager replay with the head levels side by side (a dependent launch costs ~1.8 us in a
             # graph against ~5 us eagerly for EMPTY kernels, tools/micro/graph_floor.hip, but behind real kernels the
@@ -235,6 +237,11 @@ class DetectorRunner:
                         if p is not None and id(p) not in seen:
                             seen.add(id(p))
                             s.used_params.append(p)
+            for op in g.ops:      # affine pairs of group norms, weights of linear layers: their launches write the gradients directly
+                for p in getattr(op, "own_params", ()):
+                    if id(p) not in seen:
+                        seen.add(id(p))
+                        s.used_params.append(p)
             for (_, w, b) in g.pack_entries:
                 for p in (w, b):
                     if p is not None and id(p) not in seen:

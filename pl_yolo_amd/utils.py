@@ -55,6 +55,8 @@ def conv_macs(model, height, width):
             macs += pos * sum(int(w.numel()) for (w, _, _) in pc.sources)
         if isinstance(op, G.DwConvUnitOp):      # depthwise weights are not packed
             macs += op.x.H * op.x.W * int(op.w.numel())
+        if isinstance(op, G.LinearOp):
+            macs += op.macs
     return macs
 
 
