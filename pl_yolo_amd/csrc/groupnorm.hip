@@ -4,9 +4,12 @@
 //   du = dout act'(u),  dbeta = sum du,  dgamma = sum du xh,  v = gamma du
 //   dx = rstd (v - mean(v) - xh mean(v xh))                                  means over the same (image, group)
 //
-// Both directions are HBM streams around one reduction, and the reduction separates them into two launches: the first leaves one partial
-// per (image, chunk of rows) in the workspace, the second joins the partials of its image in a fixed order in its prologue (a few KB out of
-// L2) and streams.  A thread owns one vector of channels for the whole launch and walks down the rows, as in the BatchNorm kernels.
+// Both directions are HBM streams around one reduction.
+//   resident   a workgroup owns (image, slice of whole groups) and holds its rows in registers across the reduction: one launch, every
+//              operand read once (gn_res_*_kernel).  Taken wherever the slice fits.
+//   streaming  two launches: the first leaves one partial per (image, chunk of rows) in the workspace, the second joins the partials of its
+//              image in a fixed order in its prologue (a few KB out of L2) and streams.
+// A thread owns one vector of channels for the whole launch and walks down the rows, as in the BatchNorm kernels.
 //
 // The variance is never formed as E[x^2] - E[x]^2: a thread sums deviations from its own first value, (count, mean, M2) triples are joined
 // by Chan's formula, and the means of the triples are kept as distances from the first value of their (image, group): neither a mean of
@@ -17,15 +20,46 @@ namespace {
 
 constexpr int GN_MAXC = 4096;    // channels (LDS: two floats each)
 
-// V channels of one row as fp32: the 16-byte vector of Vec<T>, or (V == 1) one element at any alignment
-template <typename T, int V> struct Lane {
-  static DEVINL void load(const T* p, float (&f)[V]) { Vec<T>::load(p, f); }
-  static DEVINL void store(T* p, const float (&f)[V]) { Vec<T>::store(p, f); }
+typedef u32x4 __attribute__((aligned(2))) u32x4_any;     // 16 bytes at any element address: the same instruction as the aligned access
+typedef f32x4 __attribute__((aligned(4))) f32x4_any;
+
+// V channels of one row: a 16-byte vector (8 bf16, 4 fp32) at any element address, or (V == 1) one element
+template <typename T, int V> struct Lane;
+template <> struct Lane<bf16_t, 8> {
+  typedef u32x4 raw;
+  static DEVINL raw get(const bf16_t* p) { return *(const u32x4_any*)p; }
+  static DEVINL void cvt(const raw& v, float (&f)[8]) { Vec<bf16_t>::cvt(v, f); }
+  static DEVINL void store(bf16_t* p, const float (&f)[8]) {
+    u32x4 v;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = pack2bf(f[2 * i], f[2 * i + 1]);
+    *(u32x4_any*)p = v;
+  }
+};
+template <> struct Lane<float, 4> {
+  typedef f32x4 raw;
+  static DEVINL raw get(const float* p) { return *(const f32x4_any*)p; }
+  static DEVINL void cvt(const raw& v, float (&f)[4]) { Vec<float>::cvt(v, f); }
+  static DEVINL void store(float* p, const float (&f)[4]) { *(f32x4_any*)p = f32x4{f[0], f[1], f[2], f[3]}; }
 };
 template <typename T> struct Lane<T, 1> {
-  static DEVINL void load(const T* p, float (&f)[1]) { f[0] = ActT<T>::ld(p); }
+  typedef T raw;
+  static DEVINL raw get(const T* p) { return *p; }
+  static DEVINL void cvt(const raw& v, float (&f)[1]) { f[0] = ActT<T>::ld(&v); }
   static DEVINL void store(T* p, const float (&f)[1]) { ActT<T>::st(p, f[0]); }
 };
+template <typename T, int V> DEVINL void lane_load(const T* p, float (&f)[V]) { Lane<T, V>::cvt(Lane<T, V>::get(p), f); }
+
+// act(u) and act'(u).  bf16 SiLU is written out: both passes of the backward recompute it, and at 8 TB/s the vector ALU has about fifteen
+// issue slots per element (the hardware exponential and reciprocal take four each)
+template <bool PRECISE> DEVINL float gn_act(float u, int act) { return actf<PRECISE>(u, act); }
+template <bool PRECISE> DEVINL float gn_act_grad(float u, int act) {
+  if (!PRECISE && act == PLYOLO_ACT_SILU) {
+    const float s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(u * -1.4426950408889634f));
+    return fmaf(s, fmaf(-u, s, u), s);
+  }
+  return act_grad<PRECISE>(u, act);
+}
 
 struct GnP {
   const void* x;
@@ -80,11 +114,11 @@ template <typename T, int V> __global__ __launch_bounds__(256) void gn_stats_ker
       float k[V], s[V], q[V], f[V];
 #pragma unroll
       for (int e = 0; e < V; ++e) k[e] = s[e] = q[e] = 0.f;
-      if (trow < nr) Lane<T, V>::load(px + (size_t)trow * p.x_ld, k);
+      if (trow < nr) lane_load<T, V>(px + (size_t)trow * p.x_ld, k);
       int cnt = trow < nr ? 1 : 0;
 #pragma unroll 4
       for (int r = trow + rpb; r < nr; r += rpb) {
-        Lane<T, V>::load(px + (size_t)r * p.x_ld, f);
+        lane_load<T, V>(px + (size_t)r * p.x_ld, f);
 #pragma unroll
         for (int e = 0; e < V; ++e) {
           const float d = f[e] - k[e];
@@ -102,15 +136,15 @@ template <typename T, int V> __global__ __launch_bounds__(256) void gn_stats_ker
       }
     }
     __syncthreads();
-    const int nch = min(cols, cv - cb) * V;
+    const int nch = min(cols, cv - cb) * V, nrow = min(rpb, nr);
     for (int t = threadIdx.x; t < nch; t += 256) {
-      float cnt = 0.f, mean = 0.f, m2 = 0.f;
-      for (int w = 0; w < rpb && w < nr; ++w) {
+      float mean = 0.f, m2 = 0.f;
+      for (int w = 0; w < nrow; ++w) mean = fmaf(red[w * cols * V + t].x, (float)((nr - w + rpb - 1) / rpb), mean);
+      mean /= (float)nr;
+      for (int w = 0; w < nrow; ++w) {
         const float2 o = red[w * cols * V + t];
-        const float nb = (float)((nr - w + rpb - 1) / rpb), tot = cnt + nb, d = o.x - mean;
-        m2 += o.y + (cnt > 0.f ? d * d * (cnt * nb / tot) : 0.f);
-        mean += d * (nb / tot);
-        cnt = tot;
+        const float d = o.x - mean;
+        m2 += fmaf(d * d, (float)((nr - w + rpb - 1) / rpb), o.y);
       }
       chan[(size_t)cb * V + t] = make_float2(mean, m2);
     }
@@ -140,7 +174,8 @@ template <typename T, int V> __global__ __launch_bounds__(256) void gn_stats_ker
   }
 }
 
-// joins the chunk partials of image n: gm[2 g], gm[2 g + 1] = mean, rstd
+// joins the chunk partials of image n: gm[2 g], gm[2 g + 1] = mean, rstd.  A lane requests its (up to) 16 partials before it uses the first:
+// the joins are one round trip to L2, not one per partial.
 DEVINL void gn_join_stats(const GnP& p, int n, float* gm) {
   const int L = join_lanes(p.G), gl = threadIdx.x % L, gstep = 256 / L;
   const float2* part = p.gpart + (size_t)n * p.chunks * p.G;
@@ -148,17 +183,33 @@ DEVINL void gn_join_stats(const GnP& p, int n, float* gm) {
   for (int g0 = 0; g0 < p.G; g0 += gstep) {
     const int g = g0 + threadIdx.x / L;
     const bool on = g < p.G;
+    float2 o[16];
     double sm = 0.0;
-    if (on)
-      for (int j = gl; j < p.chunks; j += L) sm += (double)part[(size_t)j * p.G + g].x * (double)min(p.HW - j * p.rows, p.rows);
+    for (int j0 = gl; j0 < p.chunks; j0 += 16 * L) {
+#pragma unroll
+      for (int k = 0; k < 16; ++k) {
+        const int j = j0 + k * L;
+        o[k] = (on && j < p.chunks) ? part[(size_t)j * p.G + g] : make_float2(0.f, 0.f);
+      }
+#pragma unroll
+      for (int k = 0; k < 16; ++k) sm += (double)o[k].x * (double)max(min(p.HW - (j0 + k * L) * p.rows, p.rows), 0);
+    }
     const double mean = lane_sum(sm, L) / (double)p.HW;
     double m2 = 0.0;
-    if (on)
-      for (int j = gl; j < p.chunks; j += L) {
-        const float2 o = part[(size_t)j * p.G + g];
-        const double d = (double)o.x - mean;
-        m2 += (double)o.y + d * d * ((double)min(p.HW - j * p.rows, p.rows) * p.cg);
+    for (int j0 = gl; j0 < p.chunks; j0 += 16 * L) {
+      if (p.chunks > 16 * L) {
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+          const int j = j0 + k * L;
+          o[k] = (on && j < p.chunks) ? part[(size_t)j * p.G + g] : make_float2(0.f, 0.f);
+        }
       }
+#pragma unroll
+      for (int k = 0; k < 16; ++k) {
+        const double d = (double)o[k].x - mean;
+        m2 += (double)o[k].y + d * d * ((double)max(min(p.HW - (j0 + k * L) * p.rows, p.rows), 0) * p.cg);
+      }
+    }
     m2 = lane_sum(m2, L);
     if (on && gl == 0) {
       gm[2 * g] = (float)(mean + (double)p.origin[(size_t)n * p.G + g]);
@@ -167,42 +218,81 @@ DEVINL void gn_join_stats(const GnP& p, int n, float* gm) {
   }
 }
 
+constexpr int GN_U = 4;    // rows a thread has in flight
+
 template <typename T, int V, int ACTC> __global__ __launch_bounds__(256) void gn_apply_kernel(const GnP p) {
   extern __shared__ float gm[];                // [G][2]
-  const int n = blockIdx.x / p.chunks, j = blockIdx.x % p.chunks;
+  // last chunk first: what the statistics read last is still in the last-level cache
+  const int blk = gridDim.x - 1 - blockIdx.x, n = blk / p.chunks, j = blk % p.chunks;
   const int r0 = j * p.rows, nr = min(p.HW - r0, p.rows);
   const int act = ACTC >= 0 ? ACTC : p.act;
+  const int cv = p.C / V, cols = min(cv, 256), rpb = 256 / cols;
+  const int tcol = threadIdx.x % cols, trow = threadIdx.x / cols;
+  const size_t row0 = (size_t)n * p.HW + r0;
+  typedef typename Lane<T, V>::raw raw_t;
+  raw_t rx[GN_U], rr[GN_U];
+  const bool rows_mine = trow < rpb;
+  // the first rows and the affine pair are requested in front of the join, so that its round trips to L2 run beside them
+  auto request = [&](const int col, const int r) {
+    const T* px = (const T*)p.x + row0 * p.x_ld + (size_t)col * V;
+    const T* pr = (const T*)p.res + row0 * p.r_ld + (size_t)col * V;
+#pragma unroll
+    for (int u = 0; u < GN_U; ++u)
+      if (r + u * rpb < nr) {
+        rx[u] = Lane<T, V>::get(px + (size_t)(r + u * rpb) * p.x_ld);
+        if (p.res) rr[u] = Lane<T, V>::get(pr + (size_t)(r + u * rpb) * p.r_ld);
+      }
+  };
+  float a[V], b[V], mu[V];
+  auto affine = [&](const int col) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      a[e] = p.gamma ? p.gamma[col * V + e] : 1.f;
+      b[e] = p.beta ? p.beta[col * V + e] : 0.f;
+    }
+  };
+  if (rows_mine) {
+    request(tcol, trow);
+    affine(tcol);
+  }
   gn_join_stats(p, n, gm);
   __syncthreads();
   if (j == 0)
     for (int t = threadIdx.x; t < 2 * p.G; t += 256) p.stats[(size_t)n * 2 * p.G + t] = gm[t];
-  const int cv = p.C / V, cols = min(cv, 256), rpb = 256 / cols;
-  const int tcol = threadIdx.x % cols, trow = threadIdx.x / cols;
-  if (trow >= rpb) return;
-  const size_t row0 = (size_t)n * p.HW + r0;
+  if (!rows_mine) return;
   for (int col = tcol; col < cv; col += cols) {
-    float mu[V], a[V], b[V];
+    if (col != tcol) {
+      request(col, trow);
+      affine(col);
+    }
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-      const int c = col * V + e, g = c / p.cg;
+      const int g = (col * V + e) / p.cg;
       mu[e] = gm[2 * g];
-      a[e] = gm[2 * g + 1] * (p.gamma ? p.gamma[c] : 1.f);
-      b[e] = p.beta ? p.beta[c] : 0.f;
+      a[e] *= gm[2 * g + 1];
     }
-    const T* px = (const T*)p.x + row0 * p.x_ld + (size_t)col * V;
-    const T* pr = p.res ? (const T*)p.res + row0 * p.r_ld + (size_t)col * V : nullptr;
     T* po = (T*)p.out + row0 * p.o_ld + (size_t)col * V;
-#pragma unroll 4
-    for (int r = trow; r < nr; r += rpb) {
-      float f[V], t[V];
-      Lane<T, V>::load(px + (size_t)r * p.x_ld, f);
-      if (pr) Lane<T, V>::load(pr + (size_t)r * p.r_ld, t);
+    for (int r = trow; r < nr; r += GN_U * rpb) {
+      raw_t cx[GN_U], cr[GN_U];
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        f[e] = actf<Vec<T>::precise>(fmaf(f[e] - mu[e], a[e], b[e]), act);
-        if (pr) f[e] += t[e];
+      for (int u = 0; u < GN_U; ++u) {
+        cx[u] = rx[u];
+        cr[u] = rr[u];
       }
-      Lane<T, V>::store(po + (size_t)r * p.o_ld, f);
+      request(col, r + GN_U * rpb);
+#pragma unroll
+      for (int u = 0; u < GN_U; ++u)
+        if (r + u * rpb < nr) {
+          float f[V], t[V];
+          Lane<T, V>::cvt(cx[u], f);
+          if (p.res) Lane<T, V>::cvt(cr[u], t);
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            f[e] = gn_act<Vec<T>::precise>(fmaf(f[e] - mu[e], a[e], b[e]), act);
+            if (p.res) f[e] += t[e];
+          }
+          Lane<T, V>::store(po + (size_t)(r + u * rpb) * p.o_ld, f);
+        }
     }
   }
 }
@@ -229,27 +319,27 @@ template <typename T, int V, int ACTC> __global__ __launch_bounds__(256) void gn
         const int c = col * V + e, g = c / p.cg;
         mu[e] = st[2 * g];
         rs[e] = st[2 * g + 1];
-        ga[e] = p.gamma ? p.gamma[c] : 1.f;
+        ga[e] = rs[e] * (p.gamma ? p.gamma[c] : 1.f);
         be[e] = p.beta ? p.beta[c] : 0.f;
         sa[e] = sb[e] = 0.f;
       }
       const T* px = (const T*)p.x + row0 * p.x_ld + (size_t)col * V;
       const T* pd = (const T*)p.dout + row0 * p.d_ld + (size_t)col * V;
-#pragma unroll 2
+#pragma unroll 4
       for (int r = trow; r < nr; r += rpb) {
         float f[V], d[V];
-        Lane<T, V>::load(px + (size_t)r * p.x_ld, f);
-        Lane<T, V>::load(pd + (size_t)r * p.d_ld, d);
+        lane_load<T, V>(px + (size_t)r * p.x_ld, f);
+        lane_load<T, V>(pd + (size_t)r * p.d_ld, d);
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-          const float xh = (f[e] - mu[e]) * rs[e];
-          const float du = d[e] * act_grad<Vec<T>::precise>(fmaf(ga[e], xh, be[e]), act);
+          const float c = f[e] - mu[e];                     // xh = rs c
+          const float du = d[e] * gn_act_grad<Vec<T>::precise>(fmaf(ga[e], c, be[e]), act);
           sa[e] += du;
-          sb[e] = fmaf(du, xh, sb[e]);
+          sb[e] = fmaf(du, c, sb[e]);
         }
       }
 #pragma unroll
-      for (int e = 0; e < V; ++e) red[(trow * cols + tcol) * V + e] = make_float2(sa[e], sb[e]);
+      for (int e = 0; e < V; ++e) red[(trow * cols + tcol) * V + e] = make_float2(sa[e], sb[e] * rs[e]);
     }
     __syncthreads();
     const int nch = min(cols, cv - cb) * V;
@@ -284,35 +374,42 @@ template <typename T, int V, int ACTC> __global__ __launch_bounds__(256) void gn
 
 constexpr int GN_PC = 32;    // channels per parameter workgroup
 
+// dgamma / dbeta of GN_PC channels from `parts` per-channel partials, in a fixed order (256 threads)
+DEVINL void gn_params(const GnP& p, int block, size_t parts) {
+  __shared__ double da[256], db[256];
+  const int c = block * GN_PC + threadIdx.x % GN_PC, lane = threadIdx.x / GN_PC;
+  double a = 0.0, b = 0.0;
+  if (c < p.C) {
+#pragma unroll 8
+    for (size_t i = lane; i < parts; i += 256 / GN_PC) {
+      const float2 o = p.cpart[i * p.C + c];
+      a += (double)o.x;
+      b += (double)o.y;
+    }
+  }
+  da[threadIdx.x] = a;
+  db[threadIdx.x] = b;
+  __syncthreads();
+  if (lane == 0 && c < p.C) {
+    for (int w = 1; w < 256 / GN_PC; ++w) {
+      a += da[w * GN_PC + threadIdx.x];
+      b += db[w * GN_PC + threadIdx.x];
+    }
+    if (p.dbeta) p.dbeta[c] = (float)(a + (p.acc_par ? (double)p.dbeta[c] : 0.0));
+    if (p.dgamma) p.dgamma[c] = (float)(b + (p.acc_par ? (double)p.dgamma[c] : 0.0));
+  }
+}
+__global__ __launch_bounds__(256) void gn_params_kernel(const GnP p) { gn_params(p, blockIdx.x, (size_t)p.N); }
+
 // workgroups [0, npar): dgamma / dbeta of GN_PC channels, summed over all chunks in a fixed order; the others: dx of one chunk of rows
 template <typename T, int V, int ACTC> __global__ __launch_bounds__(256) void gn_bwd_dx_kernel(const GnP p, const int npar) {
   extern __shared__ float gm[];                // [G][2]: the two means of the group
   const int act = ACTC >= 0 ? ACTC : p.act;
   if ((int)blockIdx.x < npar) {
-    const int c = blockIdx.x * GN_PC + threadIdx.x % GN_PC, lane = threadIdx.x / GN_PC;
-    double a = 0.0, b = 0.0;
-    const size_t parts = (size_t)p.N * p.chunks;
-    if (c < p.C)
-      for (size_t i = lane; i < parts; i += 256 / GN_PC) {
-        const float2 o = p.cpart[i * p.C + c];
-        a += (double)o.x;
-        b += (double)o.y;
-      }
-    __shared__ double da[256], db[256];
-    da[threadIdx.x] = a;
-    db[threadIdx.x] = b;
-    __syncthreads();
-    if (lane == 0 && c < p.C) {
-      for (int w = 1; w < 256 / GN_PC; ++w) {
-        a += da[w * GN_PC + threadIdx.x];
-        b += db[w * GN_PC + threadIdx.x];
-      }
-      if (p.dbeta) p.dbeta[c] = (float)(a + (p.acc_par ? (double)p.dbeta[c] : 0.0));
-      if (p.dgamma) p.dgamma[c] = (float)(b + (p.acc_par ? (double)p.dgamma[c] : 0.0));
-    }
+    gn_params(p, blockIdx.x, (size_t)p.N * p.chunks);
     return;
   }
-  const int blk = blockIdx.x - npar, n = blk / p.chunks, j = blk % p.chunks;
+  const int blk = gridDim.x - 1 - blockIdx.x, n = blk / p.chunks, j = blk % p.chunks;      // last chunk first, as in gn_apply_kernel
   const int r0 = j * p.rows, nr = min(p.HW - r0, p.rows);
   {
     const int L = join_lanes(p.G), gl = threadIdx.x % L, gstep = 256 / L;
@@ -321,12 +418,16 @@ template <typename T, int V, int ACTC> __global__ __launch_bounds__(256) void gn
     for (int g0 = 0; g0 < p.G; g0 += gstep) {
       const int g = g0 + threadIdx.x / L;
       double a = 0.0, b = 0.0;
-      if (g < p.G)
-        for (int i = gl; i < p.chunks; i += L) {
-          const float2 o = part[(size_t)i * p.G + g];
-          a += (double)o.x;
-          b += (double)o.y;
+      for (int j0 = gl; j0 < p.chunks; j0 += 16 * L) {
+        float2 o[16];
+#pragma unroll
+        for (int k = 0; k < 16; ++k) o[k] = (g < p.G && j0 + k * L < p.chunks) ? part[(size_t)(j0 + k * L) * p.G + g] : make_float2(0.f, 0.f);
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+          a += (double)o[k].x;
+          b += (double)o[k].y;
         }
+      }
       a = lane_sum(a, L);
       b = lane_sum(b, L);
       if (g < p.G && gl == 0) {
@@ -342,31 +443,31 @@ template <typename T, int V, int ACTC> __global__ __launch_bounds__(256) void gn
   const size_t row0 = (size_t)n * p.HW + r0;
   const float* st = p.stats + (size_t)n * 2 * p.G;
   for (int col = tcol; col < cv; col += cols) {
-    float mu[V], rs[V], ga[V], be[V], m1[V], m2[V];
+    float mu[V], ga[V], be[V], k0[V], k1[V];      // dx = (rs gamma) du + k0 + k1 c with c = x - mean
 #pragma unroll
     for (int e = 0; e < V; ++e) {
       const int c = col * V + e, g = c / p.cg;
+      const float rs = st[2 * g + 1];
       mu[e] = st[2 * g];
-      rs[e] = st[2 * g + 1];
-      ga[e] = p.gamma ? p.gamma[c] : 1.f;
+      ga[e] = rs * (p.gamma ? p.gamma[c] : 1.f);
       be[e] = p.beta ? p.beta[c] : 0.f;
-      m1[e] = gm[2 * g];
-      m2[e] = gm[2 * g + 1];
+      k0[e] = -rs * gm[2 * g];
+      k1[e] = -rs * rs * gm[2 * g + 1];
     }
     const T* px = (const T*)p.x + row0 * p.x_ld + (size_t)col * V;
     const T* pd = (const T*)p.dout + row0 * p.d_ld + (size_t)col * V;
     T* po = (T*)p.out + row0 * p.o_ld + (size_t)col * V;
-#pragma unroll 2
+#pragma unroll 4
     for (int r = trow; r < nr; r += rpb) {
       float f[V], d[V], o[V];
-      Lane<T, V>::load(px + (size_t)r * p.x_ld, f);
-      Lane<T, V>::load(pd + (size_t)r * p.d_ld, d);
-      if (p.acc_dx) Lane<T, V>::load(po + (size_t)r * p.o_ld, o);
+      lane_load<T, V>(px + (size_t)r * p.x_ld, f);
+      lane_load<T, V>(pd + (size_t)r * p.d_ld, d);
+      if (p.acc_dx) lane_load<T, V>(po + (size_t)r * p.o_ld, o);
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        const float xh = (f[e] - mu[e]) * rs[e];
-        const float v = ga[e] * d[e] * act_grad<Vec<T>::precise>(fmaf(ga[e], xh, be[e]), act);
-        const float g = rs[e] * (v - m1[e] - xh * m2[e]);
+        const float c = f[e] - mu[e];
+        const float du = d[e] * gn_act_grad<Vec<T>::precise>(fmaf(ga[e], c, be[e]), act);
+        const float g = fmaf(ga[e], du, fmaf(k1[e], c, k0[e]));
         d[e] = p.acc_dx ? o[e] + g : g;
       }
       Lane<T, V>::store(po + (size_t)r * p.o_ld, d);
@@ -374,12 +475,284 @@ template <typename T, int V, int ACTC> __global__ __launch_bounds__(256) void gn
   }
 }
 
+// ------------------------------------------------------------------------------------------------ resident slices
+// One workgroup = (image, slice of sv vectors that hold whole groups); thread t owns vector column t % sv and rows t / sv + i * rpb, i < NV, as
+// raw vectors in registers.  Slices of one image share 128-byte lines, so they get neighbouring ids on one XCD (its L2 serves the line's
+// other readers).
+constexpr int RES_NT = 512;
+
+struct ResP {
+  GnP g;
+  int sv, slices, rpb;     // vectors per slice, slices per image, rows per pass of the workgroup
+};
+
+DEVINL int xcd_contiguous(int id, int n) {      // hardware deals workgroup ids round robin over the 8 XCDs: give each a contiguous range
+  const int q = n >> 3, r = n & 7, x = id & 7;
+  return (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + (id >> 3);
+}
+
+// lanes that share the reduction of one of n items: a power of two, whole waves at most
+DEVINL int res_lanes(int n) {
+  int l = 64;
+  while (l > 1 && l * n > RES_NT) l >>= 1;
+  return l;
+}
+
+template <typename T, int V, int NV, int ACTC> __global__ __launch_bounds__(RES_NT) void gn_res_fwd_kernel(const ResP q) {
+  const GnP& p = q.g;
+  __shared__ float2 red[V * RES_NT];           // [channel of the vector][thread]: (mean, M2) of the thread's values
+  extern __shared__ float2 chan[];             // [channels of the slice] (mean - origin, M2), behind them [groups][2] mean, rstd
+  float* gm = (float*)(chan + q.sv * V);
+  const int id = xcd_contiguous(blockIdx.x, gridDim.x), n = id / q.slices, c0 = (id % q.slices) * q.sv * V;
+  const int tid = threadIdx.x, col = tid % q.sv, row = tid / q.sv, act = ACTC >= 0 ? ACTC : p.act;
+  const bool on = row < q.rpb;
+  const T* px = (const T*)p.x + (size_t)n * p.HW * p.x_ld + c0 + (size_t)col * V;
+  typename Lane<T, V>::raw raw[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int r = row + i * q.rpb;
+    if (on && r < p.HW) raw[i] = Lane<T, V>::get(px + (size_t)r * p.x_ld);
+  }
+  const int per = p.HW / q.rpb, extra = p.HW % q.rpb;      // rows of a row lane: per, one more in the first `extra` lanes
+  const int cnt = on ? per + (row < extra ? 1 : 0) : 0;
+  {
+    float s[V], k[V], m2[V], f[V];
+    if (cnt > 0) Lane<T, V>::cvt(raw[0], k);
+#pragma unroll
+    for (int e = 0; e < V; ++e) s[e] = m2[e] = 0.f;
+#pragma unroll
+    for (int i = 1; i < NV; ++i)
+      if (i < cnt) {
+        Lane<T, V>::cvt(raw[i], f);
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          const float d = f[e] - k[e];
+          s[e] += d;
+          m2[e] = fmaf(d, d, m2[e]);
+        }
+      }
+    const float inv = cnt > 0 ? 1.0f / (float)cnt : 0.f;
+    if (cnt > 0) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const float o = gn_origin<T>(p, n, (c0 + col * V + e) / p.cg), v = m2[e] - s[e] * s[e] * inv;
+        red[e * RES_NT + tid] = make_float2((k[e] - o) + s[e] * inv, v < 0.f ? 0.f : v);
+      }
+    }
+  }
+  __syncthreads();
+  // row lanes -> channels (a channel's partials are res_lanes(nch) lanes' work, about V each) -> groups
+  const int nch = q.sv * V, nrow = min(q.rpb, p.HW);
+  {
+    const int L = res_lanes(nch), lane = tid % L;
+    for (int k = 0; k < nch; k += RES_NT / L) {
+      const int c = k + tid / L;
+      const bool live = c < nch;
+      const float2* e = red + (live ? (c % V) * RES_NT + c / V : 0);
+      float mean = 0.f, m2 = 0.f;
+      if (live)
+        for (int r = lane; r < nrow; r += L) mean = fmaf(e[r * q.sv].x, (float)(per + (r < extra ? 1 : 0)), mean);
+      mean = lane_sum(mean, L) / (float)p.HW;
+      if (live)
+        for (int r = lane; r < nrow; r += L) {
+          const float2 o = e[r * q.sv];
+          const float d = o.x - mean;
+          m2 += fmaf(d * d, (float)(per + (r < extra ? 1 : 0)), o.y);
+        }
+      m2 = lane_sum(m2, L);
+      if (live && lane == 0) chan[c] = make_float2(mean, m2);
+    }
+  }
+  __syncthreads();
+  const int gs = nch / p.cg;
+  {
+    const int L = res_lanes(gs), lane = tid % L;
+    for (int k = 0; k < gs; k += RES_NT / L) {
+      const int g = k + tid / L;
+      const bool live = g < gs;
+      float mean = 0.f, m2 = 0.f;
+      if (live)
+        for (int c = g * p.cg + lane; c < (g + 1) * p.cg; c += L) mean += chan[c].x;
+      mean = lane_sum(mean, L) / (float)p.cg;
+      if (live)
+        for (int c = g * p.cg + lane; c < (g + 1) * p.cg; c += L) {
+          const float d = chan[c].x - mean;
+          m2 += fmaf(d * d, (float)p.HW, chan[c].y);
+        }
+      m2 = lane_sum(m2, L);
+      if (live && lane == 0) {
+        const int gg = c0 / p.cg + g;
+        const float mu = (float)((double)mean + (double)gn_origin<T>(p, n, gg));
+        const float rs = (float)(1.0 / sqrt((double)m2 / ((double)p.HW * p.cg) + (double)p.eps));
+        gm[2 * g] = mu;
+        gm[2 * g + 1] = rs;
+        p.stats[((size_t)n * p.G + gg) * 2] = mu;
+        p.stats[((size_t)n * p.G + gg) * 2 + 1] = rs;
+      }
+    }
+  }
+  __syncthreads();
+  if (cnt == 0) return;
+  float mu[V], a[V], b[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    const int c = c0 + col * V + e, g = (col * V + e) / p.cg;
+    mu[e] = gm[2 * g];
+    a[e] = gm[2 * g + 1] * (p.gamma ? p.gamma[c] : 1.f);
+    b[e] = p.beta ? p.beta[c] : 0.f;
+  }
+  const size_t row0 = (size_t)n * p.HW + row;
+  const T* pr = p.res ? (const T*)p.res + row0 * p.r_ld + c0 + (size_t)col * V : nullptr;
+  T* po = (T*)p.out + row0 * p.o_ld + c0 + (size_t)col * V;
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+    if (i < cnt) {
+      float f[V], t[V];
+      Lane<T, V>::cvt(raw[i], f);
+      if (pr) lane_load<T, V>(pr + (size_t)i * q.rpb * p.r_ld, t);
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        f[e] = gn_act<Vec<T>::precise>(fmaf(f[e] - mu[e], a[e], b[e]), act);
+        if (pr) f[e] += t[e];
+      }
+      Lane<T, V>::store(po + (size_t)i * q.rpb * p.o_ld, f);
+    }
+}
+
+template <typename T, int V, int NV, int ACTC> __global__ __launch_bounds__(RES_NT) void gn_res_bwd_kernel(const ResP q) {
+  const GnP& p = q.g;
+  __shared__ float2 red[V * RES_NT];           // (sum du, sum du c) of the thread's rows, then [channel] totals
+  extern __shared__ float2 chan[];             // [channels of the slice] (sum du, sum du xh), behind them [groups][2] means
+  const int id = xcd_contiguous(blockIdx.x, gridDim.x), n = id / q.slices, nch = q.sv * V, c0 = (id % q.slices) * nch;
+  float2* gmean = chan + nch;
+  const int tid = threadIdx.x, col = tid % q.sv, row = tid / q.sv, act = ACTC >= 0 ? ACTC : p.act;
+  const int cnt = row < q.rpb ? p.HW / q.rpb + (row < p.HW % q.rpb ? 1 : 0) : 0;
+  const size_t row0 = (size_t)n * p.HW + row;
+  const T* px = (const T*)p.x + row0 * p.x_ld + c0 + (size_t)col * V;
+  const T* pd = (const T*)p.dout + row0 * p.d_ld + c0 + (size_t)col * V;
+  typename Lane<T, V>::raw rx[NV], rd[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+    if (i < cnt) {
+      rx[i] = Lane<T, V>::get(px + (size_t)i * q.rpb * p.x_ld);
+      rd[i] = Lane<T, V>::get(pd + (size_t)i * q.rpb * p.d_ld);
+    }
+  const float* st = p.stats + ((size_t)n * p.G + c0 / p.cg) * 2;
+  float mu[V], ga[V], be[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    const int c = c0 + col * V + e, g = (col * V + e) / p.cg;
+    mu[e] = st[2 * g];
+    ga[e] = st[2 * g + 1] * (p.gamma ? p.gamma[c] : 1.f);
+    be[e] = p.beta ? p.beta[c] : 0.f;
+  }
+  {
+    float sa[V], sb[V], f[V], d[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) sa[e] = sb[e] = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (i < cnt) {
+        Lane<T, V>::cvt(rx[i], f);
+        Lane<T, V>::cvt(rd[i], d);
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          const float c = f[e] - mu[e];
+          const float du = d[e] * gn_act_grad<Vec<T>::precise>(fmaf(ga[e], c, be[e]), act);
+          sa[e] += du;
+          sb[e] = fmaf(du, c, sb[e]);
+        }
+      }
+    if (cnt > 0) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) red[e * RES_NT + tid] = make_float2(sa[e], sb[e]);
+    }
+  }
+  __syncthreads();
+  const int nrow = min(q.rpb, p.HW);
+  {
+    const int L = res_lanes(nch), lane = tid % L;
+    for (int k = 0; k < nch; k += RES_NT / L) {
+      const int c = k + tid / L;
+      const bool live = c < nch;
+      const float2* e = red + (live ? (c % V) * RES_NT + c / V : 0);
+      float a = 0.f, b = 0.f;
+      if (live)
+        for (int r = lane; r < nrow; r += L) {
+          const float2 o = e[r * q.sv];
+          a += o.x;
+          b += o.y;
+        }
+      a = lane_sum(a, L);
+      b = lane_sum(b, L);
+      if (live && lane == 0) {
+        b *= st[2 * (c / p.cg) + 1];
+        chan[c] = make_float2(a, b);
+        if (p.N > 1) {
+          p.cpart[(size_t)n * p.C + c0 + c] = make_float2(a, b);
+        } else {
+          if (p.dbeta) p.dbeta[c0 + c] = a + (p.acc_par ? p.dbeta[c0 + c] : 0.f);
+          if (p.dgamma) p.dgamma[c0 + c] = b + (p.acc_par ? p.dgamma[c0 + c] : 0.f);
+        }
+      }
+    }
+  }
+  __syncthreads();
+  const int gs = nch / p.cg;
+  {
+    const int L = res_lanes(gs), lane = tid % L;
+    for (int k = 0; k < gs; k += RES_NT / L) {
+      const int g = k + tid / L;
+      float a = 0.f, b = 0.f;
+      if (g < gs)
+        for (int c = g * p.cg + lane; c < (g + 1) * p.cg; c += L) {
+          const float w = p.gamma ? p.gamma[c0 + c] : 1.f;
+          a = fmaf(w, chan[c].x, a);
+          b = fmaf(w, chan[c].y, b);
+        }
+      a = lane_sum(a, L);
+      b = lane_sum(b, L);
+      if (g < gs && lane == 0) {
+        const double inv = 1.0 / ((double)p.HW * p.cg);
+        gmean[g] = make_float2((float)(a * inv), (float)(b * inv));
+      }
+    }
+  }
+  __syncthreads();
+  if (cnt == 0) return;
+  float k0[V], k1[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    const int g = (col * V + e) / p.cg;
+    const float rs = st[2 * g + 1];
+    k0[e] = -rs * gmean[g].x;
+    k1[e] = -rs * rs * gmean[g].y;
+  }
+  T* po = (T*)p.out + row0 * p.o_ld + c0 + (size_t)col * V;
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+    if (i < cnt) {
+      float f[V], d[V], o[V];
+      Lane<T, V>::cvt(rx[i], f);
+      Lane<T, V>::cvt(rd[i], d);
+      if (p.acc_dx) lane_load<T, V>(po + (size_t)i * q.rpb * p.o_ld, o);
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const float c = f[e] - mu[e];
+        const float du = d[e] * gn_act_grad<Vec<T>::precise>(fmaf(ga[e], c, be[e]), act);
+        const float g = fmaf(ga[e], du, fmaf(k1[e], c, k0[e]));
+        d[e] = p.acc_dx ? o[e] + g : g;
+      }
+      Lane<T, V>::store(po + (size_t)i * q.rpb * p.o_ld, d);
+    }
+}
+
 // ------------------------------------------------------------------------------------------------ host side
-// Row chunks of one image.  A function of the descriptor's sizes alone, so that the workspace does not depend on addresses: about eight
+// Row chunks of one image.  A function of the descriptor's sizes alone, so that the workspace does not depend on addresses: about four
 // workgroups per compute unit over the whole batch, and at least 8192 values per chunk.
 void gn_chunks(const plyolo_gn_desc* d, int* chunks, int* rows) {
   const int64_t all = (int64_t)d->N * d->HW;
-  int64_t r = (all + 2047) / 2048;
+  int64_t r = (all + 1023) / 1024;
   const int64_t least = (8192 + d->C - 1) / d->C;
   if (r < least) r = least;
   if (r > d->HW) r = d->HW;
@@ -417,10 +790,42 @@ GnP gn_params(const plyolo_gn_desc* d, void* ws) {
   return p;
 }
 
+// The resident split of the descriptor, or nv = 0 where no slice fits.  A slice is a multiple of the least run of vectors that holds whole
+// groups; it grows towards 128-byte row pieces as long as the batch still gives every compute unit a workgroup and the rows fit the
+// registers (NV vectors a thread; the backward holds two operands and takes half).
+struct ResPlan { int sv, slices, rpb, nv; };
+ResPlan res_plan(const plyolo_gn_desc* d, int V, int max_nv) {
+  ResPlan r{};
+  const int cg = d->C / d->groups;
+  int least = 1;
+  while ((least * V) % cg != 0 && least * V < d->C) ++least;
+  const int cv = d->C / V;
+  if (least * V > 2048 || least > RES_NT || cv % least != 0) return r;      // (LDS: two floats per channel of the slice)
+  const int esz = V == 1 ? 8 : 1;                     // element lanes: count eight of them as a vector
+  for (int sv = least; sv <= cv && sv <= 8 * esz + least; sv += least) {
+    if (cv % sv != 0 || sv > RES_NT) continue;
+    const int rpb = RES_NT / sv, nv = (d->HW + rpb - 1) / rpb;
+    if (nv > max_nv) break;
+    if (sv > least && (int64_t)d->N * (cv / sv) < 256) break;
+    r.sv = sv; r.slices = cv / sv; r.rpb = rpb; r.nv = nv;
+  }
+  return r;
+}
+
+#define GN_RES_FWD(T, V, nv, ACT)                                                                      \
+  ((nv) <= 2 ? gn_res_fwd_kernel<T, V, 2, ACT> : (nv) <= 4 ? gn_res_fwd_kernel<T, V, 4, ACT>           \
+   : (nv) <= 8 ? gn_res_fwd_kernel<T, V, 8, ACT> : (nv) <= 16 ? gn_res_fwd_kernel<T, V, 16, ACT> : gn_res_fwd_kernel<T, V, 32, ACT>)
+#define GN_RES_BWD(T, V, nv, ACT) \
+  ((nv) <= 2 ? gn_res_bwd_kernel<T, V, 2, ACT> : (nv) <= 4 ? gn_res_bwd_kernel<T, V, 4, ACT> : gn_res_bwd_kernel<T, V, 8, ACT>)
+#define GN_RES_DISPATCH(dtype, wide, act, NAME, KERN, nv)                                                                                   \
+  ((dtype) == PLYOLO_BF16 ? ((wide) ? ((act) == PLYOLO_ACT_SILU ? NAME(bf16_t, 8, nv, PLYOLO_ACT_SILU) : NAME(bf16_t, 8, nv, -1))            \
+                                    : KERN<bf16_t, 1, 16, -1>)                                                                             \
+                          : ((wide) ? NAME(float, 4, nv, -1) : KERN<float, 1, 16, -1>))
+
 #define GN_DISPATCH(dtype, wide, act, KERN)                                                                                     \
   ((dtype) == PLYOLO_BF16 ? ((wide) ? ((act) == PLYOLO_ACT_SILU ? KERN<bf16_t, 8, PLYOLO_ACT_SILU> : KERN<bf16_t, 8, -1>)         \
                                     : KERN<bf16_t, 1, -1>)                                                                      \
-                          : ((wide) ? ((act) == PLYOLO_ACT_SILU ? KERN<float, 4, PLYOLO_ACT_SILU> : KERN<float, 4, -1>) : KERN<float, 1, -1>))
+                          : ((wide) ? KERN<float, 4, -1> : KERN<float, 1, -1>))
 
 }  // namespace
 
@@ -442,8 +847,20 @@ int plyolo_gn_act_fwd(const plyolo_gn_desc* d, const void* x, const float* gamma
   GnP p = gn_params(d, workspace);
   p.x = x; p.res = res; p.out = out; p.gamma = gamma; p.beta = beta; p.stats = stats; p.o_ld = d->o_ld;
   const int V = d->dtype == PLYOLO_BF16 ? 8 : 4, dtype = d->dtype, act = d->act;
-  const bool wide = d->C % V == 0 && d->x_ld % V == 0 && d->o_ld % V == 0 && (!res || d->r_ld % V == 0) && ((size_t)x | (size_t)out | (size_t)res) % 16 == 0;
+  const bool wide = d->C % V == 0;
   plyolo::annotate("gn_act_fwd", 0.0, (double)p.N * p.HW * p.C * es * (res ? 3.0 : 2.0));
+  const ResPlan rp = res_plan(d, wide ? V : 1, wide ? 32 : 16);
+  if (rp.nv) {
+    ResP q{};
+    q.g = p; q.sv = rp.sv; q.slices = rp.slices; q.rpb = rp.rpb;
+    const int nch = rp.sv * (wide ? V : 1);
+    const size_t lds = (size_t)(nch + nch / p.cg) * sizeof(float2);
+    return plyolo::submit(stream, [=](hipStream_t s) -> hipError_t {
+      auto k = GN_RES_DISPATCH(dtype, wide, act, GN_RES_FWD, gn_res_fwd_kernel, rp.nv);
+      hipLaunchKernelGGL(k, dim3((unsigned)p.N * rp.slices), dim3(RES_NT), lds, s, q);
+      return hipGetLastError();
+    });
+  }
   return plyolo::submit(stream, [=](hipStream_t s) -> hipError_t {
     const dim3 grid((unsigned)p.N * p.chunks), blk(256);
     auto ks = dtype == PLYOLO_BF16 ? (wide ? gn_stats_kernel<bf16_t, 8> : gn_stats_kernel<bf16_t, 1>) : (wide ? gn_stats_kernel<float, 4> : gn_stats_kernel<float, 1>);
@@ -471,8 +888,21 @@ int plyolo_gn_act_bwd(const plyolo_gn_desc* d, const void* dout, int d_ld, const
   p.x = x; p.dout = dout; p.out = dx; p.gamma = gamma; p.beta = beta; p.stats = (float*)stats;
   p.dgamma = dgamma; p.dbeta = dbeta; p.d_ld = d_ld; p.o_ld = dx_ld; p.acc_dx = accumulate_dx ? 1 : 0; p.acc_par = accumulate_params ? 1 : 0;
   const int V = d->dtype == PLYOLO_BF16 ? 8 : 4, dtype = d->dtype, act = d->act;
-  const bool wide = d->C % V == 0 && d->x_ld % V == 0 && d_ld % V == 0 && dx_ld % V == 0 && ((size_t)x | (size_t)dout | (size_t)dx) % 16 == 0;
+  const bool wide = d->C % V == 0;
   plyolo::annotate("gn_act_bwd", 0.0, (double)p.N * p.HW * p.C * es * (accumulate_dx ? 4.0 : 3.0));
+  const ResPlan rp = res_plan(d, wide ? V : 1, wide ? 8 : 16);
+  if (rp.nv) {
+    ResP q{};
+    q.g = p; q.sv = rp.sv; q.slices = rp.slices; q.rpb = rp.rpb;
+    const int nch = rp.sv * (wide ? V : 1);
+    const size_t lds = (size_t)(nch + nch / p.cg) * sizeof(float2);
+    return plyolo::submit(stream, [=](hipStream_t s) -> hipError_t {
+      auto k = GN_RES_DISPATCH(dtype, wide, act, GN_RES_BWD, gn_res_bwd_kernel, rp.nv);
+      hipLaunchKernelGGL(k, dim3((unsigned)p.N * rp.slices), dim3(RES_NT), lds, s, q);
+      if (p.N > 1 && (p.dgamma || p.dbeta)) hipLaunchKernelGGL(gn_params_kernel, dim3((unsigned)((p.C + GN_PC - 1) / GN_PC)), dim3(256), 0, s, p);
+      return hipGetLastError();
+    });
+  }
   return plyolo::submit(stream, [=](hipStream_t s) -> hipError_t {
     const unsigned nblk = (unsigned)p.N * p.chunks;
     const int npar = (p.dgamma || p.dbeta) ? (p.C + GN_PC - 1) / GN_PC : 0;
