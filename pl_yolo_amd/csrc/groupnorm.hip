@@ -183,13 +183,14 @@ DEVINL void gn_join_stats(const GnP& p, int n, float* gm) {
   for (int g0 = 0; g0 < p.G; g0 += gstep) {
     const int g = g0 + threadIdx.x / L;
     const bool on = g < p.G;
+    const int gc = min(g, p.G - 1);
     float2 o[16];
     double sm = 0.0;
     for (int j0 = gl; j0 < p.chunks; j0 += 16 * L) {
 #pragma unroll
       for (int k = 0; k < 16; ++k) {
         const int j = j0 + k * L;
-        o[k] = (on && j < p.chunks) ? part[(size_t)j * p.G + g] : make_float2(0.f, 0.f);
+        o[k] = part[min(j, p.chunks - 1) * p.G + gc];       // (no branch around a request: a chunk beyond the last has no rows, weight 0)
       }
 #pragma unroll
       for (int k = 0; k < 16; ++k) sm += (double)o[k].x * (double)max(min(p.HW - (j0 + k * L) * p.rows, p.rows), 0);
@@ -201,13 +202,14 @@ DEVINL void gn_join_stats(const GnP& p, int n, float* gm) {
 #pragma unroll
         for (int k = 0; k < 16; ++k) {
           const int j = j0 + k * L;
-          o[k] = (on && j < p.chunks) ? part[(size_t)j * p.G + g] : make_float2(0.f, 0.f);
+          o[k] = part[min(j, p.chunks - 1) * p.G + gc];
         }
       }
 #pragma unroll
       for (int k = 0; k < 16; ++k) {
         const double d = (double)o[k].x - mean;
-        m2 += (double)o[k].y + d * d * ((double)max(min(p.HW - (j0 + k * L) * p.rows, p.rows), 0) * p.cg);
+        const double m = (double)o[k].y + d * d * ((double)min(p.HW - (j0 + k * L) * p.rows, p.rows) * p.cg);
+        m2 += j0 + k * L < p.chunks ? m : 0.0;
       }
     }
     m2 = lane_sum(m2, L);
@@ -298,6 +300,18 @@ template <typename T, int V, int ACTC> __global__ __launch_bounds__(256) void gn
 }
 
 // ------------------------------------------------------------------------------------------------ backward
+constexpr int GN_BU = 2;   // rows of x and dout a thread has in flight
+
+template <typename T, int V>
+DEVINL void gn_request(typename Lane<T, V>::raw (&rx)[GN_BU], typename Lane<T, V>::raw (&rd)[GN_BU], const T* px, const T* pd, const GnP& p, int r, int nr, int rpb) {
+#pragma unroll
+  for (int u = 0; u < GN_BU; ++u)
+    if (r + u * rpb < nr) {
+      rx[u] = Lane<T, V>::get(px + (size_t)(r + u * rpb) * p.x_ld);
+      rd[u] = Lane<T, V>::get(pd + (size_t)(r + u * rpb) * p.d_ld);
+    }
+}
+
 // per chunk: (sum du, sum du xh) of every channel, and (sum v, sum v xh) of every group
 template <typename T, int V, int ACTC> __global__ __launch_bounds__(256) void gn_bwd_sums_kernel(const GnP p) {
   extern __shared__ float2 chan[];
@@ -325,18 +339,29 @@ template <typename T, int V, int ACTC> __global__ __launch_bounds__(256) void gn
       }
       const T* px = (const T*)p.x + row0 * p.x_ld + (size_t)col * V;
       const T* pd = (const T*)p.dout + row0 * p.d_ld + (size_t)col * V;
-#pragma unroll 4
-      for (int r = trow; r < nr; r += rpb) {
-        float f[V], d[V];
-        lane_load<T, V>(px + (size_t)r * p.x_ld, f);
-        lane_load<T, V>(pd + (size_t)r * p.d_ld, d);
+      typename Lane<T, V>::raw rx[GN_BU], rd[GN_BU], cx[GN_BU], cd[GN_BU];
+      gn_request<T, V>(rx, rd, px, pd, p, trow, nr, rpb);
+      for (int r = trow; r < nr; r += GN_BU * rpb) {
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-          const float c = f[e] - mu[e];                     // xh = rs c
-          const float du = d[e] * gn_act_grad<Vec<T>::precise>(fmaf(ga[e], c, be[e]), act);
-          sa[e] += du;
-          sb[e] = fmaf(du, c, sb[e]);
+        for (int u = 0; u < GN_BU; ++u) {
+          cx[u] = rx[u];
+          cd[u] = rd[u];
         }
+        gn_request<T, V>(rx, rd, px, pd, p, r + GN_BU * rpb, nr, rpb);
+#pragma unroll
+        for (int u = 0; u < GN_BU; ++u)
+          if (r + u * rpb < nr) {
+            float f[V], d[V];
+            Lane<T, V>::cvt(cx[u], f);
+            Lane<T, V>::cvt(cd[u], d);
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+              const float c = f[e] - mu[e];                     // xh = rs c
+              const float du = d[e] * gn_act_grad<Vec<T>::precise>(fmaf(ga[e], c, be[e]), act);
+              sa[e] += du;
+              sb[e] = fmaf(du, c, sb[e]);
+            }
+          }
       }
 #pragma unroll
       for (int e = 0; e < V; ++e) red[(trow * cols + tcol) * V + e] = make_float2(sa[e], sb[e] * rs[e]);
@@ -421,11 +446,11 @@ template <typename T, int V, int ACTC> __global__ __launch_bounds__(256) void gn
       for (int j0 = gl; j0 < p.chunks; j0 += 16 * L) {
         float2 o[16];
 #pragma unroll
-        for (int k = 0; k < 16; ++k) o[k] = (g < p.G && j0 + k * L < p.chunks) ? part[(size_t)(j0 + k * L) * p.G + g] : make_float2(0.f, 0.f);
+        for (int k = 0; k < 16; ++k) o[k] = part[min(j0 + k * L, p.chunks - 1) * p.G + min(g, p.G - 1)];
 #pragma unroll
         for (int k = 0; k < 16; ++k) {
-          a += (double)o[k].x;
-          b += (double)o[k].y;
+          a += j0 + k * L < p.chunks ? (double)o[k].x : 0.0;
+          b += j0 + k * L < p.chunks ? (double)o[k].y : 0.0;
         }
       }
       a = lane_sum(a, L);
@@ -457,20 +482,31 @@ template <typename T, int V, int ACTC> __global__ __launch_bounds__(256) void gn
     const T* px = (const T*)p.x + row0 * p.x_ld + (size_t)col * V;
     const T* pd = (const T*)p.dout + row0 * p.d_ld + (size_t)col * V;
     T* po = (T*)p.out + row0 * p.o_ld + (size_t)col * V;
-#pragma unroll 4
-    for (int r = trow; r < nr; r += rpb) {
-      float f[V], d[V], o[V];
-      lane_load<T, V>(px + (size_t)r * p.x_ld, f);
-      lane_load<T, V>(pd + (size_t)r * p.d_ld, d);
-      if (p.acc_dx) lane_load<T, V>(po + (size_t)r * p.o_ld, o);
+    typename Lane<T, V>::raw rx[GN_BU], rd[GN_BU], cx[GN_BU], cd[GN_BU];
+    gn_request<T, V>(rx, rd, px, pd, p, trow, nr, rpb);
+    for (int r = trow; r < nr; r += GN_BU * rpb) {
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const float c = f[e] - mu[e];
-        const float du = d[e] * gn_act_grad<Vec<T>::precise>(fmaf(ga[e], c, be[e]), act);
-        const float g = fmaf(ga[e], du, fmaf(k1[e], c, k0[e]));
-        d[e] = p.acc_dx ? o[e] + g : g;
+      for (int u = 0; u < GN_BU; ++u) {
+        cx[u] = rx[u];
+        cd[u] = rd[u];
       }
-      Lane<T, V>::store(po + (size_t)r * p.o_ld, d);
+      gn_request<T, V>(rx, rd, px, pd, p, r + GN_BU * rpb, nr, rpb);
+#pragma unroll
+      for (int u = 0; u < GN_BU; ++u)
+        if (r + u * rpb < nr) {
+          float f[V], d[V], o[V];
+          Lane<T, V>::cvt(cx[u], f);
+          Lane<T, V>::cvt(cd[u], d);
+          if (p.acc_dx) lane_load<T, V>(po + (size_t)(r + u * rpb) * p.o_ld, o);
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            const float c = f[e] - mu[e];
+            const float du = d[e] * gn_act_grad<Vec<T>::precise>(fmaf(ga[e], c, be[e]), act);
+            const float g = fmaf(ga[e], du, fmaf(k1[e], c, k0[e]));
+            d[e] = p.acc_dx ? o[e] + g : g;
+          }
+          Lane<T, V>::store(po + (size_t)(r + u * rpb) * p.o_ld, d);
+        }
     }
   }
 }
@@ -748,8 +784,9 @@ template <typename T, int V, int NV, int ACTC> __global__ __launch_bounds__(RES_
 }
 
 // ------------------------------------------------------------------------------------------------ host side
-// Row chunks of one image.  A function of the descriptor's sizes alone, so that the workspace does not depend on addresses: about four
-// workgroups per compute unit over the whole batch, and at least 8192 values per chunk.
+// Row chunks of one image in the streaming launches.  A function of the descriptor's sizes alone, so that the workspace does not depend on
+// addresses: four workgroups per compute unit over the whole batch (with eight the joins cost more than they hide: backward of
+// 8 x 25600 x 320 bf16 171 instead of 150 us), and at least 8192 values per chunk.
 void gn_chunks(const plyolo_gn_desc* d, int* chunks, int* rows) {
   const int64_t all = (int64_t)d->N * d->HW;
   int64_t r = (all + 1023) / 1024;
@@ -776,7 +813,7 @@ int check_gn(const plyolo_gn_desc* d, const char* who) {
 size_t gn_ws_bytes(const plyolo_gn_desc* d) {
   int chunks, rows;
   gn_chunks(d, &chunks, &rows);
-  return (size_t)d->N * chunks * ((size_t)d->groups + d->C) * sizeof(float2) + (size_t)d->N * d->groups * sizeof(float);
+  return (size_t)d->N * (chunks * ((size_t)d->groups + d->C) * sizeof(float2) + d->groups * sizeof(float));
 }
 
 GnP gn_params(const plyolo_gn_desc* d, void* ws) {
@@ -790,11 +827,15 @@ GnP gn_params(const plyolo_gn_desc* d, void* ws) {
   return p;
 }
 
-// The resident split of the descriptor, or nv = 0 where no slice fits.  A slice is a multiple of the least run of vectors that holds whole
-// groups; it grows towards 128-byte row pieces as long as the batch still gives every compute unit a workgroup and the rows fit the
-// registers (NV vectors a thread; the backward holds two operands and takes half).
+// The resident split of the descriptor, or nv = 0 for the streaming launches.  A slice is a multiple of the least run of vectors that holds
+// whole groups; it grows towards 128-byte row pieces as long as the batch still gives every compute unit a workgroup and the rows fit the
+// registers (nv vectors a thread).  Measured, resident / streaming: the forward keeps its lead to the register limit when there are
+// workgroups to fill the chip (32 x 6400 x 128 bf16, nv 25: 41 / 48 us; 32 x 1600 x 256: 20 / 37), one image on a few workgroups loses it
+// beyond 12 vectors (1 x 6400 x 128, nv 13: 20 / 15).  The backward holds two operands and has nothing to hide narrow row pieces behind: 16
+// vectors in pieces of 64 bytes and more (32 x 1600 x 256, sv 4: 31 / 44; 16 x 1600 x 640, sv 5: 39 / 51), 8 in narrower ones
+// (32 x 6400 x 128, sv 1, nv 13: 91 / 72) and on few workgroups.
 struct ResPlan { int sv, slices, rpb, nv; };
-ResPlan res_plan(const plyolo_gn_desc* d, int V, int max_nv) {
+ResPlan res_plan(const plyolo_gn_desc* d, int V, bool bwd) {
   ResPlan r{};
   const int cg = d->C / d->groups;
   int least = 1;
@@ -804,9 +845,10 @@ ResPlan res_plan(const plyolo_gn_desc* d, int V, int max_nv) {
   const int esz = V == 1 ? 8 : 1;                     // element lanes: count eight of them as a vector
   for (int sv = least; sv <= cv && sv <= 8 * esz + least; sv += least) {
     if (cv % sv != 0 || sv > RES_NT) continue;
+    const int64_t wgs = (int64_t)d->N * (cv / sv);
     const int rpb = RES_NT / sv, nv = (d->HW + rpb - 1) / rpb;
-    if (nv > max_nv) break;
-    if (sv > least && (int64_t)d->N * (cv / sv) < 256) break;
+    if (nv > (V == 1 ? 16 : wgs < 64 ? (bwd ? 8 : 12) : bwd ? (sv >= 4 ? 16 : 8) : 32)) continue;
+    if (sv > least && wgs < 256) break;
     r.sv = sv; r.slices = cv / sv; r.rpb = rpb; r.nv = nv;
   }
   return r;
@@ -816,7 +858,8 @@ ResPlan res_plan(const plyolo_gn_desc* d, int V, int max_nv) {
   ((nv) <= 2 ? gn_res_fwd_kernel<T, V, 2, ACT> : (nv) <= 4 ? gn_res_fwd_kernel<T, V, 4, ACT>           \
    : (nv) <= 8 ? gn_res_fwd_kernel<T, V, 8, ACT> : (nv) <= 16 ? gn_res_fwd_kernel<T, V, 16, ACT> : gn_res_fwd_kernel<T, V, 32, ACT>)
 #define GN_RES_BWD(T, V, nv, ACT) \
-  ((nv) <= 2 ? gn_res_bwd_kernel<T, V, 2, ACT> : (nv) <= 4 ? gn_res_bwd_kernel<T, V, 4, ACT> : gn_res_bwd_kernel<T, V, 8, ACT>)
+  ((nv) <= 2 ? gn_res_bwd_kernel<T, V, 2, ACT> : (nv) <= 4 ? gn_res_bwd_kernel<T, V, 4, ACT>           \
+   : (nv) <= 8 ? gn_res_bwd_kernel<T, V, 8, ACT> : gn_res_bwd_kernel<T, V, 16, ACT>)
 #define GN_RES_DISPATCH(dtype, wide, act, NAME, KERN, nv)                                                                                   \
   ((dtype) == PLYOLO_BF16 ? ((wide) ? ((act) == PLYOLO_ACT_SILU ? NAME(bf16_t, 8, nv, PLYOLO_ACT_SILU) : NAME(bf16_t, 8, nv, -1))            \
                                     : KERN<bf16_t, 1, 16, -1>)                                                                             \
@@ -849,7 +892,7 @@ int plyolo_gn_act_fwd(const plyolo_gn_desc* d, const void* x, const float* gamma
   const int V = d->dtype == PLYOLO_BF16 ? 8 : 4, dtype = d->dtype, act = d->act;
   const bool wide = d->C % V == 0;
   plyolo::annotate("gn_act_fwd", 0.0, (double)p.N * p.HW * p.C * es * (res ? 3.0 : 2.0));
-  const ResPlan rp = res_plan(d, wide ? V : 1, wide ? 32 : 16);
+  const ResPlan rp = res_plan(d, wide ? V : 1, false);
   if (rp.nv) {
     ResP q{};
     q.g = p; q.sv = rp.sv; q.slices = rp.slices; q.rpb = rp.rpb;
@@ -862,14 +905,11 @@ int plyolo_gn_act_fwd(const plyolo_gn_desc* d, const void* x, const float* gamma
     });
   }
   return plyolo::submit(stream, [=](hipStream_t s) -> hipError_t {
-    const dim3 grid((unsigned)p.N * p.chunks), blk(256);
     auto ks = dtype == PLYOLO_BF16 ? (wide ? gn_stats_kernel<bf16_t, 8> : gn_stats_kernel<bf16_t, 1>) : (wide ? gn_stats_kernel<float, 4> : gn_stats_kernel<float, 1>);
-    const size_t lc = (size_t)p.C * sizeof(float2), lg = (size_t)p.G * sizeof(float2);
-    if (hipError_t e = plyolo::ensure_dynamic_lds((const void*)ks, lc); e != hipSuccess) return e;
-    hipLaunchKernelGGL(ks, grid, blk, lc, s, p);
     auto ka = GN_DISPATCH(dtype, wide, act, gn_apply_kernel);
-    if (hipError_t e = plyolo::ensure_dynamic_lds((const void*)ka, lg); e != hipSuccess) return e;
-    hipLaunchKernelGGL(ka, grid, blk, lg, s, p);
+    const dim3 grid((unsigned)p.N * p.chunks), blk(256);
+    hipLaunchKernelGGL(ks, grid, blk, (size_t)p.C * sizeof(float2), s, p);
+    hipLaunchKernelGGL(ka, grid, blk, (size_t)p.G * sizeof(float2), s, p);
     return hipGetLastError();
   });
 }
@@ -890,7 +930,7 @@ int plyolo_gn_act_bwd(const plyolo_gn_desc* d, const void* dout, int d_ld, const
   const int V = d->dtype == PLYOLO_BF16 ? 8 : 4, dtype = d->dtype, act = d->act;
   const bool wide = d->C % V == 0;
   plyolo::annotate("gn_act_bwd", 0.0, (double)p.N * p.HW * p.C * es * (accumulate_dx ? 4.0 : 3.0));
-  const ResPlan rp = res_plan(d, wide ? V : 1, wide ? 8 : 16);
+  const ResPlan rp = res_plan(d, wide ? V : 1, true);
   if (rp.nv) {
     ResP q{};
     q.g = p; q.sv = rp.sv; q.slices = rp.slices; q.rpb = rp.rpb;
@@ -904,16 +944,12 @@ int plyolo_gn_act_bwd(const plyolo_gn_desc* d, const void* dout, int d_ld, const
     });
   }
   return plyolo::submit(stream, [=](hipStream_t s) -> hipError_t {
+    auto ks = GN_DISPATCH(dtype, wide, act, gn_bwd_sums_kernel);
+    auto kd = GN_DISPATCH(dtype, wide, act, gn_bwd_dx_kernel);
     const unsigned nblk = (unsigned)p.N * p.chunks;
     const int npar = (p.dgamma || p.dbeta) ? (p.C + GN_PC - 1) / GN_PC : 0;
-    const dim3 blk(256);
-    const size_t lc = (size_t)p.C * sizeof(float2), lg = (size_t)p.G * sizeof(float2);
-    auto ks = GN_DISPATCH(dtype, wide, act, gn_bwd_sums_kernel);
-    if (hipError_t e = plyolo::ensure_dynamic_lds((const void*)ks, lc); e != hipSuccess) return e;
-    hipLaunchKernelGGL(ks, dim3(nblk), blk, lc, s, p);
-    auto kd = GN_DISPATCH(dtype, wide, act, gn_bwd_dx_kernel);
-    if (hipError_t e = plyolo::ensure_dynamic_lds((const void*)kd, lg); e != hipSuccess) return e;
-    hipLaunchKernelGGL(kd, dim3(nblk + npar), blk, lg, s, p, npar);
+    hipLaunchKernelGGL(ks, dim3(nblk), dim3(256), (size_t)p.C * sizeof(float2), s, p);
+    hipLaunchKernelGGL(kd, dim3(nblk + npar), dim3(256), (size_t)p.G * sizeof(float2), s, p, npar);
     return hipGetLastError();
   });
 }

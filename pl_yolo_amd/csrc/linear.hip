@@ -32,10 +32,11 @@ struct LinP {
 
 // ------------------------------------------------------------------------------------------------ bf16
 constexpr int BK = 64;           // contraction elements per stage
-constexpr int TI = 128, TJ = 128;
 typedef u32x4 __attribute__((aligned(2))) u32x4_any;     // 16 bytes at any element address
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 DEVINL s16x4 tr_read(const unsigned char* p) { return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p); }
+
+__device__ u32x4 zero_granule;   // where the lanes of a direct load that have nothing to fetch read from
 
 // eight consecutive elements of which `n` exist (the others are zero)
 DEVINL u32x4 load8(const bf16_t* p, int n) {
@@ -47,39 +48,71 @@ DEVINL u32x4 load8(const bf16_t* p, int n) {
   return v;
 }
 
-// One operand tile: T rows (output index) x 64 (contraction).
+DEVINL int xcd_contiguous(int id, int n) {      // hardware deals workgroup ids round robin over the 8 XCDs: give each a contiguous range
+  const int q = n >> 3, r = n & 7, x = id & 7;
+  return (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + (id >> 3);
+}
+
+// One operand tile: T rows (output index) x 64 (contraction), 256 threads.
 // KC image: [T][64] elements, 128-byte rows of eight 16-byte granules, granule g of row r at position g ^ (r & 7).
 // RC image: [64][T] elements, rows of T / 16 32-byte segments, segment s of row k at position s ^ f(k): the 16 rows that one transposed read
 // of a wave touches spread over all banks.
-template <bool RC, int T> struct Tile {
+// DIRECT: whole granules at 16-byte addresses go to LDS without passing registers (a lane's destination is fixed by the instruction, so the
+// swizzle is applied to its source); otherwise through registers, granule by granule, with tails element by element.
+template <bool RC, int T, bool DIRECT> struct Tile {
   static constexpr int NG = T * BK / 8 / 256;      // 16-byte granules per thread
   static constexpr int BYTES = T * BK * 2;
-  static DEVINL int swz(int k) { return (T >= 128 ? (k & 3) | ((k >> 1) & 4) : (k & 3)); }
-  static DEVINL void request(u32x4 (&v)[NG], const bf16_t* base, int ld, int row0, int rows, int k0, int kend) {
+  static DEVINL int swz(int k) { return T >= 128 ? (k & 3) | ((k >> 1) & 4) : (k & 3); }
+  const bf16_t* src[NG];     // granule u at contraction 0 of the workgroup (NULL: its row does not exist)
+  int kof[NG];               // its contraction offset inside a stage
+  u32x4 v[DIRECT ? 1 : NG];
+  int len[DIRECT ? 1 : NG];  // RC: elements of the granule that exist
+
+  DEVINL void init(const bf16_t* base, int ld, int row0, int rows, int kbeg) {
 #pragma unroll
     for (int u = 0; u < NG; ++u) {
       const int idx = threadIdx.x + u * 256;
       if (RC) {
-        const int k = k0 + idx / (T / 8), r = row0 + (idx % (T / 8)) * 8;
-        const int n = k < kend ? rows - r : 0;
-        v[u] = n > 0 ? load8(base + (size_t)k * ld + r, n) : u32x4{0u, 0u, 0u, 0u};
+        const int k = idx / (T / 8), pos = idx % (T / 8);
+        const int g = DIRECT ? ((((pos >> 1) ^ swz(k)) << 1) | (pos & 1)) : pos;
+        const int r = row0 + g * 8;
+        kof[u] = k;
+        src[u] = r < rows ? base + (size_t)(kbeg + k) * ld + r : nullptr;
+        if (!DIRECT) len[u] = rows - r;
       } else {
-        const int r = row0 + idx / 8, k = k0 + (idx % 8) * 8;
-        const int n = r < rows ? kend - k : 0;
-        v[u] = n > 0 ? load8(base + (size_t)r * ld + k, n) : u32x4{0u, 0u, 0u, 0u};
+        const int r = row0 + idx / 8, pos = idx % 8, g = DIRECT ? pos ^ ((idx / 8) & 7) : pos;
+        kof[u] = g * 8;
+        src[u] = r < rows ? base + (size_t)r * ld + kbeg + g * 8 : nullptr;
       }
     }
   }
-  static DEVINL void commit(const u32x4 (&v)[NG], unsigned char* img) {
+  // the stage that starts `k` elements behind kbeg, `left` elements of the contraction are left there
+  DEVINL void request(unsigned char* img, size_t k, int ld, int left) {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+#pragma unroll
+    for (int u = 0; u < NG; ++u) {
+      const bf16_t* q = src[u] + (RC ? k * ld : k);
+      const bool ok = src[u] != nullptr && kof[u] < left;
+      if (DIRECT) {
+        const void* g = ok ? (const void*)q : (const void*)&zero_granule;
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)g,
+                                         (__attribute__((address_space(3))) void*)(img + (u * 256 + wave * 64) * 16), 16, 0, 0);
+      } else {
+        v[DIRECT ? 0 : u] = ok ? load8(q, RC ? len[DIRECT ? 0 : u] : left - kof[u]) : u32x4{0u, 0u, 0u, 0u};
+      }
+    }
+  }
+  DEVINL void commit(unsigned char* img) const {
+    if (DIRECT) return;
 #pragma unroll
     for (int u = 0; u < NG; ++u) {
       const int idx = threadIdx.x + u * 256;
       if (RC) {
         const int k = idx / (T / 8), g = idx % (T / 8);
-        *(u32x4*)(img + k * (T * 2) + (((g >> 1) ^ swz(k)) << 5) + ((g & 1) << 4)) = v[u];
+        *(u32x4*)(img + k * (T * 2) + (((g >> 1) ^ swz(k)) << 5) + ((g & 1) << 4)) = v[DIRECT ? 0 : u];
       } else {
         const int r = idx / 8, g = idx % 8;
-        *(u32x4*)(img + r * 128 + ((g ^ (r & 7)) << 4)) = v[u];
+        *(u32x4*)(img + r * 128 + ((g ^ (r & 7)) << 4)) = v[DIRECT ? 0 : u];
       }
     }
   }
@@ -97,24 +130,25 @@ template <bool RC, int T> struct Tile {
   }
 };
 
-// four consecutive columns j.. of output row i; nv of them exist
-template <int MODE> DEVINL void store4(const LinP& p, int i, int j, f32x4 v) {
+// four consecutive columns j.. of output row i; nv of them exist.  HEAVY: hswish / GELU (their code stays out of the other instances)
+template <int MODE, bool HEAVY> DEVINL void store4(const LinP& p, int i, int j, f32x4 v, const f32x4 bias) {
   const int nv = p.J - j;
   if (i >= p.I || nv <= 0) return;
   if (MODE == MODE_DW) {
     float* o = (float*)p.out + ((size_t)blockIdx.y * p.I + i) * p.J + j;
+    if (p.vec4 && nv >= 4) {
+      *(f32x4*)o = v;
+    } else {
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (e < nv) o[e] = v[e];
+      for (int e = 0; e < 4; ++e)
+        if (e < nv) o[e] = v[e];
+    }
     return;
   }
   const bool whole = p.vec4 && nv >= 4;
   if (MODE == MODE_FWD) {
-    if (p.bias) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (e < nv) v[e] += p.bias[j + e];
-    }
+    for (int e = 0; e < 4; ++e) v[e] += bias[e];
     if (p.z) {
       bf16_t* z = (bf16_t*)p.z + (size_t)i * p.z_ld + j;
       if (whole) *(uint2*)z = make_uint2(pack2bf(v[0], v[1]), pack2bf(v[2], v[3]));
@@ -123,8 +157,13 @@ template <int MODE> DEVINL void store4(const LinP& p, int i, int j, f32x4 v) {
         for (int e = 0; e < 4; ++e)
           if (e < nv) z[e] = f2bf(v[e]);
     }
+    if (!HEAVY && p.act == PLYOLO_ACT_SILU) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = act_fwd(v[e], p.act);
+      for (int e = 0; e < 4; ++e) v[e] = act_fwd_core(v[e], PLYOLO_ACT_SILU);
+    } else if (HEAVY || p.act != PLYOLO_ACT_NONE) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = HEAVY ? act_fwd(v[e], p.act) : act_fwd_core(v[e], p.act);
+    }
   }
   bf16_t* o = (bf16_t*)p.out + (size_t)i * p.o_ld + j;
   const bf16_t* r = MODE == MODE_FWD ? (p.res ? (const bf16_t*)p.res + (size_t)i * p.r_ld + j : nullptr) : (p.accumulate ? o : nullptr);
@@ -144,52 +183,106 @@ template <int MODE> DEVINL void store4(const LinP& p, int i, int j, f32x4 v) {
   }
 }
 
-template <int MODE> __global__ __launch_bounds__(256) void linear_bf16_kernel(const LinP p) {
+template <int MODE> DEVINL f32x4 bias4(const LinP& p, int j) {
+  f32x4 b = {0.f, 0.f, 0.f, 0.f};
+  if (MODE == MODE_FWD && p.bias) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (j + e < p.J) b[e] = p.bias[j + e];
+  }
+  return b;
+}
+
+// TI x TJ tile, four waves of TI / 2 x TJ / 2, two LDS images per operand, one barrier per stage: stage s + 1 is requested behind the barrier
+// that ends the reads of its image and lands under the MFMAs of stage s.
+template <int MODE, int TI, int TJ, bool DIRECT, bool HEAVY> __global__ __launch_bounds__(256) void linear_bf16_kernel(const LinP p) {
   constexpr bool ARC = MODE == MODE_DW, BRC = MODE != MODE_FWD;
-  typedef Tile<ARC, TI> TA;
-  typedef Tile<BRC, TJ> TB;
-  __shared__ __align__(16) unsigned char smem[2][TA::BYTES + TB::BYTES];
-  const int i0 = (int)(blockIdx.x / p.nj) * TI, j0 = (int)(blockIdx.x % p.nj) * TJ;
-  const int wave = threadIdx.x >> 6, wi = (wave >> 1) * 64, wj = (wave & 1) * 64;
+  typedef Tile<ARC, TI, DIRECT> TA;
+  typedef Tile<BRC, TJ, DIRECT> TB;
+  constexpr int FA = TI / 32, FB = TJ / 32, STAGE = TA::BYTES + TB::BYTES;
+  extern __shared__ __align__(16) unsigned char smem[];
+  const int id = xcd_contiguous(blockIdx.x, gridDim.x);
+  const int i0 = id / p.nj * TI, j0 = id % p.nj * TJ;
+  const int wave = threadIdx.x >> 6, wi = (wave >> 1) * (TI / 2), wj = (wave & 1) * (TJ / 2);
   const int kbeg = MODE == MODE_DW ? (int)blockIdx.y * p.ksteps * BK : 0;
-  const int kend = MODE == MODE_DW ? min(p.Kc, kbeg + p.ksteps * BK) : p.Kc;
-  f32x4 acc[4][4];
+  const int klen = (MODE == MODE_DW ? min(p.Kc, kbeg + p.ksteps * BK) : p.Kc) - kbeg;
+  f32x4 acc[FA][FB];
 #pragma unroll
-  for (int a = 0; a < 4; ++a)
+  for (int a = 0; a < FA; ++a)
 #pragma unroll
-    for (int b = 0; b < 4; ++b) acc[a][b] = f32x4{0.f, 0.f, 0.f, 0.f};
-  u32x4 va[TA::NG], vb[TB::NG];
-  TA::request(va, (const bf16_t*)p.a, p.a_ld, i0, p.I, kbeg, kend);
-  TB::request(vb, (const bf16_t*)p.b, p.b_ld, j0, p.J, kbeg, kend);
+    for (int b = 0; b < FB; ++b) acc[a][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+  TA ta;
+  TB tb;
+  ta.init((const bf16_t*)p.a, p.a_ld, i0, p.I, kbeg);
+  tb.init((const bf16_t*)p.b, p.b_ld, j0, p.J, kbeg);
+  ta.request(smem, 0, p.a_ld, klen);
+  tb.request(smem + TA::BYTES, 0, p.b_ld, klen);
   int buf = 0;
-  for (int k0 = kbeg; k0 < kend; k0 += BK, buf ^= 1) {
-    unsigned char *ia = smem[buf], *ib = smem[buf] + TA::BYTES;
-    TA::commit(va, ia);
-    TB::commit(vb, ib);
+  for (int k0 = 0; k0 < klen; k0 += BK, buf ^= 1) {
+    unsigned char *ia = smem + buf * STAGE, *ib = ia + TA::BYTES, *na = smem + (buf ^ 1) * STAGE;
+    ta.commit(ia);
+    tb.commit(ib);
+    if (DIRECT) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();      // image `buf` is whole; image buf ^ 1 was last read before every wave came here
-    if (k0 + BK < kend) {
-      TA::request(va, (const bf16_t*)p.a, p.a_ld, i0, p.I, k0 + BK, kend);
-      TB::request(vb, (const bf16_t*)p.b, p.b_ld, j0, p.J, k0 + BK, kend);
+    if (k0 + BK < klen) {
+      ta.request(na, k0 + BK, p.a_ld, klen - k0 - BK);
+      tb.request(na + TA::BYTES, k0 + BK, p.b_ld, klen - k0 - BK);
     }
 #pragma unroll
     for (int kk = 0; kk < 2; ++kk) {
-      s16x8 fa[4], fb[4];
+      s16x8 fa[FA], fb[FB];
 #pragma unroll
-      for (int a = 0; a < 4; ++a) fa[a] = TA::frag(ia, wi + a * 16, kk);
+      for (int a = 0; a < FA; ++a) fa[a] = TA::frag(ia, wi + a * 16, kk);
 #pragma unroll
-      for (int b = 0; b < 4; ++b) fb[b] = TB::frag(ib, wj + b * 16, kk);
+      for (int b = 0; b < FB; ++b) fb[b] = TB::frag(ib, wj + b * 16, kk);
 #pragma unroll
-      for (int a = 0; a < 4; ++a)
+      for (int a = 0; a < FA; ++a)
 #pragma unroll
-        for (int b = 0; b < 4; ++b)
+        for (int b = 0; b < FB; ++b)
           acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*(const bf16x8*)&fb[b], *(const bf16x8*)&fa[a], acc[a][b], 0, 0, 0);
     }
   }
   const int lane = threadIdx.x & 63;
 #pragma unroll
-  for (int a = 0; a < 4; ++a)
+  for (int b = 0; b < FB; ++b) {
+    const int j = j0 + wj + b * 16 + 4 * (lane >> 4);
+    const f32x4 bias = bias4<MODE>(p, j);
 #pragma unroll
-    for (int b = 0; b < 4; ++b) store4<MODE>(p, i0 + wi + a * 16 + (lane & 15), j0 + wj + b * 16 + 4 * (lane >> 4), acc[a][b]);
+    for (int a = 0; a < FA; ++a) store4<MODE, HEAVY>(p, i0 + wi + a * 16 + (lane & 15), j, acc[a][b], bias);
+  }
+}
+
+// Few output values: one workgroup per 16 x 16 block, the contraction split over its waves (forward only: both operands run along the
+// contraction, so fragments come straight from memory; every load of a wave's range is in flight at once), partial blocks added in wave order.
+template <bool HEAVY> __global__ __launch_bounds__(1024) void linear_bf16_narrow_kernel(const LinP p, const int kper) {
+  __shared__ f32x4 part[16][64];
+  const int waves = blockDim.x >> 6, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int i0 = (int)(blockIdx.x / p.nj) * 16, j0 = (int)(blockIdx.x % p.nj) * 16;
+  const int i = i0 + (lane & 15), jr = j0 + (lane & 15), ko = 8 * (lane >> 4);
+  const bf16_t* pa = (const bf16_t*)p.a + (size_t)i * p.a_ld;
+  const bf16_t* pb = (const bf16_t*)p.b + (size_t)jr * p.b_ld;
+  const int k0 = wave * kper, k1 = min(p.Kc, k0 + kper);
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  for (int k = k0; k < k1; k += 128) {
+    u32x4 fa[4], fb[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int kk = k + u * 32 + ko, n = k1 - kk;
+      fa[u] = i < p.I && n > 0 ? load8(pa + kk, n) : u32x4{0u, 0u, 0u, 0u};
+      fb[u] = jr < p.J && n > 0 ? load8(pb + kk, n) : u32x4{0u, 0u, 0u, 0u};
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*(const bf16x8*)&fb[u], *(const bf16x8*)&fa[u], acc, 0, 0, 0);
+  }
+  if (waves > 1) {
+    part[wave][lane] = acc;
+    __syncthreads();
+    if (wave) return;
+    acc = part[0][lane];
+    for (int w = 1; w < waves; ++w) acc += part[w][lane];
+  }
+  const int j = j0 + 4 * (lane >> 4);
+  store4<MODE_FWD, HEAVY>(p, i0 + (lane & 15), j, acc, bias4<MODE_FWD>(p, j));
 }
 
 // ------------------------------------------------------------------------------------------------ fp32 (parity mode)
@@ -210,6 +303,29 @@ template <bool RC> DEVINL void f32_commit(const float (&v)[4], float* img) {
   for (int u = 0; u < 4; ++u) {
     const int idx = threadIdx.x + u * 256;
     img[(RC ? idx / FT : idx % FK) * FP + (RC ? idx % FT : idx / FK)] = v[u];
+  }
+}
+
+template <int MODE> DEVINL void f32_store(const LinP& p, int i, int j, const f32x4 acc) {
+  if (i >= p.I) return;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if (j + e >= p.J) continue;
+    float v = acc[e];
+    if (MODE == MODE_DW) {
+      ((float*)p.out)[((size_t)blockIdx.y * p.I + i) * p.J + j + e] = v;
+      continue;
+    }
+    float* o = (float*)p.out + (size_t)i * p.o_ld + j + e;
+    if (MODE == MODE_FWD) {
+      if (p.bias) v += p.bias[j + e];
+      if (p.z) ((float*)p.z)[(size_t)i * p.z_ld + j + e] = v;
+      v = act_fwd_precise(v, p.act);
+      if (p.res) v += ((const float*)p.res)[(size_t)i * p.r_ld + j + e];
+    } else if (p.accumulate) {
+      v += *o;
+    }
+    *o = v;
   }
 }
 
@@ -255,32 +371,64 @@ template <int MODE> __global__ __launch_bounds__(256) void linear_f32_kernel(con
 #pragma unroll
   for (int a = 0; a < 2; ++a)
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      const int i = i0 + wi + a * 16 + (lane & 15), j = j0 + wj + b * 16 + 4 * (lane >> 4);
-      if (i >= p.I) continue;
+    for (int b = 0; b < 2; ++b) f32_store<MODE>(p, i0 + wi + a * 16 + (lane & 15), j0 + wj + b * 16 + 4 * (lane >> 4), acc[a][b]);
+}
+
+// Few output values, fp32: as linear_bf16_narrow_kernel; a lane takes four consecutive k and feeds them to four MFMAs in turn (both operands
+// in the same order, which is all a sum needs).
+DEVINL f32x4 load4(const float* p, int n) {
+  typedef f32x4 __attribute__((aligned(4))) f32x4_any;
+  if (n >= 4) return *(const f32x4_any*)p;
+  f32x4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if (j + e >= p.J) continue;
-        float v = acc[a][b][e];
-        if (MODE == MODE_DW) {
-          ((float*)p.out)[((size_t)blockIdx.y * p.I + i) * p.J + j + e] = v;
-          continue;
-        }
-        float* o = (float*)p.out + (size_t)i * p.o_ld + j + e;
-        if (MODE == MODE_FWD) {
-          if (p.bias) v += p.bias[j + e];
-          if (p.z) ((float*)p.z)[(size_t)i * p.z_ld + j + e] = v;
-          v = act_fwd_precise(v, p.act);
-          if (p.res) v += ((const float*)p.res)[(size_t)i * p.r_ld + j + e];
-        } else if (p.accumulate) {
-          v += *o;
-        }
-        *o = v;
-      }
+  for (int e = 0; e < 3; ++e)
+    if (e < n) v[e] = p[e];
+  return v;
+}
+
+__global__ __launch_bounds__(1024) void linear_f32_narrow_kernel(const LinP p, const int kper) {
+  __shared__ f32x4 part[16][64];
+  const int waves = blockDim.x >> 6, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int i0 = (int)(blockIdx.x / p.nj) * 16, j0 = (int)(blockIdx.x % p.nj) * 16;
+  const int i = i0 + (lane & 15), jr = j0 + (lane & 15), ko = 4 * (lane >> 4);
+  const float* pa = (const float*)p.a + (size_t)i * p.a_ld;
+  const float* pb = (const float*)p.b + (size_t)jr * p.b_ld;
+  const int k0 = wave * kper, k1 = min(p.Kc, k0 + kper);
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  for (int k = k0; k < k1; k += 64) {
+    f32x4 fa[4], fb[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int kk = k + u * 16 + ko, n = k1 - kk;
+      fa[u] = i < p.I && n > 0 ? load4(pa + kk, n) : f32x4{0.f, 0.f, 0.f, 0.f};
+      fb[u] = jr < p.J && n > 0 ? load4(pb + kk, n) : f32x4{0.f, 0.f, 0.f, 0.f};
     }
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(fb[u][e], fa[u][e], acc, 0, 0, 0);
+  }
+  if (waves > 1) {
+    part[wave][lane] = acc;
+    __syncthreads();
+    if (wave) return;
+    acc = part[0][lane];
+    for (int w = 1; w < waves; ++w) acc += part[w][lane];
+  }
+  f32_store<MODE_FWD>(p, i0 + (lane & 15), j0 + 4 * (lane >> 4), acc);
 }
 
 // ------------------------------------------------------------------------------------------------ dz, db, slab sums
+DEVINL void load_vec(const bf16_t* p, int n, float (&f)[8]) { Vec<bf16_t>::cvt(load8(p, n), f); }
+DEVINL void load_vec(const float* p, int n, float (&f)[4]) { Vec<float>::cvt(load4(p, n), f); }
+template <bool PRECISE> DEVINL float dz_act_grad(float u, int act) {
+  if (!PRECISE && act == PLYOLO_ACT_SILU) {
+    const float s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(u * -1.4426950408889634f));
+    return fmaf(s, fmaf(-u, s, u), s);
+  }
+  return act_grad<PRECISE>(u, act);
+}
+
 struct DzP {
   const void* dy;
   const void* z;        // NULL: dz = dy (only the column sums are formed)
@@ -289,67 +437,124 @@ struct DzP {
   int M, N, dy_ld, z_ld, dz_ld, act, rows;
 };
 
-// 64 columns x 4 row lanes per workgroup, `rows` rows
+// dz and the column sums of `rows` rows: a thread owns one vector of columns (16 bytes of T, at any element address) and walks down the rows.
+// dz leaves with a pitch of whole vectors and zeros behind column N: the products then take it on their wide path whatever N is.
 template <typename T> __global__ __launch_bounds__(256) void linear_dz_kernel(const DzP p) {
-  const int c = (int)blockIdx.x * 64 + (threadIdx.x & 63), rl = threadIdx.x >> 6;
-  const int64_t m0 = (int64_t)blockIdx.y * p.rows;
-  const int64_t m1 = min((int64_t)p.M, m0 + p.rows);
-  float s = 0.f;
-  for (int64_t m = m0 + rl; m < m1; m += 4) {
-    float d = 0.f;
-    if (c < p.N) {
-      d = ActT<T>::ld((const T*)p.dy + (size_t)m * p.dy_ld + c);
-      if (p.z) d *= act_grad<Vec<T>::precise>(ActT<T>::ld((const T*)p.z + (size_t)m * p.z_ld + c), p.act);
-      s += d;
+  constexpr int V = Vec<T>::N, U = 4;
+  __shared__ float red[256 * V];
+  const int cv = (p.N + V - 1) / V, cols = min(cv, 256), rpb = 256 / cols;
+  const int tcol = threadIdx.x % cols, trow = threadIdx.x / cols;
+  const int64_t m0 = (int64_t)blockIdx.x * p.rows;
+  const int nr = (int)min((int64_t)p.rows, (int64_t)p.M - m0);
+  for (int cb = 0; cb < cv; cb += cols) {
+    const int col = cb + tcol, n = p.N - col * V;        // n < V: the last, partial vector
+    float s[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) s[e] = 0.f;
+    if (col < cv && trow < rpb) {
+      const T* pd = (const T*)p.dy + (size_t)m0 * p.dy_ld + col * V;
+      const T* pz = p.z ? (const T*)p.z + (size_t)m0 * p.z_ld + col * V : nullptr;
+      T* po = p.dz ? (T*)p.dz + (size_t)m0 * p.dz_ld + col * V : nullptr;
+      for (int r0 = trow; r0 < nr; r0 += U * rpb) {
+        float d[U][V], z[U][V];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (r0 + u * rpb < nr) {
+            load_vec(pd + (size_t)(r0 + u * rpb) * p.dy_ld, n, d[u]);
+            if (pz) load_vec(pz + (size_t)(r0 + u * rpb) * p.z_ld, n, z[u]);
+          }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (r0 + u * rpb < nr) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+              if (pz) d[u][e] *= dz_act_grad<Vec<T>::precise>(z[u][e], p.act);
+              s[e] += d[u][e];
+            }
+            if (po) Vec<T>::store(po + (size_t)(r0 + u * rpb) * p.dz_ld, d[u]);
+          }
+      }
+#pragma unroll
+      for (int e = 0; e < V; ++e) red[(trow * cols + tcol) * V + e] = s[e];
     }
-    if (p.dz && c < p.dz_ld) ActT<T>::st((T*)p.dz + (size_t)m * p.dz_ld + c, d);
+    if (p.part) {
+      __syncthreads();
+      const int nch = min(cols, cv - cb) * V;
+      for (int t = threadIdx.x; t < nch; t += 256)
+        if (cb * V + t < p.N) {
+          float a = 0.f;
+          for (int w = 0; w < rpb && w < nr; ++w) a += red[w * cols * V + t];
+          p.part[(size_t)blockIdx.x * p.N + cb * V + t] = a;
+        }
+      __syncthreads();
+    }
   }
-  __shared__ float red[256];
-  red[threadIdx.x] = s;
-  __syncthreads();
-  if (rl == 0 && c < p.N && p.part) p.part[(size_t)blockIdx.y * p.N + c] = (s + red[threadIdx.x + 64]) + (red[threadIdx.x + 128] + red[threadIdx.x + 192]);
 }
 
-// out[e] (+)= sum over S slabs of part[s][e], in order; 64 elements x 4 slab lanes per workgroup
-template <typename O> __global__ __launch_bounds__(256) void linear_fold_kernel(const float* part, int S, size_t elems, O* out, int accumulate) {
-  const size_t e = (size_t)blockIdx.x * 64 + (threadIdx.x & 63);
-  const int sl = threadIdx.x >> 6;
+// out[e] (+)= sum over S slabs of part[s][e] in a fixed order.  16 elements x 16 slab lanes per workgroup, eight slabs in flight per lane; the
+// weight gradient's workgroups come first, the bias gradient's behind them (one launch for both)
+struct FoldP {
+  const float* part;
+  void* out;
+  size_t elems;
+  int S, f32, blocks;
+};
+__global__ __launch_bounds__(256) void linear_fold_kernel(const FoldP w, const FoldP b, const int accumulate) {
+  const bool second = (int)blockIdx.x >= w.blocks;
+  const FoldP q = second ? b : w;
+  const size_t e = (size_t)(blockIdx.x - (second ? w.blocks : 0)) * 16 + (threadIdx.x & 15);
+  const int sl = threadIdx.x >> 4;
   float v = 0.f;
-  if (e < elems)
-    for (int s = sl; s < S; s += 4) v += part[(size_t)s * elems + e];
+  if (e < q.elems) {
+#pragma unroll 8
+    for (int s = sl; s < q.S; s += 16) v += q.part[(size_t)s * q.elems + e];
+  }
   __shared__ float red[256];
   red[threadIdx.x] = v;
   __syncthreads();
-  if (sl == 0 && e < elems) {
-    v = (v + red[threadIdx.x + 64]) + (red[threadIdx.x + 128] + red[threadIdx.x + 192]);
-    if (accumulate) v += ActT<O>::ld(out + e);
-    ActT<O>::st(out + e, v);
+  if (sl == 0 && e < q.elems) {
+#pragma unroll
+    for (int w2 = 1; w2 < 16; ++w2) v += red[w2 * 16 + threadIdx.x];
+    if (q.f32) {
+      float* o = (float*)q.out + e;
+      *o = accumulate ? *o + v : v;
+    } else {
+      bf16_t* o = (bf16_t*)q.out + e;
+      *o = f2bf(accumulate ? bf2f(*o) + v : v);
+    }
   }
 }
 
 // ------------------------------------------------------------------------------------------------ host side
-constexpr int DZ_ROWS = 256;     // rows per workgroup of linear_dz_kernel (more where that would make over 4096 of them)
-
 struct BwdPlan {
-  int dz_ld, S, ksteps, dzblk, dzrows;
+  int dz_ld, S, ksteps, dzblk, dzrows, ti, tj;
   size_t dz_bytes, part_off, part_bytes, slab_off, slab_bytes, total;
 };
 
 size_t up16(size_t v) { return (v + 15) & ~(size_t)15; }
 
+// Tile of an I x J output (bf16): the large tile reads less LDS per MFMA, the small one fills the chip on small outputs.
+void pick_tile(int64_t I, int64_t J, int* ti, int* tj) {
+  auto tiles = [&](int a, int b) { return ((I + a - 1) / a) * ((J + b - 1) / b); };
+  if (tiles(256, 128) >= 256 && J > 64) { *ti = 256; *tj = 128; }
+  else if (tiles(128, 128) >= 192 && J > 64) { *ti = 128; *tj = 128; }
+  else { *ti = 64; *tj = 64; }
+}
+
 // Slabs of dw: enough row ranges to give every compute unit a workgroup, at least four stages each.
 BwdPlan bwd_plan(const plyolo_linear_desc* d) {
   BwdPlan b{};
   const bool half = d->dtype == PLYOLO_BF16;
-  const int es = half ? 2 : 4, ti = half ? TI : FT, bk = half ? BK : FK;
+  const int es = half ? 2 : 4, bk = half ? BK : FK;
   b.dz_ld = (d->N + 7) & ~7;
   b.dz_bytes = d->act == PLYOLO_ACT_NONE ? 0 : up16((size_t)d->M * b.dz_ld * es);
-  b.dzrows = max(DZ_ROWS, cdiv(d->M, 4096));
+  b.dzrows = max(32, cdiv(d->M, 512));
   b.dzblk = cdiv(d->M, b.dzrows);
   b.part_off = b.dz_bytes;
   b.part_bytes = up16((size_t)b.dzblk * d->N * 4);
   b.slab_off = b.part_off + b.part_bytes;
-  const int64_t tiles = (int64_t)cdiv(d->N, ti) * cdiv(d->K, ti);
+  b.ti = b.tj = half ? (d->N > 64 && d->K > 64 ? 128 : 64) : FT;
+  const int64_t tiles = (int64_t)cdiv(d->N, b.ti) * cdiv(d->K, b.tj);
   const int steps = cdiv(d->M, bk);
   int64_t s = (256 + tiles - 1) / tiles;
   if (s > (steps + 3) / 4) s = (steps + 3) / 4;
@@ -372,17 +577,36 @@ int check_linear(const plyolo_linear_desc* d, const char* who) {
 }
 
 // tile grid of an I x J output; the column tiles of one row tile are neighbours, so that its rows are read from HBM once
-int tile_grid(LinP& p, int t, const char* who) {
-  p.nj = cdiv(p.J, t);
-  const int64_t n = (int64_t)cdiv(p.I, t) * p.nj;
+int tile_grid(LinP& p, int ti, int tj, const char* who) {
+  p.nj = cdiv(p.J, tj);
+  const int64_t n = (int64_t)cdiv(p.I, ti) * p.nj;
   PLY_CHECK_ARG(n < 2147483647, "%s: more than 2^31 tiles", who);
   return (int)n;
 }
 
-template <int MODE> hipError_t launch_gemm(int dtype, const LinP& p, int grid, int slabs, hipStream_t s) {
-  if (dtype == PLYOLO_BF16) hipLaunchKernelGGL(linear_bf16_kernel<MODE>, dim3(grid, slabs), dim3(256), 0, s, p);
-  else hipLaunchKernelGGL(linear_f32_kernel<MODE>, dim3(grid, slabs), dim3(256), 0, s, p);
+bool rows16(const void* p, int ld, int len) { return (size_t)p % 16 == 0 && ld % 8 == 0 && len % 8 == 0; }
+
+template <int MODE, int TI, int TJ, bool DIRECT, bool HEAVY> hipError_t launch_tile(const LinP& p, int grid, int slabs, hipStream_t s) {
+  constexpr size_t lds = 2 * (size_t)(TI + TJ) * BK * 2;
+  auto k = linear_bf16_kernel<MODE, TI, TJ, DIRECT, HEAVY>;
+  if (hipError_t e = plyolo::ensure_dynamic_lds((const void*)k, lds); e != hipSuccess) return e;
+  hipLaunchKernelGGL(k, dim3(grid, slabs), dim3(256), lds, s, p);
   return hipGetLastError();
+}
+template <int MODE, bool DIRECT, bool HEAVY> hipError_t launch_bf16(const LinP& p, int ti, int grid, int slabs, hipStream_t s) {
+  if (MODE != MODE_DW && ti == 256) return launch_tile<MODE, MODE != MODE_DW ? 256 : 128, 128, DIRECT, HEAVY>(p, grid, slabs, s);
+  if (ti == 128) return launch_tile<MODE, 128, 128, DIRECT, HEAVY>(p, grid, slabs, s);
+  return launch_tile<MODE, 64, 64, DIRECT, HEAVY>(p, grid, slabs, s);
+}
+// direct: both operands' granules are whole and 16-byte aligned
+template <int MODE> hipError_t launch_gemm(int dtype, const LinP& p, int ti, int grid, int slabs, bool direct, hipStream_t s) {
+  if (dtype != PLYOLO_BF16) {
+    hipLaunchKernelGGL(linear_f32_kernel<MODE>, dim3(grid, slabs), dim3(256), 0, s, p);
+    return hipGetLastError();
+  }
+  const bool heavy = MODE == MODE_FWD && p.act > PLYOLO_ACT_LRELU;
+  if (direct) return heavy ? launch_bf16<MODE, true, MODE == MODE_FWD>(p, ti, grid, slabs, s) : launch_bf16<MODE, true, false>(p, ti, grid, slabs, s);
+  return heavy ? launch_bf16<MODE, false, MODE == MODE_FWD>(p, ti, grid, slabs, s) : launch_bf16<MODE, false, false>(p, ti, grid, slabs, s);
 }
 
 }  // namespace
@@ -408,11 +632,30 @@ int plyolo_linear_fwd(const plyolo_linear_desc* d, const void* x, const void* w,
   p.act = d->act;
   p.vec4 = d->y_ld % 4 == 0 && (!z || d->z_ld % 4 == 0) && (!res || d->r_ld % 4 == 0) && ((size_t)y | (size_t)z | (size_t)res) % 8 == 0;
   const int dtype = d->dtype;
-  const int grid = tile_grid(p, dtype == PLYOLO_BF16 ? TI : FT, "linear_fwd");
-  if (grid < 0) return -1;
   const double m = d->M, n = d->N, k = d->K;
   plyolo::annotate("linear_fwd", 2.0 * m * n * k, (m * k + n * k + m * n * (1.0 + (z ? 1 : 0) + (res ? 1 : 0))) * es);
-  return plyolo::submit(stream, [=](hipStream_t s) -> hipError_t { return launch_gemm<MODE_FWD>(dtype, p, grid, 1, s); });
+  // 16 x 16 blocks re-read x once per 16 columns and w once per 16 rows; while that is little, they fill the chip where tiles would not
+  const double again = (m * k * cdiv(d->N, 16) + n * k * cdiv(d->M, 16)) * es;
+  if (again < 32e6) {
+    const int grid = tile_grid(p, 16, 16, "linear_fwd");
+    if (grid < 0) return -1;
+    const int step = dtype == PLYOLO_BF16 ? 32 : 16;
+    int waves = 1;
+    while (waves < 16 && waves * 2 * step <= d->K && (int64_t)grid * waves < 4096) waves *= 2;
+    const int kper = cdiv(cdiv(d->K, waves), step) * step;
+    return plyolo::submit(stream, [=](hipStream_t s) -> hipError_t {
+      if (dtype != PLYOLO_BF16) hipLaunchKernelGGL(linear_f32_narrow_kernel, dim3(grid), dim3(64 * waves), 0, s, p, kper);
+      else if (p.act > PLYOLO_ACT_LRELU) hipLaunchKernelGGL(linear_bf16_narrow_kernel<true>, dim3(grid), dim3(64 * waves), 0, s, p, kper);
+      else hipLaunchKernelGGL(linear_bf16_narrow_kernel<false>, dim3(grid), dim3(64 * waves), 0, s, p, kper);
+      return hipGetLastError();
+    });
+  }
+  int ti = FT, tj = FT;
+  if (dtype == PLYOLO_BF16) pick_tile(d->M, d->N, &ti, &tj);
+  const int grid = tile_grid(p, ti, tj, "linear_fwd");
+  if (grid < 0) return -1;
+  const bool direct = rows16(x, d->x_ld, d->K) && rows16(w, d->w_ld, d->K);
+  return plyolo::submit(stream, [=](hipStream_t s) -> hipError_t { return launch_gemm<MODE_FWD>(dtype, p, ti, grid, 1, direct, s); });
 }
 
 int plyolo_linear_bwd(const plyolo_linear_desc* d, const void* dy, const void* z, const void* x, const void* w, void* dx, int dx_ld,
@@ -440,33 +683,42 @@ int plyolo_linear_bwd(const plyolo_linear_desc* d, const void* dy, const void* z
   LinP px{}, pw{};
   const void* g = has_act ? (const void*)ws : dy;
   const int g_ld = has_act ? b.dz_ld : d->y_ld;
-  px.a = g; px.b = w; px.out = dx; px.I = d->M; px.J = d->K; px.Kc = d->N;
+  px.a = g; px.b = w; px.out = dx; px.I = d->M; px.J = d->K;
+  px.Kc = d->N;
   px.a_ld = g_ld; px.b_ld = d->w_ld; px.o_ld = dx_ld; px.accumulate = accumulate_dx ? 1 : 0;
   px.vec4 = dx_ld % 4 == 0 && (size_t)dx % 8 == 0;
   pw.a = g; pw.b = x; pw.out = ws + b.slab_off; pw.I = d->N; pw.J = d->K; pw.Kc = d->M;
   pw.a_ld = g_ld; pw.b_ld = d->x_ld; pw.ksteps = b.ksteps;
-  const int t = dtype == PLYOLO_BF16 ? TI : FT;
-  const int gx = tile_grid(px, t, "linear_bwd"), gw = tile_grid(pw, t, "linear_bwd");
+  pw.vec4 = d->K % 4 == 0;
+  int ti = FT, tj = FT;
+  if (dtype == PLYOLO_BF16) pick_tile(d->M, d->K, &ti, &tj);
+  const int gx = tile_grid(px, ti, tj, "linear_bwd"), gw = tile_grid(pw, b.ti, b.tj, "linear_bwd");
   if (gx < 0 || gw < 0) return -1;
-  const size_t elems = (size_t)d->N * d->K;
-  const int N = d->N, acc = accumulate_params ? 1 : 0;
-  const dim3 dzgrid(cdiv(has_act ? b.dz_ld : d->N, 64), b.dzblk);
+  // dz rows are padded to whole vectors of zeros, dy rows end at N
+  const int g_len = has_act ? b.dz_ld : d->N;
+  const bool dx_direct = rows16(g, g_ld, g_len) && rows16(w, d->w_ld, d->K), dw_direct = rows16(g, g_ld, g_len) && rows16(x, d->x_ld, d->K);
+  FoldP fw{}, fb{};
+  if (dw) {
+    fw.part = (const float*)(ws + b.slab_off); fw.out = dw; fw.elems = (size_t)d->N * d->K; fw.S = b.S; fw.f32 = dw_dtype == PLYOLO_F32;
+    fw.blocks = (int)cdivz(fw.elems, 16);
+  }
+  if (db) {
+    fb.part = q.part; fb.out = db; fb.elems = (size_t)d->N; fb.S = b.dzblk; fb.f32 = 1;
+    fb.blocks = (int)cdivz(fb.elems, 16);
+  }
+  const int acc = accumulate_params ? 1 : 0;
   const double m = d->M, n = d->N, k = d->K;
   plyolo::annotate("linear_bwd", 2.0 * m * n * k * ((dx ? 1 : 0) + (dw ? 1 : 0)), (m * n * (has_act ? 2.0 : 1.0) + 2.0 * m * k + 2.0 * n * k) * es);
   return plyolo::submit(stream, [=](hipStream_t s) -> hipError_t {
     if (q.dz || q.part) {
-      if (dtype == PLYOLO_BF16) hipLaunchKernelGGL(linear_dz_kernel<bf16_t>, dzgrid, dim3(256), 0, s, q);
-      else hipLaunchKernelGGL(linear_dz_kernel<float>, dzgrid, dim3(256), 0, s, q);
+      if (dtype == PLYOLO_BF16) hipLaunchKernelGGL(linear_dz_kernel<bf16_t>, dim3(b.dzblk), dim3(256), 0, s, q);
+      else hipLaunchKernelGGL(linear_dz_kernel<float>, dim3(b.dzblk), dim3(256), 0, s, q);
     }
-    if (db) hipLaunchKernelGGL(linear_fold_kernel<float>, dim3((unsigned)cdiv(N, 64)), dim3(256), 0, s, q.part, b.dzblk, (size_t)N, db, acc);
     if (dx)
-      if (hipError_t e = launch_gemm<MODE_DX>(dtype, px, gx, 1, s); e != hipSuccess) return e;
-    if (dw) {
-      if (hipError_t e = launch_gemm<MODE_DW>(dtype, pw, gw, b.S, s); e != hipSuccess) return e;
-      const dim3 fg((unsigned)cdivz(elems, 64));
-      if (dw_dtype == PLYOLO_F32) hipLaunchKernelGGL(linear_fold_kernel<float>, fg, dim3(256), 0, s, (const float*)pw.out, b.S, elems, (float*)dw, acc);
-      else hipLaunchKernelGGL(linear_fold_kernel<bf16_t>, fg, dim3(256), 0, s, (const float*)pw.out, b.S, elems, (bf16_t*)dw, acc);
-    }
+      if (hipError_t e = launch_gemm<MODE_DX>(dtype, px, ti, gx, 1, dx_direct, s); e != hipSuccess) return e;
+    if (dw)
+      if (hipError_t e = launch_gemm<MODE_DW>(dtype, pw, b.ti, gw, b.S, dw_direct, s); e != hipSuccess) return e;
+    if (dw || db) hipLaunchKernelGGL(linear_fold_kernel, dim3((unsigned)(fw.blocks + fb.blocks)), dim3(256), 0, s, fw, fb, acc);
     return hipGetLastError();
   });
 }
