@@ -48,6 +48,16 @@ DEVINL u32x4 load8(const bf16_t* p, int n) {
   return v;
 }
 
+DEVINL void store8(bf16_t* p, int n, u32x4 v) {
+  if (n >= 8) {
+    *(u32x4_any*)p = v;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < n) p[e] = (bf16_t)(v[e >> 1] >> (16 * (e & 1)));
+  }
+}
+
 DEVINL int xcd_contiguous(int id, int n) {      // hardware deals workgroup ids round robin over the 8 XCDs: give each a contiguous range
   const int q = n >> 3, r = n & 7, x = id & 7;
   return (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + (id >> 3);
@@ -130,7 +140,18 @@ template <bool RC, int T, bool DIRECT> struct Tile {
   }
 };
 
-// four consecutive columns j.. of output row i; nv of them exist.  HEAVY: hswish / GELU (their code stays out of the other instances)
+// HEAVY: hswish / GELU (their code stays out of the other instances)
+template <bool HEAVY> DEVINL void act4(f32x4& v, int act) {
+  if (!HEAVY && act == PLYOLO_ACT_SILU) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = act_fwd_core(v[e], PLYOLO_ACT_SILU);
+  } else if (HEAVY || act != PLYOLO_ACT_NONE) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = HEAVY ? act_fwd(v[e], act) : act_fwd_core(v[e], act);
+  }
+}
+
+// four consecutive columns j.. of output row i; nv of them exist
 template <int MODE, bool HEAVY> DEVINL void store4(const LinP& p, int i, int j, f32x4 v, const f32x4 bias) {
   const int nv = p.J - j;
   if (i >= p.I || nv <= 0) return;
@@ -157,13 +178,7 @@ template <int MODE, bool HEAVY> DEVINL void store4(const LinP& p, int i, int j, 
         for (int e = 0; e < 4; ++e)
           if (e < nv) z[e] = f2bf(v[e]);
     }
-    if (!HEAVY && p.act == PLYOLO_ACT_SILU) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = act_fwd_core(v[e], PLYOLO_ACT_SILU);
-    } else if (HEAVY || p.act != PLYOLO_ACT_NONE) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = HEAVY ? act_fwd(v[e], p.act) : act_fwd_core(v[e], p.act);
-    }
+    act4<HEAVY>(v, p.act);
   }
   bf16_t* o = (bf16_t*)p.out + (size_t)i * p.o_ld + j;
   const bf16_t* r = MODE == MODE_FWD ? (p.res ? (const bf16_t*)p.res + (size_t)i * p.r_ld + j : nullptr) : (p.accumulate ? o : nullptr);
@@ -243,12 +258,59 @@ template <int MODE, int TI, int TJ, bool DIRECT, bool HEAVY> __global__ __launch
     }
   }
   const int lane = threadIdx.x & 63;
+  if (MODE == MODE_DW) {
+#pragma unroll
+    for (int b = 0; b < FB; ++b)
+#pragma unroll
+      for (int a = 0; a < FA; ++a)
+        store4<MODE, HEAVY>(p, i0 + wi + a * 16 + (lane & 15), j0 + wj + b * 16 + 4 * (lane >> 4), acc[a][b], f32x4{0.f, 0.f, 0.f, 0.f});
+    return;
+  }
+  // Rows leave (and the shortcut's rows, or dx's own for an accumulation, arrive) through LDS: a lane of the MFMA result holds 8 bytes of a row,
+  // written as they are they would cost four times the requests of whole 256-byte row pieces
+  constexpr int PITCH = TJ * 2 + 16, RV = TJ / 8;
+  unsigned char *ty = smem, *tz = smem + TI * PITCH;
+  const bf16_t* rows = MODE == MODE_FWD ? (const bf16_t*)p.res : p.accumulate ? (const bf16_t*)p.out : nullptr;
+  const int rows_ld = MODE == MODE_FWD ? p.r_ld : p.o_ld;
+  const bool with_z = MODE == MODE_FWD && p.z != nullptr;
+  __syncthreads();
+  if (rows) {
+    for (int idx = threadIdx.x; idx < TI * RV; idx += 256) {
+      const int r = idx / RV, c = idx % RV * 8;
+      if (i0 + r < p.I && j0 + c < p.J) *(u32x4*)(ty + r * PITCH + c * 2) = load8(rows + (size_t)(i0 + r) * rows_ld + j0 + c, p.J - j0 - c);
+    }
+    __syncthreads();
+  }
 #pragma unroll
   for (int b = 0; b < FB; ++b) {
-    const int j = j0 + wj + b * 16 + 4 * (lane >> 4);
-    const f32x4 bias = bias4<MODE>(p, j);
+    const int c = wj + b * 16 + 4 * (lane >> 4);
+    const f32x4 bias = bias4<MODE>(p, j0 + c);
 #pragma unroll
-    for (int a = 0; a < FA; ++a) store4<MODE, HEAVY>(p, i0 + wi + a * 16 + (lane & 15), j, acc[a][b], bias);
+    for (int a = 0; a < FA; ++a) {
+      const int at = (wi + a * 16 + (lane & 15)) * PITCH + c * 2;
+      f32x4 v = acc[a][b];
+      if (MODE == MODE_FWD) {
+        v += bias;
+        if (with_z) *(uint2*)(tz + at) = make_uint2(pack2bf(v[0], v[1]), pack2bf(v[2], v[3]));
+        act4<HEAVY>(v, p.act);
+      }
+      if (rows) {
+        const uint2 t = *(const uint2*)(ty + at);
+        v[0] += __uint_as_float(t.x << 16);
+        v[1] += __uint_as_float(t.x & 0xffff0000u);
+        v[2] += __uint_as_float(t.y << 16);
+        v[3] += __uint_as_float(t.y & 0xffff0000u);
+      }
+      *(uint2*)(ty + at) = make_uint2(pack2bf(v[0], v[1]), pack2bf(v[2], v[3]));
+    }
+  }
+  __syncthreads();
+#pragma unroll 4
+  for (int idx = threadIdx.x; idx < TI * RV; idx += 256) {
+    const int r = idx / RV, c = idx % RV * 8, n = p.J - j0 - c;
+    if (i0 + r >= p.I || n <= 0) continue;
+    store8((bf16_t*)p.out + (size_t)(i0 + r) * p.o_ld + j0 + c, n, *(const u32x4*)(ty + r * PITCH + c * 2));
+    if (with_z) store8((bf16_t*)p.z + (size_t)(i0 + r) * p.z_ld + j0 + c, n, *(const u32x4*)(tz + r * PITCH + c * 2));
   }
 }
 
@@ -536,8 +598,7 @@ size_t up16(size_t v) { return (v + 15) & ~(size_t)15; }
 // Tile of an I x J output (bf16): the large tile reads less LDS per MFMA, the small one fills the chip on small outputs.
 void pick_tile(int64_t I, int64_t J, int* ti, int* tj) {
   auto tiles = [&](int a, int b) { return ((I + a - 1) / a) * ((J + b - 1) / b); };
-  if (tiles(256, 128) >= 256 && J > 64) { *ti = 256; *tj = 128; }
-  else if (tiles(128, 128) >= 192 && J > 64) { *ti = 128; *tj = 128; }
+  if (tiles(128, 128) >= 192 && J > 64) { *ti = 128; *tj = 128; }
   else { *ti = 64; *tj = 64; }
 }
 
@@ -587,14 +648,14 @@ int tile_grid(LinP& p, int ti, int tj, const char* who) {
 bool rows16(const void* p, int ld, int len) { return (size_t)p % 16 == 0 && ld % 8 == 0 && len % 8 == 0; }
 
 template <int MODE, int TI, int TJ, bool DIRECT, bool HEAVY> hipError_t launch_tile(const LinP& p, int grid, int slabs, hipStream_t s) {
-  constexpr size_t lds = 2 * (size_t)(TI + TJ) * BK * 2;
+  constexpr size_t stages = 2 * (size_t)(TI + TJ) * BK * 2, rows = (size_t)TI * (TJ * 2 + 16);
+  const size_t out = MODE == MODE_DW ? 0 : rows * (MODE == MODE_FWD && p.z ? 2 : 1), lds = out > stages ? out : stages;
   auto k = linear_bf16_kernel<MODE, TI, TJ, DIRECT, HEAVY>;
   if (hipError_t e = plyolo::ensure_dynamic_lds((const void*)k, lds); e != hipSuccess) return e;
   hipLaunchKernelGGL(k, dim3(grid, slabs), dim3(256), lds, s, p);
   return hipGetLastError();
 }
 template <int MODE, bool DIRECT, bool HEAVY> hipError_t launch_bf16(const LinP& p, int ti, int grid, int slabs, hipStream_t s) {
-  if (MODE != MODE_DW && ti == 256) return launch_tile<MODE, MODE != MODE_DW ? 256 : 128, 128, DIRECT, HEAVY>(p, grid, slabs, s);
   if (ti == 128) return launch_tile<MODE, 128, 128, DIRECT, HEAVY>(p, grid, slabs, s);
   return launch_tile<MODE, 64, 64, DIRECT, HEAVY>(p, grid, slabs, s);
 }
