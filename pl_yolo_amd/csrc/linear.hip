@@ -31,7 +31,7 @@ struct LinP {
 };
 
 // ------------------------------------------------------------------------------------------------ bf16
-constexpr int BK = 64;           // contraction elements per stage
+constexpr int BK = 64;           // contraction elements per stage (and the unit that dw's row ranges are counted in)
 typedef u32x4 __attribute__((aligned(2))) u32x4_any;     // 16 bytes at any element address
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 DEVINL s16x4 tr_read(const unsigned char* p) { return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p); }
@@ -63,16 +63,18 @@ DEVINL int xcd_contiguous(int id, int n) {      // hardware deals workgroup ids 
   return (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + (id >> 3);
 }
 
-// One operand tile: T rows (output index) x 64 (contraction), 256 threads.
-// KC image: [T][64] elements, 128-byte rows of eight 16-byte granules, granule g of row r at position g ^ (r & 7).
-// RC image: [64][T] elements, rows of T / 16 32-byte segments, segment s of row k at position s ^ f(k): the 16 rows that one transposed read
+// One operand tile: T rows (output index) x K contraction elements, NT threads.
+// KC image: [T][K] elements, rows of K / 8 16-byte granules, granule g of row r at position g ^ f(r).
+// RC image: [K][T] elements, rows of T / 16 32-byte segments, segment s of row k at position s ^ f(k): the 16 rows that one transposed read
 // of a wave touches spread over all banks.
 // DIRECT: whole granules at 16-byte addresses go to LDS without passing registers (a lane's destination is fixed by the instruction, so the
 // swizzle is applied to its source); otherwise through registers, granule by granule, with tails element by element.
-template <bool RC, int T, bool DIRECT> struct Tile {
-  static constexpr int NG = T * BK / 8 / 256;      // 16-byte granules per thread
-  static constexpr int BYTES = T * BK * 2;
-  static DEVINL int swz(int k) { return T >= 128 ? (k & 3) | ((k >> 1) & 4) : (k & 3); }
+template <bool RC, int T, int K, int NT, bool DIRECT> struct Tile {
+  static constexpr int NG = T * K / 8 / NT;      // 16-byte granules per thread
+  static constexpr int BYTES = T * K * 2, KG = K / 8, TG = T / 8;
+  static_assert(NG * NT * 8 == T * K, "whole granules per thread");
+  static DEVINL int swz_k(int k) { return T >= 128 ? (k & 3) | ((k >> 1) & 4) : (k & 3); }
+  static DEVINL int swz_r(int r) { return K == 64 ? r & 7 : (r >> 1) & 3; }
   const bf16_t* src[NG];     // granule u at contraction 0 of the workgroup (NULL: its row does not exist)
   int kof[NG];               // its contraction offset inside a stage
   u32x4 v[DIRECT ? 1 : NG];
@@ -81,22 +83,22 @@ template <bool RC, int T, bool DIRECT> struct Tile {
   DEVINL void init(const bf16_t* base, int ld, int row0, int rows, int kbeg) {
 #pragma unroll
     for (int u = 0; u < NG; ++u) {
-      const int idx = threadIdx.x + u * 256;
+      const int idx = threadIdx.x + u * NT;
       if (RC) {
-        const int k = idx / (T / 8), pos = idx % (T / 8);
-        const int g = DIRECT ? ((((pos >> 1) ^ swz(k)) << 1) | (pos & 1)) : pos;
+        const int k = idx / TG, pos = idx % TG;
+        const int g = DIRECT ? ((((pos >> 1) ^ swz_k(k)) << 1) | (pos & 1)) : pos;
         const int r = row0 + g * 8;
         kof[u] = k;
         src[u] = r < rows ? base + (size_t)(kbeg + k) * ld + r : nullptr;
         if (!DIRECT) len[u] = rows - r;
       } else {
-        const int r = row0 + idx / 8, pos = idx % 8, g = DIRECT ? pos ^ ((idx / 8) & 7) : pos;
+        const int r = row0 + idx / KG, pos = idx % KG, g = DIRECT ? pos ^ swz_r(idx / KG) : pos;
         kof[u] = g * 8;
         src[u] = r < rows ? base + (size_t)r * ld + kbeg + g * 8 : nullptr;
       }
     }
   }
-  // the stage that starts `k` elements behind kbeg, `left` elements of the contraction are left there
+  // the stage that starts `k` elements behind kbeg, `left` elements of the contraction are left there (none: zeros)
   DEVINL void request(unsigned char* img, size_t k, int ld, int left) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 #pragma unroll
@@ -106,7 +108,7 @@ template <bool RC, int T, bool DIRECT> struct Tile {
       if (DIRECT) {
         const void* g = ok ? (const void*)q : (const void*)&zero_granule;
         __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)g,
-                                         (__attribute__((address_space(3))) void*)(img + (u * 256 + wave * 64) * 16), 16, 0, 0);
+                                         (__attribute__((address_space(3))) void*)(img + (u * NT + wave * 64) * 16), 16, 0, 0);
       } else {
         v[DIRECT ? 0 : u] = ok ? load8(q, RC ? len[DIRECT ? 0 : u] : left - kof[u]) : u32x4{0u, 0u, 0u, 0u};
       }
@@ -116,27 +118,27 @@ template <bool RC, int T, bool DIRECT> struct Tile {
     if (DIRECT) return;
 #pragma unroll
     for (int u = 0; u < NG; ++u) {
-      const int idx = threadIdx.x + u * 256;
+      const int idx = threadIdx.x + u * NT;
       if (RC) {
-        const int k = idx / (T / 8), g = idx % (T / 8);
-        *(u32x4*)(img + k * (T * 2) + (((g >> 1) ^ swz(k)) << 5) + ((g & 1) << 4)) = v[DIRECT ? 0 : u];
+        const int k = idx / TG, g = idx % TG;
+        *(u32x4*)(img + k * (T * 2) + (((g >> 1) ^ swz_k(k)) << 5) + ((g & 1) << 4)) = v[DIRECT ? 0 : u];
       } else {
-        const int r = idx / 8, g = idx % 8;
-        *(u32x4*)(img + r * 128 + ((g ^ (r & 7)) << 4)) = v[DIRECT ? 0 : u];
+        const int r = idx / KG, g = idx % KG;
+        *(u32x4*)(img + r * (K * 2) + ((g ^ swz_r(r)) << 4)) = v[DIRECT ? 0 : u];
       }
     }
   }
-  // fragment of 16 output indices starting at r0, 32 contraction elements of half kk
+  // fragment of 16 output indices starting at r0, contraction elements 32 kk .. 32 kk + 31
   static DEVINL s16x8 frag(const unsigned char* img, int r0, int kk) {
     const int lane = threadIdx.x & 63, g4 = lane >> 4, i16 = lane & 15;
     if (RC) {
       const int k = kk * 32 + 8 * g4 + (i16 >> 2), seg = r0 >> 4;
-      const unsigned char* p = img + k * (T * 2) + ((seg ^ swz(k)) << 5) + ((i16 & 3) << 3);
-      const s16x4 lo = tr_read(p), hi = tr_read(p + 4 * (T * 2));       // (swz(k + 4) == swz(k))
+      const unsigned char* p = img + k * (T * 2) + ((seg ^ swz_k(k)) << 5) + ((i16 & 3) << 3);
+      const s16x4 lo = tr_read(p), hi = tr_read(p + 4 * (T * 2));       // (swz_k(k + 4) == swz_k(k))
       return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
     }
     const int r = r0 + i16, g = kk * 4 + g4;
-    return *(const s16x8*)(img + r * 128 + ((g ^ (r & 7)) << 4));
+    return *(const s16x8*)(img + r * (K * 2) + ((g ^ swz_r(r)) << 4));
   }
 };
 
@@ -198,22 +200,112 @@ template <int MODE, bool HEAVY> DEVINL void store4(const LinP& p, int i, int j, 
   }
 }
 
+// the bias of columns j .. j + 3 (zeros where there is none)
 template <int MODE> DEVINL f32x4 bias4(const LinP& p, int j) {
+  typedef f32x4 __attribute__((aligned(4))) f32x4_any;
   f32x4 b = {0.f, 0.f, 0.f, 0.f};
   if (MODE == MODE_FWD && p.bias) {
+    if (j + 4 <= p.J) {
+      b = *(const f32x4_any*)(p.bias + j);
+    } else {
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (j + e < p.J) b[e] = p.bias[j + e];
+      for (int e = 0; e < 3; ++e)
+        if (j + e < p.J) b[e] = p.bias[j + e];
+    }
   }
   return b;
 }
+// ... of a wave's columns, requested in front of the contraction
+template <int MODE, int FB> struct Bias {
+  f32x4 v[MODE == MODE_FWD ? FB : 1];
+  DEVINL Bias(const LinP& p, int j0) {
+    if (MODE == MODE_FWD) {
+#pragma unroll
+      for (int b = 0; b < FB; ++b) v[b] = bias4<MODE>(p, j0 + b * 16 + 4 * ((threadIdx.x & 63) >> 4));
+    }
+  }
+};
 
-// TI x TJ tile, four waves of TI / 2 x TJ / 2, two LDS images per operand, one barrier per stage: stage s + 1 is requested behind the barrier
-// that ends the reads of its image and lands under the MFMAs of stage s.
-template <int MODE, int TI, int TJ, bool DIRECT, bool HEAVY> __global__ __launch_bounds__(256) void linear_bf16_kernel(const LinP p) {
+// Rows leave (and the shortcut's rows, or dx's own for an accumulation, arrive) through LDS: a lane of the MFMA result holds 8 bytes of a row,
+// written as they are they would cost four times the requests of whole row pieces.  z and y take the same image one after the other: less LDS
+// is one workgroup per compute unit more.
+template <int TI, int TJ> constexpr size_t out_bytes() { return (size_t)TI * (TJ * 2 + 16); }
+
+template <int TI, int TJ, int NT> DEVINL void rows_out(const LinP& p, const unsigned char* img, int i0, int j0, bf16_t* out, int ld) {
+  constexpr int PITCH = TJ * 2 + 16, RV = TJ / 8;
+#pragma unroll 4
+  for (int idx = threadIdx.x; idx < TI * RV; idx += NT) {
+    const int r = idx / RV, c = idx % RV * 8, n = p.J - j0 - c;
+    if (i0 + r < p.I && n > 0) store8(out + (size_t)(i0 + r) * ld + j0 + c, n, *(const u32x4*)(img + r * PITCH + c * 2));
+  }
+}
+
+template <int MODE, int TI, int TJ, int NT, int WI, int WJ, bool HEAVY>
+DEVINL void tile_out(const LinP& p, unsigned char* img, int i0, int j0, const int wi, const int wj, f32x4 (&acc)[WI / 16][WJ / 16],
+                     const Bias<MODE, WJ / 16>& bias) {
+  constexpr int PITCH = TJ * 2 + 16, RV = TJ / 8, FA = WI / 16, FB = WJ / 16;
+  const int lane = threadIdx.x & 63, at0 = (wi + (lane & 15)) * PITCH + (wj + 4 * (lane >> 4)) * 2;
+  __syncthreads();
+  if (MODE == MODE_FWD) {
+#pragma unroll
+    for (int a = 0; a < FA; ++a)
+#pragma unroll
+      for (int b = 0; b < FB; ++b) acc[a][b] += bias.v[b];
+    if (p.z) {
+#pragma unroll
+      for (int a = 0; a < FA; ++a)
+#pragma unroll
+        for (int b = 0; b < FB; ++b)
+          *(uint2*)(img + at0 + a * 16 * PITCH + b * 32) = make_uint2(pack2bf(acc[a][b][0], acc[a][b][1]), pack2bf(acc[a][b][2], acc[a][b][3]));
+      __syncthreads();
+      rows_out<TI, TJ, NT>(p, img, i0, j0, (bf16_t*)p.z, p.z_ld);
+      __syncthreads();
+    }
+  }
+  const bf16_t* rows = MODE == MODE_FWD ? (const bf16_t*)p.res : p.accumulate ? (const bf16_t*)p.out : nullptr;
+  if (rows) {
+    const int ld = MODE == MODE_FWD ? p.r_ld : p.o_ld;
+    for (int idx = threadIdx.x; idx < TI * RV; idx += NT) {
+      const int r = idx / RV, c = idx % RV * 8;
+      if (i0 + r < p.I && j0 + c < p.J) *(u32x4*)(img + r * PITCH + c * 2) = load8(rows + (size_t)(i0 + r) * ld + j0 + c, p.J - j0 - c);
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int a = 0; a < FA; ++a)
+#pragma unroll
+    for (int b = 0; b < FB; ++b) {
+      unsigned char* at = img + at0 + a * 16 * PITCH + b * 32;
+      f32x4 v = acc[a][b];
+      if (MODE == MODE_FWD) act4<HEAVY>(v, p.act);
+      if (rows) {
+        const uint2 t = *(const uint2*)at;
+        v[0] += __uint_as_float(t.x << 16);
+        v[1] += __uint_as_float(t.x & 0xffff0000u);
+        v[2] += __uint_as_float(t.y << 16);
+        v[3] += __uint_as_float(t.y & 0xffff0000u);
+      }
+      *(uint2*)at = make_uint2(pack2bf(v[0], v[1]), pack2bf(v[2], v[3]));
+    }
+  __syncthreads();
+  rows_out<TI, TJ, NT>(p, img, i0, j0, (bf16_t*)p.out, p.o_ld);
+}
+
+template <int MODE, int WI, int WJ> DEVINL void slab_out(const LinP& p, int i0, int j0, f32x4 (&acc)[WI / 16][WJ / 16]) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int b = 0; b < WJ / 16; ++b)
+#pragma unroll
+    for (int a = 0; a < WI / 16; ++a)
+      store4<MODE, false>(p, i0 + a * 16 + (lane & 15), j0 + b * 16 + 4 * (lane >> 4), acc[a][b], f32x4{0.f, 0.f, 0.f, 0.f});
+}
+
+// Any size, pitch and alignment: TI x TJ tile, four waves of TI / 2 x TJ / 2, operands through registers into two LDS images, one barrier per
+// stage: stage s + 1 is requested behind the barrier of stage s and lands under its MFMAs.
+template <int MODE, int TI, int TJ, bool HEAVY> __global__ __launch_bounds__(256) void linear_bf16_any_kernel(const LinP p) {
   constexpr bool ARC = MODE == MODE_DW, BRC = MODE != MODE_FWD;
-  typedef Tile<ARC, TI, DIRECT> TA;
-  typedef Tile<BRC, TJ, DIRECT> TB;
+  typedef Tile<ARC, TI, BK, 256, false> TA;
+  typedef Tile<BRC, TJ, BK, 256, false> TB;
   constexpr int FA = TI / 32, FB = TJ / 32, STAGE = TA::BYTES + TB::BYTES;
   extern __shared__ __align__(16) unsigned char smem[];
   const int id = xcd_contiguous(blockIdx.x, gridDim.x);
@@ -226,22 +318,22 @@ template <int MODE, int TI, int TJ, bool DIRECT, bool HEAVY> __global__ __launch
   for (int a = 0; a < FA; ++a)
 #pragma unroll
     for (int b = 0; b < FB; ++b) acc[a][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const Bias<MODE, FB> bias(p, j0 + wj);
   TA ta;
   TB tb;
   ta.init((const bf16_t*)p.a, p.a_ld, i0, p.I, kbeg);
   tb.init((const bf16_t*)p.b, p.b_ld, j0, p.J, kbeg);
   ta.request(smem, 0, p.a_ld, klen);
-  tb.request(smem + TA::BYTES, 0, p.b_ld, klen);
+  tb.request(smem, 0, p.b_ld, klen);
   int buf = 0;
   for (int k0 = 0; k0 < klen; k0 += BK, buf ^= 1) {
-    unsigned char *ia = smem + buf * STAGE, *ib = ia + TA::BYTES, *na = smem + (buf ^ 1) * STAGE;
+    unsigned char *ia = smem + buf * STAGE, *ib = ia + TA::BYTES;
     ta.commit(ia);
     tb.commit(ib);
-    if (DIRECT) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();      // image `buf` is whole; image buf ^ 1 was last read before every wave came here
     if (k0 + BK < klen) {
-      ta.request(na, k0 + BK, p.a_ld, klen - k0 - BK);
-      tb.request(na + TA::BYTES, k0 + BK, p.b_ld, klen - k0 - BK);
+      ta.request(smem, k0 + BK, p.a_ld, klen - k0 - BK);
+      tb.request(smem, k0 + BK, p.b_ld, klen - k0 - BK);
     }
 #pragma unroll
     for (int kk = 0; kk < 2; ++kk) {
@@ -257,61 +349,68 @@ template <int MODE, int TI, int TJ, bool DIRECT, bool HEAVY> __global__ __launch
           acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*(const bf16x8*)&fb[b], *(const bf16x8*)&fa[a], acc[a][b], 0, 0, 0);
     }
   }
-  const int lane = threadIdx.x & 63;
-  if (MODE == MODE_DW) {
+  if (MODE == MODE_DW) slab_out<MODE, TI / 2, TJ / 2>(p, i0 + wi, j0 + wj, acc);
+  else tile_out<MODE, TI, TJ, 256, TI / 2, TJ / 2, HEAVY>(p, smem, i0, j0, wi, wj, acc, bias);
+}
+
+// Aligned operands: NWI x NWJ waves of WI x WJ, ST LDS images of 32 contraction elements filled by direct loads, ST - 1 stages in flight: a
+// stage's wait leaves the younger stages' loads outstanding.  One barrier per stage: behind it the image that was read in the stage before is
+// free for the youngest request.
+template <int N> DEVINL void wait_and_meet() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory"); }
+
+template <int MODE, int NWI, int NWJ, int WI, int WJ, int ST, bool HEAVY>
+__global__ __launch_bounds__(64 * NWI * NWJ) void linear_bf16_kernel(const LinP p) {
+  constexpr bool ARC = MODE == MODE_DW, BRC = MODE != MODE_FWD;
+  constexpr int NT = 64 * NWI * NWJ, TI = NWI * WI, TJ = NWJ * WJ, K = 32, FA = WI / 16, FB = WJ / 16;
+  typedef Tile<ARC, TI, K, NT, true> TA;
+  typedef Tile<BRC, TJ, K, NT, true> TB;
+  constexpr int STAGE = TA::BYTES + TB::BYTES, LOADS = TA::NG + TB::NG;
+  static_assert(ST == 3 || ST == 4, "the waits below");
+  extern __shared__ __align__(16) unsigned char smem[];
+  const int id = xcd_contiguous(blockIdx.x, gridDim.x);
+  const int i0 = id / p.nj * TI, j0 = id % p.nj * TJ;
+  const int wave = threadIdx.x >> 6, wi = wave / NWJ * WI, wj = wave % NWJ * WJ;
+  const int kbeg = MODE == MODE_DW ? (int)blockIdx.y * p.ksteps * BK : 0;
+  const int klen = (MODE == MODE_DW ? min(p.Kc, kbeg + p.ksteps * BK) : p.Kc) - kbeg;
+  f32x4 acc[FA][FB];
 #pragma unroll
-    for (int b = 0; b < FB; ++b)
+  for (int a = 0; a < FA; ++a)
 #pragma unroll
-      for (int a = 0; a < FA; ++a)
-        store4<MODE, HEAVY>(p, i0 + wi + a * 16 + (lane & 15), j0 + wj + b * 16 + 4 * (lane >> 4), acc[a][b], f32x4{0.f, 0.f, 0.f, 0.f});
-    return;
+    for (int b = 0; b < FB; ++b) acc[a][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const Bias<MODE, FB> bias(p, j0 + wj);
+  TA ta;
+  TB tb;
+  ta.init((const bf16_t*)p.a, p.a_ld, i0, p.I, kbeg);
+  tb.init((const bf16_t*)p.b, p.b_ld, j0, p.J, kbeg);
+  for (int s = 0; s < ST - 1 && s * K < klen; ++s) {
+    ta.request(smem + s * STAGE, s * K, p.a_ld, klen - s * K);
+    tb.request(smem + s * STAGE + TA::BYTES, s * K, p.b_ld, klen - s * K);
   }
-  // Rows leave (and the shortcut's rows, or dx's own for an accumulation, arrive) through LDS: a lane of the MFMA result holds 8 bytes of a row,
-  // written as they are they would cost four times the requests of whole 256-byte row pieces
-  constexpr int PITCH = TJ * 2 + 16, RV = TJ / 8;
-  unsigned char *ty = smem, *tz = smem + TI * PITCH;
-  const bf16_t* rows = MODE == MODE_FWD ? (const bf16_t*)p.res : p.accumulate ? (const bf16_t*)p.out : nullptr;
-  const int rows_ld = MODE == MODE_FWD ? p.r_ld : p.o_ld;
-  const bool with_z = MODE == MODE_FWD && p.z != nullptr;
-  __syncthreads();
-  if (rows) {
-    for (int idx = threadIdx.x; idx < TI * RV; idx += 256) {
-      const int r = idx / RV, c = idx % RV * 8;
-      if (i0 + r < p.I && j0 + c < p.J) *(u32x4*)(ty + r * PITCH + c * 2) = load8(rows + (size_t)(i0 + r) * rows_ld + j0 + c, p.J - j0 - c);
+  int buf = 0;
+  for (int k0 = 0; k0 < klen; k0 += K, buf = buf + 1 == ST ? 0 : buf + 1) {
+    unsigned char *ia = smem + buf * STAGE, *ib = ia + TA::BYTES;
+    const int behind = klen - k0;                  // stages requested behind this one: as many as there are, ST - 2 at most
+    if (ST == 4 && behind > 2 * K) wait_and_meet<2 * LOADS>();
+    else if (behind > K) wait_and_meet<LOADS>();
+    else wait_and_meet<0>();
+    if (behind > (ST - 1) * K) {
+      unsigned char* na = smem + (buf == 0 ? ST - 1 : buf - 1) * STAGE;
+      ta.request(na, k0 + (ST - 1) * K, p.a_ld, behind - (ST - 1) * K);
+      tb.request(na + TA::BYTES, k0 + (ST - 1) * K, p.b_ld, behind - (ST - 1) * K);
     }
-    __syncthreads();
-  }
+    s16x8 fa[FA], fb[FB];
 #pragma unroll
-  for (int b = 0; b < FB; ++b) {
-    const int c = wj + b * 16 + 4 * (lane >> 4);
-    const f32x4 bias = bias4<MODE>(p, j0 + c);
+    for (int b = 0; b < FB; ++b) fb[b] = TB::frag(ib, wj + b * 16, 0);
 #pragma unroll
-    for (int a = 0; a < FA; ++a) {
-      const int at = (wi + a * 16 + (lane & 15)) * PITCH + c * 2;
-      f32x4 v = acc[a][b];
-      if (MODE == MODE_FWD) {
-        v += bias;
-        if (with_z) *(uint2*)(tz + at) = make_uint2(pack2bf(v[0], v[1]), pack2bf(v[2], v[3]));
-        act4<HEAVY>(v, p.act);
-      }
-      if (rows) {
-        const uint2 t = *(const uint2*)(ty + at);
-        v[0] += __uint_as_float(t.x << 16);
-        v[1] += __uint_as_float(t.x & 0xffff0000u);
-        v[2] += __uint_as_float(t.y << 16);
-        v[3] += __uint_as_float(t.y & 0xffff0000u);
-      }
-      *(uint2*)(ty + at) = make_uint2(pack2bf(v[0], v[1]), pack2bf(v[2], v[3]));
-    }
+    for (int a = 0; a < FA; ++a) fa[a] = TA::frag(ia, wi + a * 16, 0);
+#pragma unroll
+    for (int a = 0; a < FA; ++a)
+#pragma unroll
+      for (int b = 0; b < FB; ++b)
+        acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*(const bf16x8*)&fb[b], *(const bf16x8*)&fa[a], acc[a][b], 0, 0, 0);
   }
-  __syncthreads();
-#pragma unroll 4
-  for (int idx = threadIdx.x; idx < TI * RV; idx += 256) {
-    const int r = idx / RV, c = idx % RV * 8, n = p.J - j0 - c;
-    if (i0 + r >= p.I || n <= 0) continue;
-    store8((bf16_t*)p.out + (size_t)(i0 + r) * p.o_ld + j0 + c, n, *(const u32x4*)(ty + r * PITCH + c * 2));
-    if (with_z) store8((bf16_t*)p.z + (size_t)(i0 + r) * p.z_ld + j0 + c, n, *(const u32x4*)(tz + r * PITCH + c * 2));
-  }
+  if (MODE == MODE_DW) slab_out<MODE, WI, WJ>(p, i0 + wi, j0 + wj, acc);
+  else tile_out<MODE, TI, TJ, NT, WI, WJ, HEAVY>(p, smem, i0, j0, wi, wj, acc, bias);
 }
 
 // Few output values: one workgroup per 16 x 16 block, the contraction split over its waves (forward only: both operands run along the
@@ -589,17 +688,19 @@ __global__ __launch_bounds__(256) void linear_fold_kernel(const FoldP w, const F
 
 // ------------------------------------------------------------------------------------------------ host side
 struct BwdPlan {
-  int dz_ld, S, ksteps, dzblk, dzrows, ti, tj;
+  int dz_ld, S, ksteps, dzblk, dzrows, tile;
   size_t dz_bytes, part_off, part_bytes, slab_off, slab_bytes, total;
 };
 
 size_t up16(size_t v) { return (v + 15) & ~(size_t)15; }
 
-// Tile of an I x J output (bf16): the large tile reads less LDS per MFMA, the small one fills the chip on small outputs.
-void pick_tile(int64_t I, int64_t J, int* ti, int* tj) {
-  auto tiles = [&](int a, int b) { return ((I + a - 1) / a) * ((J + b - 1) / b); };
-  if (tiles(128, 128) >= 192 && J > 64) { *ti = 128; *tj = 128; }
-  else { *ti = 64; *tj = 64; }
+// Tile edge of an I x J output (bf16): the larger the tile, the fewer LDS reads per MFMA and the fewer re-reads of the operands; the smaller,
+// the more of the chip a small output fills.
+int pick_tile(int64_t I, int64_t J, int64_t Kc, bool direct) {
+  auto tiles = [&](int a) { return ((I + a - 1) / a) * ((J + a - 1) / a); };
+  if (direct && tiles(256) >= 128 && J > 128 && Kc >= 512) return 256;
+  if (tiles(128) >= 192 && J > 64) return 128;
+  return 64;
 }
 
 // Slabs of dw: enough row ranges to give every compute unit a workgroup, at least four stages each.
@@ -614,8 +715,8 @@ BwdPlan bwd_plan(const plyolo_linear_desc* d) {
   b.part_off = b.dz_bytes;
   b.part_bytes = up16((size_t)b.dzblk * d->N * 4);
   b.slab_off = b.part_off + b.part_bytes;
-  b.ti = b.tj = half ? (d->N > 64 && d->K > 64 ? 128 : 64) : FT;
-  const int64_t tiles = (int64_t)cdiv(d->N, b.ti) * cdiv(d->K, b.tj);
+  b.tile = half ? (d->N > 64 && d->K > 64 ? 128 : 64) : FT;
+  const int64_t tiles = (int64_t)cdiv(d->N, b.tile) * cdiv(d->K, b.tile);
   const int steps = cdiv(d->M, bk);
   int64_t s = (256 + tiles - 1) / tiles;
   if (s > (steps + 3) / 4) s = (steps + 3) / 4;
@@ -638,36 +739,50 @@ int check_linear(const plyolo_linear_desc* d, const char* who) {
 }
 
 // tile grid of an I x J output; the column tiles of one row tile are neighbours, so that its rows are read from HBM once
-int tile_grid(LinP& p, int ti, int tj, const char* who) {
-  p.nj = cdiv(p.J, tj);
-  const int64_t n = (int64_t)cdiv(p.I, ti) * p.nj;
+int tile_grid(LinP& p, int tile, const char* who) {
+  p.nj = cdiv(p.J, tile);
+  const int64_t n = (int64_t)cdiv(p.I, tile) * p.nj;
   PLY_CHECK_ARG(n < 2147483647, "%s: more than 2^31 tiles", who);
   return (int)n;
 }
 
 bool rows16(const void* p, int ld, int len) { return (size_t)p % 16 == 0 && ld % 8 == 0 && len % 8 == 0; }
 
-template <int MODE, int TI, int TJ, bool DIRECT, bool HEAVY> hipError_t launch_tile(const LinP& p, int grid, int slabs, hipStream_t s) {
-  constexpr size_t stages = 2 * (size_t)(TI + TJ) * BK * 2, rows = (size_t)TI * (TJ * 2 + 16);
-  const size_t out = MODE == MODE_DW ? 0 : rows * (MODE == MODE_FWD && p.z ? 2 : 1), lds = out > stages ? out : stages;
-  auto k = linear_bf16_kernel<MODE, TI, TJ, DIRECT, HEAVY>;
+template <int MODE, int TI, int TJ> size_t tile_lds(size_t stages) {
+  const size_t out = MODE == MODE_DW ? 0 : out_bytes<TI, TJ>();
+  return out > stages ? out : stages;
+}
+template <int MODE, int T, bool HEAVY> hipError_t launch_any(const LinP& p, int grid, int slabs, hipStream_t s) {
+  const size_t lds = tile_lds<MODE, T, T>(2 * (size_t)(2 * T) * BK * 2);
+  auto k = linear_bf16_any_kernel<MODE, T, T, HEAVY>;
   if (hipError_t e = plyolo::ensure_dynamic_lds((const void*)k, lds); e != hipSuccess) return e;
   hipLaunchKernelGGL(k, dim3(grid, slabs), dim3(256), lds, s, p);
   return hipGetLastError();
 }
-template <int MODE, bool DIRECT, bool HEAVY> hipError_t launch_bf16(const LinP& p, int ti, int grid, int slabs, hipStream_t s) {
-  if (ti == 128) return launch_tile<MODE, 128, 128, DIRECT, HEAVY>(p, grid, slabs, s);
-  return launch_tile<MODE, 64, 64, DIRECT, HEAVY>(p, grid, slabs, s);
+template <int MODE, int NWI, int NWJ, int WI, int WJ, int ST, bool HEAVY> hipError_t launch_direct(const LinP& p, int grid, int slabs, hipStream_t s) {
+  constexpr int TI = NWI * WI, TJ = NWJ * WJ;
+  const size_t lds = tile_lds<MODE, TI, TJ>(ST * (size_t)(TI + TJ) * 32 * 2);
+  auto k = linear_bf16_kernel<MODE, NWI, NWJ, WI, WJ, ST, HEAVY>;
+  if (hipError_t e = plyolo::ensure_dynamic_lds((const void*)k, lds); e != hipSuccess) return e;
+  hipLaunchKernelGGL(k, dim3(grid, slabs), dim3(64 * NWI * NWJ), lds, s, p);
+  return hipGetLastError();
 }
 // direct: both operands' granules are whole and 16-byte aligned
-template <int MODE> hipError_t launch_gemm(int dtype, const LinP& p, int ti, int grid, int slabs, bool direct, hipStream_t s) {
+template <int MODE, bool HEAVY> hipError_t launch_bf16(const LinP& p, int tile, int grid, int slabs, bool direct, hipStream_t s) {
+  if (direct) {
+    if constexpr (MODE != MODE_DW) if (tile == 256) return launch_direct<MODE, 2, 4, 128, 64, 4, HEAVY>(p, grid, slabs, s);
+    if (tile == 128) return launch_direct<MODE, 2, 2, 64, 64, 3, HEAVY>(p, grid, slabs, s);
+    return launch_direct<MODE, 2, 2, 32, 32, 4, HEAVY>(p, grid, slabs, s);
+  }
+  return tile == 128 ? launch_any<MODE, 128, HEAVY>(p, grid, slabs, s) : launch_any<MODE, 64, HEAVY>(p, grid, slabs, s);
+}
+template <int MODE> hipError_t launch_gemm(int dtype, const LinP& p, int tile, int grid, int slabs, bool direct, hipStream_t s) {
   if (dtype != PLYOLO_BF16) {
     hipLaunchKernelGGL(linear_f32_kernel<MODE>, dim3(grid, slabs), dim3(256), 0, s, p);
     return hipGetLastError();
   }
-  const bool heavy = MODE == MODE_FWD && p.act > PLYOLO_ACT_LRELU;
-  if (direct) return heavy ? launch_bf16<MODE, true, MODE == MODE_FWD>(p, ti, grid, slabs, s) : launch_bf16<MODE, true, false>(p, ti, grid, slabs, s);
-  return heavy ? launch_bf16<MODE, false, MODE == MODE_FWD>(p, ti, grid, slabs, s) : launch_bf16<MODE, false, false>(p, ti, grid, slabs, s);
+  if (MODE == MODE_FWD && p.act > PLYOLO_ACT_LRELU) return launch_bf16<MODE, MODE == MODE_FWD>(p, tile, grid, slabs, direct, s);
+  return launch_bf16<MODE, false>(p, tile, grid, slabs, direct, s);
 }
 
 }  // namespace
@@ -698,7 +813,7 @@ int plyolo_linear_fwd(const plyolo_linear_desc* d, const void* x, const void* w,
   // 16 x 16 blocks re-read x once per 16 columns and w once per 16 rows; while that is little, they fill the chip where tiles would not
   const double again = (m * k * cdiv(d->N, 16) + n * k * cdiv(d->M, 16)) * es;
   if (again < 32e6) {
-    const int grid = tile_grid(p, 16, 16, "linear_fwd");
+    const int grid = tile_grid(p, 16, "linear_fwd");
     if (grid < 0) return -1;
     const int step = dtype == PLYOLO_BF16 ? 32 : 16;
     int waves = 1;
@@ -711,12 +826,11 @@ int plyolo_linear_fwd(const plyolo_linear_desc* d, const void* x, const void* w,
       return hipGetLastError();
     });
   }
-  int ti = FT, tj = FT;
-  if (dtype == PLYOLO_BF16) pick_tile(d->M, d->N, &ti, &tj);
-  const int grid = tile_grid(p, ti, tj, "linear_fwd");
-  if (grid < 0) return -1;
   const bool direct = rows16(x, d->x_ld, d->K) && rows16(w, d->w_ld, d->K);
-  return plyolo::submit(stream, [=](hipStream_t s) -> hipError_t { return launch_gemm<MODE_FWD>(dtype, p, ti, grid, 1, direct, s); });
+  const int tile = dtype == PLYOLO_BF16 ? pick_tile(d->M, d->N, d->K, direct) : FT;
+  const int grid = tile_grid(p, tile, "linear_fwd");
+  if (grid < 0) return -1;
+  return plyolo::submit(stream, [=](hipStream_t s) -> hipError_t { return launch_gemm<MODE_FWD>(dtype, p, tile, grid, 1, direct, s); });
 }
 
 int plyolo_linear_bwd(const plyolo_linear_desc* d, const void* dy, const void* z, const void* x, const void* w, void* dx, int dx_ld,
@@ -751,13 +865,12 @@ int plyolo_linear_bwd(const plyolo_linear_desc* d, const void* dy, const void* z
   pw.a = g; pw.b = x; pw.out = ws + b.slab_off; pw.I = d->N; pw.J = d->K; pw.Kc = d->M;
   pw.a_ld = g_ld; pw.b_ld = d->x_ld; pw.ksteps = b.ksteps;
   pw.vec4 = d->K % 4 == 0;
-  int ti = FT, tj = FT;
-  if (dtype == PLYOLO_BF16) pick_tile(d->M, d->K, &ti, &tj);
-  const int gx = tile_grid(px, ti, tj, "linear_bwd"), gw = tile_grid(pw, b.ti, b.tj, "linear_bwd");
-  if (gx < 0 || gw < 0) return -1;
   // dz rows are padded to whole vectors of zeros, dy rows end at N
   const int g_len = has_act ? b.dz_ld : d->N;
   const bool dx_direct = rows16(g, g_ld, g_len) && rows16(w, d->w_ld, d->K), dw_direct = rows16(g, g_ld, g_len) && rows16(x, d->x_ld, d->K);
+  const int tx = dtype == PLYOLO_BF16 ? pick_tile(d->M, d->K, d->N, dx_direct) : FT;
+  const int gx = tile_grid(px, tx, "linear_bwd"), gw = tile_grid(pw, b.tile, "linear_bwd");
+  if (gx < 0 || gw < 0) return -1;
   FoldP fw{}, fb{};
   if (dw) {
     fw.part = (const float*)(ws + b.slab_off); fw.out = dw; fw.elems = (size_t)d->N * d->K; fw.S = b.S; fw.f32 = dw_dtype == PLYOLO_F32;
@@ -776,9 +889,9 @@ int plyolo_linear_bwd(const plyolo_linear_desc* d, const void* dy, const void* z
       else hipLaunchKernelGGL(linear_dz_kernel<float>, dim3(b.dzblk), dim3(256), 0, s, q);
     }
     if (dx)
-      if (hipError_t e = launch_gemm<MODE_DX>(dtype, px, ti, gx, 1, dx_direct, s); e != hipSuccess) return e;
+      if (hipError_t e = launch_gemm<MODE_DX>(dtype, px, tx, gx, 1, dx_direct, s); e != hipSuccess) return e;
     if (dw)
-      if (hipError_t e = launch_gemm<MODE_DW>(dtype, pw, b.ti, gw, b.S, dw_direct, s); e != hipSuccess) return e;
+      if (hipError_t e = launch_gemm<MODE_DW>(dtype, pw, b.tile, gw, b.S, dw_direct, s); e != hipSuccess) return e;
     if (dw || db) hipLaunchKernelGGL(linear_fold_kernel, dim3((unsigned)(fw.blocks + fb.blocks)), dim3(256), 0, s, fw, fb, acc);
     return hipGetLastError();
   });
