@@ -353,19 +353,19 @@ template <int MODE, int TI, int TJ, bool HEAVY> __global__ __launch_bounds__(256
   else tile_out<MODE, TI, TJ, 256, TI / 2, TJ / 2, HEAVY>(p, smem, i0, j0, wi, wj, acc, bias);
 }
 
-// Aligned operands: NWI x NWJ waves of WI x WJ, ST LDS images of 32 contraction elements filled by direct loads, ST - 1 stages in flight: a
+// Aligned operands: NWI x NWJ waves of WI x WJ, ST LDS images of K contraction elements filled by direct loads, ST - 1 stages in flight: a
 // stage's wait leaves the younger stages' loads outstanding.  One barrier per stage: behind it the image that was read in the stage before is
 // free for the youngest request.
 template <int N> DEVINL void wait_and_meet() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory"); }
 
-template <int MODE, int NWI, int NWJ, int WI, int WJ, int ST, bool HEAVY>
+template <int MODE, int NWI, int NWJ, int WI, int WJ, int K, int ST, bool HEAVY>
 __global__ __launch_bounds__(64 * NWI * NWJ) void linear_bf16_kernel(const LinP p) {
   constexpr bool ARC = MODE == MODE_DW, BRC = MODE != MODE_FWD;
-  constexpr int NT = 64 * NWI * NWJ, TI = NWI * WI, TJ = NWJ * WJ, K = 32, FA = WI / 16, FB = WJ / 16;
+  constexpr int NT = 64 * NWI * NWJ, TI = NWI * WI, TJ = NWJ * WJ, FA = WI / 16, FB = WJ / 16;
   typedef Tile<ARC, TI, K, NT, true> TA;
   typedef Tile<BRC, TJ, K, NT, true> TB;
   constexpr int STAGE = TA::BYTES + TB::BYTES, LOADS = TA::NG + TB::NG;
-  static_assert(ST == 3 || ST == 4, "the waits below");
+  static_assert(ST >= 2 && ST <= 4, "the waits below");
   extern __shared__ __align__(16) unsigned char smem[];
   const int id = xcd_contiguous(blockIdx.x, gridDim.x);
   const int i0 = id / p.nj * TI, j0 = id % p.nj * TJ;
@@ -391,23 +391,35 @@ __global__ __launch_bounds__(64 * NWI * NWJ) void linear_bf16_kernel(const LinP 
     unsigned char *ia = smem + buf * STAGE, *ib = ia + TA::BYTES;
     const int behind = klen - k0;                  // stages requested behind this one: as many as there are, ST - 2 at most
     if (ST == 4 && behind > 2 * K) wait_and_meet<2 * LOADS>();
-    else if (behind > K) wait_and_meet<LOADS>();
+    else if (ST >= 3 && behind > K) wait_and_meet<LOADS>();
     else wait_and_meet<0>();
     if (behind > (ST - 1) * K) {
       unsigned char* na = smem + (buf == 0 ? ST - 1 : buf - 1) * STAGE;
       ta.request(na, k0 + (ST - 1) * K, p.a_ld, behind - (ST - 1) * K);
       tb.request(na + TA::BYTES, k0 + (ST - 1) * K, p.b_ld, behind - (ST - 1) * K);
     }
-    s16x8 fa[FA], fb[FB];
 #pragma unroll
-    for (int b = 0; b < FB; ++b) fb[b] = TB::frag(ib, wj + b * 16, 0);
+    for (int kk = 0; kk < K / 32; ++kk) {
+      s16x8 fa[FA], fb[FB];
 #pragma unroll
-    for (int a = 0; a < FA; ++a) fa[a] = TA::frag(ia, wi + a * 16, 0);
+      for (int b = 0; b < FB; ++b) fb[b] = TB::frag(ib, wj + b * 16, kk);
 #pragma unroll
-    for (int a = 0; a < FA; ++a)
+      for (int a = 0; a < FA; ++a) fa[a] = TA::frag(ia, wi + a * 16, kk);
 #pragma unroll
-      for (int b = 0; b < FB; ++b)
-        acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*(const bf16x8*)&fb[b], *(const bf16x8*)&fa[a], acc[a][b], 0, 0, 0);
+      for (int a = 0; a < FA; ++a)
+#pragma unroll
+        for (int b = 0; b < FB; ++b)
+          acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*(const bf16x8*)&fb[b], *(const bf16x8*)&fa[a], acc[a][b], 0, 0, 0);
+    }
+    // the order of the stage: the first fragments, then some reads behind every row of MFMAs, so that no row waits for its own
+    constexpr int RA = ARC ? 2 : 1, RB = BRC ? 2 : 1, ROWS = FA * (K / 32);      // (a transposed fragment is two LDS instructions)
+    constexpr int FIRST = RB * FB + RA * 2, LATER = ((RB * FB + RA * FA) * (K / 32) - FIRST + ROWS - 1) / ROWS;
+    __builtin_amdgcn_sched_group_barrier(0x100, FIRST, 0);
+#pragma unroll
+    for (int g = 0; g < ROWS; ++g) {
+      __builtin_amdgcn_sched_group_barrier(0x008, FB, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, LATER, 0);
+    }
   }
   if (MODE == MODE_DW) slab_out<MODE, WI, WJ>(p, i0 + wi, j0 + wj, acc);
   else tile_out<MODE, TI, TJ, NT, WI, WJ, HEAVY>(p, smem, i0, j0, wi, wj, acc, bias);
@@ -759,10 +771,10 @@ template <int MODE, int T, bool HEAVY> hipError_t launch_any(const LinP& p, int 
   hipLaunchKernelGGL(k, dim3(grid, slabs), dim3(256), lds, s, p);
   return hipGetLastError();
 }
-template <int MODE, int NWI, int NWJ, int WI, int WJ, int ST, bool HEAVY> hipError_t launch_direct(const LinP& p, int grid, int slabs, hipStream_t s) {
+template <int MODE, int NWI, int NWJ, int WI, int WJ, int K, int ST, bool HEAVY> hipError_t launch_direct(const LinP& p, int grid, int slabs, hipStream_t s) {
   constexpr int TI = NWI * WI, TJ = NWJ * WJ;
-  const size_t lds = tile_lds<MODE, TI, TJ>(ST * (size_t)(TI + TJ) * 32 * 2);
-  auto k = linear_bf16_kernel<MODE, NWI, NWJ, WI, WJ, ST, HEAVY>;
+  const size_t lds = tile_lds<MODE, TI, TJ>(ST * (size_t)(TI + TJ) * K * 2);
+  auto k = linear_bf16_kernel<MODE, NWI, NWJ, WI, WJ, K, ST, HEAVY>;
   if (hipError_t e = plyolo::ensure_dynamic_lds((const void*)k, lds); e != hipSuccess) return e;
   hipLaunchKernelGGL(k, dim3(grid, slabs), dim3(64 * NWI * NWJ), lds, s, p);
   return hipGetLastError();
@@ -770,9 +782,9 @@ template <int MODE, int NWI, int NWJ, int WI, int WJ, int ST, bool HEAVY> hipErr
 // direct: both operands' granules are whole and 16-byte aligned
 template <int MODE, bool HEAVY> hipError_t launch_bf16(const LinP& p, int tile, int grid, int slabs, bool direct, hipStream_t s) {
   if (direct) {
-    if constexpr (MODE != MODE_DW) if (tile == 256) return launch_direct<MODE, 2, 4, 128, 64, 4, HEAVY>(p, grid, slabs, s);
-    if (tile == 128) return launch_direct<MODE, 2, 2, 64, 64, 3, HEAVY>(p, grid, slabs, s);
-    return launch_direct<MODE, 2, 2, 32, 32, 4, HEAVY>(p, grid, slabs, s);
+    if constexpr (MODE != MODE_DW) if (tile == 256) return launch_direct<MODE, 2, 4, 128, 64, 64, 2, HEAVY>(p, grid, slabs, s);
+    if (tile == 128) return launch_direct<MODE, 2, 2, 64, 64, 64, 2, HEAVY>(p, grid, slabs, s);
+    return launch_direct<MODE, 2, 2, 32, 32, 64, 3, HEAVY>(p, grid, slabs, s);
   }
   return tile == 128 ? launch_any<MODE, 128, HEAVY>(p, grid, slabs, s) : launch_any<MODE, 64, HEAVY>(p, grid, slabs, s);
 }
