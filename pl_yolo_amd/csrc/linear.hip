@@ -26,7 +26,7 @@ struct LinP {
   int I, J, Kc;        // output rows, output columns, contraction length
   int a_ld, b_ld, o_ld, z_ld, r_ld;
   int act, accumulate, vec4;
-  int nj;              // column tiles
+  int nj, tiles;       // column tiles, all tiles of the output
   int ksteps;          // contraction steps per slab (MODE_DW), all of them otherwise
 };
 
@@ -38,13 +38,15 @@ DEVINL s16x4 tr_read(const unsigned char* p) { return __builtin_amdgcn_ds_read_t
 
 __device__ u32x4 zero_granule;   // where the lanes of a direct load that have nothing to fetch read from
 
-// eight consecutive elements of which `n` exist (the others are zero)
+// eight consecutive elements of which `n` >= 1 exist (the others are zero; the loads of a tail are all requested before one is used)
 DEVINL u32x4 load8(const bf16_t* p, int n) {
   if (n >= 8) return *(const u32x4_any*)p;
-  u32x4 v = {0u, 0u, 0u, 0u};
+  unsigned h[8];
 #pragma unroll
-  for (int e = 0; e < 8; ++e)
-    if (e < n) v[e >> 1] |= (unsigned)p[e] << (16 * (e & 1));
+  for (int e = 0; e < 8; ++e) h[e] = p[min(e, n - 1)];
+  u32x4 v;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = (2 * e < n ? h[2 * e] : 0u) | (2 * e + 1 < n ? h[2 * e + 1] << 16 : 0u);
   return v;
 }
 
@@ -61,6 +63,14 @@ DEVINL void store8(bf16_t* p, int n, u32x4 v) {
 DEVINL int xcd_contiguous(int id, int n) {      // hardware deals workgroup ids round robin over the 8 XCDs: give each a contiguous range
   const int q = n >> 3, r = n & 7, x = id & 7;
   return (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + (id >> 3);
+}
+
+// Output tile and (MODE_DW) contraction slab of a workgroup.  Neighbours read the same rows, so they get neighbouring ids on one XCD and its L2
+// serves all but the first of them: column tiles of one row tile, and all tiles of one slab.
+struct Place { int i0, j0, slab; };
+template <int TI, int TJ> DEVINL Place place(const LinP& p) {
+  const int id = xcd_contiguous(blockIdx.x, gridDim.x), tile = id % p.tiles;
+  return Place{tile / p.nj * TI, tile % p.nj * TJ, id / p.tiles};
 }
 
 // One operand tile: T rows (output index) x K contraction elements, NT threads.
@@ -157,17 +167,6 @@ template <bool HEAVY> DEVINL void act4(f32x4& v, int act) {
 template <int MODE, bool HEAVY> DEVINL void store4(const LinP& p, int i, int j, f32x4 v, const f32x4 bias) {
   const int nv = p.J - j;
   if (i >= p.I || nv <= 0) return;
-  if (MODE == MODE_DW) {
-    float* o = (float*)p.out + ((size_t)blockIdx.y * p.I + i) * p.J + j;
-    if (p.vec4 && nv >= 4) {
-      *(f32x4*)o = v;
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (e < nv) o[e] = v[e];
-    }
-    return;
-  }
   const bool whole = p.vec4 && nv >= 4;
   if (MODE == MODE_FWD) {
 #pragma unroll
@@ -291,13 +290,27 @@ DEVINL void tile_out(const LinP& p, unsigned char* img, int i0, int j0, const in
   rows_out<TI, TJ, NT>(p, img, i0, j0, (bf16_t*)p.out, p.o_ld);
 }
 
-template <int MODE, int WI, int WJ> DEVINL void slab_out(const LinP& p, int i0, int j0, f32x4 (&acc)[WI / 16][WJ / 16]) {
+// fp32 partial sums of a wave's block into its slab
+template <int WI, int WJ> DEVINL void slab_out(const LinP& p, int slab, int i0, int j0, f32x4 (&acc)[WI / 16][WJ / 16]) {
   const int lane = threadIdx.x & 63;
+  float* out = (float*)p.out + (size_t)slab * p.I * p.J;
 #pragma unroll
-  for (int b = 0; b < WJ / 16; ++b)
+  for (int b = 0; b < WJ / 16; ++b) {
+    const int j = j0 + b * 16 + 4 * (lane >> 4), n = p.J - j;
 #pragma unroll
-    for (int a = 0; a < WI / 16; ++a)
-      store4<MODE, false>(p, i0 + a * 16 + (lane & 15), j0 + b * 16 + 4 * (lane >> 4), acc[a][b], f32x4{0.f, 0.f, 0.f, 0.f});
+    for (int a = 0; a < WI / 16; ++a) {
+      const int i = i0 + a * 16 + (lane & 15);
+      if (i >= p.I || n <= 0) continue;
+      float* o = out + (size_t)i * p.J + j;
+      if (p.vec4 && n >= 4) {
+        *(f32x4*)o = acc[a][b];
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (e < n) o[e] = acc[a][b][e];
+      }
+    }
+  }
 }
 
 // Any size, pitch and alignment: TI x TJ tile, four waves of TI / 2 x TJ / 2, operands through registers into two LDS images, one barrier per
@@ -308,10 +321,10 @@ template <int MODE, int TI, int TJ, bool HEAVY> __global__ __launch_bounds__(256
   typedef Tile<BRC, TJ, BK, 256, false> TB;
   constexpr int FA = TI / 32, FB = TJ / 32, STAGE = TA::BYTES + TB::BYTES;
   extern __shared__ __align__(16) unsigned char smem[];
-  const int id = xcd_contiguous(blockIdx.x, gridDim.x);
-  const int i0 = id / p.nj * TI, j0 = id % p.nj * TJ;
+  const Place at = place<TI, TJ>(p);
+  const int i0 = at.i0, j0 = at.j0;
   const int wave = threadIdx.x >> 6, wi = (wave >> 1) * (TI / 2), wj = (wave & 1) * (TJ / 2);
-  const int kbeg = MODE == MODE_DW ? (int)blockIdx.y * p.ksteps * BK : 0;
+  const int kbeg = at.slab * p.ksteps * BK;
   const int klen = (MODE == MODE_DW ? min(p.Kc, kbeg + p.ksteps * BK) : p.Kc) - kbeg;
   f32x4 acc[FA][FB];
 #pragma unroll
@@ -349,7 +362,7 @@ template <int MODE, int TI, int TJ, bool HEAVY> __global__ __launch_bounds__(256
           acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*(const bf16x8*)&fb[b], *(const bf16x8*)&fa[a], acc[a][b], 0, 0, 0);
     }
   }
-  if (MODE == MODE_DW) slab_out<MODE, TI / 2, TJ / 2>(p, i0 + wi, j0 + wj, acc);
+  if (MODE == MODE_DW) slab_out<TI / 2, TJ / 2>(p, at.slab, i0 + wi, j0 + wj, acc);
   else tile_out<MODE, TI, TJ, 256, TI / 2, TJ / 2, HEAVY>(p, smem, i0, j0, wi, wj, acc, bias);
 }
 
@@ -367,10 +380,10 @@ __global__ __launch_bounds__(64 * NWI * NWJ) void linear_bf16_kernel(const LinP 
   constexpr int STAGE = TA::BYTES + TB::BYTES, LOADS = TA::NG + TB::NG;
   static_assert(ST >= 2 && ST <= 4, "the waits below");
   extern __shared__ __align__(16) unsigned char smem[];
-  const int id = xcd_contiguous(blockIdx.x, gridDim.x);
-  const int i0 = id / p.nj * TI, j0 = id % p.nj * TJ;
+  const Place at = place<TI, TJ>(p);
+  const int i0 = at.i0, j0 = at.j0;
   const int wave = threadIdx.x >> 6, wi = wave / NWJ * WI, wj = wave % NWJ * WJ;
-  const int kbeg = MODE == MODE_DW ? (int)blockIdx.y * p.ksteps * BK : 0;
+  const int kbeg = at.slab * p.ksteps * BK;
   const int klen = (MODE == MODE_DW ? min(p.Kc, kbeg + p.ksteps * BK) : p.Kc) - kbeg;
   f32x4 acc[FA][FB];
 #pragma unroll
@@ -421,7 +434,7 @@ __global__ __launch_bounds__(64 * NWI * NWJ) void linear_bf16_kernel(const LinP 
       __builtin_amdgcn_sched_group_barrier(0x100, LATER, 0);
     }
   }
-  if (MODE == MODE_DW) slab_out<MODE, WI, WJ>(p, i0 + wi, j0 + wj, acc);
+  if (MODE == MODE_DW) slab_out<WI, WJ>(p, at.slab, i0 + wi, j0 + wj, acc);
   else tile_out<MODE, TI, TJ, NT, WI, WJ, HEAVY>(p, smem, i0, j0, wi, wj, acc, bias);
 }
 
@@ -479,14 +492,14 @@ template <bool RC> DEVINL void f32_commit(const float (&v)[4], float* img) {
   }
 }
 
-template <int MODE> DEVINL void f32_store(const LinP& p, int i, int j, const f32x4 acc) {
+template <int MODE> DEVINL void f32_store(const LinP& p, int slab, int i, int j, const f32x4 acc) {
   if (i >= p.I) return;
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     if (j + e >= p.J) continue;
     float v = acc[e];
     if (MODE == MODE_DW) {
-      ((float*)p.out)[((size_t)blockIdx.y * p.I + i) * p.J + j + e] = v;
+      ((float*)p.out)[((size_t)slab * p.I + i) * p.J + j + e] = v;
       continue;
     }
     float* o = (float*)p.out + (size_t)i * p.o_ld + j + e;
@@ -505,9 +518,10 @@ template <int MODE> DEVINL void f32_store(const LinP& p, int i, int j, const f32
 template <int MODE> __global__ __launch_bounds__(256) void linear_f32_kernel(const LinP p) {
   constexpr bool ARC = MODE == MODE_DW, BRC = MODE != MODE_FWD;
   __shared__ float smem[2][2 * FK * FP];
-  const int i0 = (int)(blockIdx.x / p.nj) * FT, j0 = (int)(blockIdx.x % p.nj) * FT;
+  const Place at = place<FT, FT>(p);
+  const int i0 = at.i0, j0 = at.j0;
   const int wave = threadIdx.x >> 6, wi = (wave >> 1) * 32, wj = (wave & 1) * 32, lane = threadIdx.x & 63;
-  const int kbeg = MODE == MODE_DW ? (int)blockIdx.y * p.ksteps * FK : 0;
+  const int kbeg = at.slab * p.ksteps * FK;
   const int kend = MODE == MODE_DW ? min(p.Kc, kbeg + p.ksteps * FK) : p.Kc;
   f32x4 acc[2][2];
 #pragma unroll
@@ -544,7 +558,7 @@ template <int MODE> __global__ __launch_bounds__(256) void linear_f32_kernel(con
 #pragma unroll
   for (int a = 0; a < 2; ++a)
 #pragma unroll
-    for (int b = 0; b < 2; ++b) f32_store<MODE>(p, i0 + wi + a * 16 + (lane & 15), j0 + wj + b * 16 + 4 * (lane >> 4), acc[a][b]);
+    for (int b = 0; b < 2; ++b) f32_store<MODE>(p, at.slab, i0 + wi + a * 16 + (lane & 15), j0 + wj + b * 16 + 4 * (lane >> 4), acc[a][b]);
 }
 
 // Few output values, fp32: as linear_bf16_narrow_kernel; a lane takes four consecutive k and feeds them to four MFMAs in turn (both operands
@@ -552,11 +566,8 @@ template <int MODE> __global__ __launch_bounds__(256) void linear_f32_kernel(con
 DEVINL f32x4 load4(const float* p, int n) {
   typedef f32x4 __attribute__((aligned(4))) f32x4_any;
   if (n >= 4) return *(const f32x4_any*)p;
-  f32x4 v = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int e = 0; e < 3; ++e)
-    if (e < n) v[e] = p[e];
-  return v;
+  const float a = p[0], b = p[min(1, n - 1)], c = p[min(2, n - 1)];
+  return f32x4{a, n > 1 ? b : 0.f, n > 2 ? c : 0.f, 0.f};
 }
 
 __global__ __launch_bounds__(1024) void linear_f32_narrow_kernel(const LinP p, const int kper) {
@@ -588,7 +599,7 @@ __global__ __launch_bounds__(1024) void linear_f32_narrow_kernel(const LinP p, c
     acc = part[0][lane];
     for (int w = 1; w < waves; ++w) acc += part[w][lane];
   }
-  f32_store<MODE_FWD>(p, i0 + (lane & 15), j0 + 4 * (lane >> 4), acc);
+  f32_store<MODE_FWD>(p, 0, i0 + (lane & 15), j0 + 4 * (lane >> 4), acc);
 }
 
 // ------------------------------------------------------------------------------------------------ dz, db, slab sums
@@ -664,38 +675,55 @@ template <typename T> __global__ __launch_bounds__(256) void linear_dz_kernel(co
   }
 }
 
-// out[e] (+)= sum over S slabs of part[s][e] in a fixed order.  16 elements x 16 slab lanes per workgroup, eight slabs in flight per lane; the
-// weight gradient's workgroups come first, the bias gradient's behind them (one launch for both)
+// out[e] (+)= sum over S slabs of part[s][e] in a fixed order: 4 E elements x 64 / E slab lanes per workgroup, eight slabs in flight per lane.
+// The weight gradient's workgroups (E = 16 or 4 by its slab count) come first, the bias gradient's (E = 4) behind them: one launch for both.
 struct FoldP {
   const float* part;
   void* out;
   size_t elems;
   int S, f32, blocks;
 };
-__global__ __launch_bounds__(256) void linear_fold_kernel(const FoldP w, const FoldP b, const int accumulate) {
-  const bool second = (int)blockIdx.x >= w.blocks;
-  const FoldP q = second ? b : w;
-  const size_t e = (size_t)(blockIdx.x - (second ? w.blocks : 0)) * 16 + (threadIdx.x & 15);
-  const int sl = threadIdx.x >> 4;
-  float v = 0.f;
-  if (e < q.elems) {
+template <int E> DEVINL void fold(const FoldP& q, int block, int accumulate, f32x4* red) {
+  constexpr int L = 256 / E;
+  const size_t e = ((size_t)block * E + threadIdx.x % E) * 4;
+  const int sl = threadIdx.x / E, n = q.elems > e ? (q.elems - e < 4 ? (int)(q.elems - e) : 4) : 0;
+  const bool whole = q.elems % 4 == 0;       // (every slab then starts on a 16-byte boundary)
+  f32x4 v = {0.f, 0.f, 0.f, 0.f};
+  if (n > 0) {
 #pragma unroll 8
-    for (int s = sl; s < q.S; s += 16) v += q.part[(size_t)s * q.elems + e];
-  }
-  __shared__ float red[256];
-  red[threadIdx.x] = v;
-  __syncthreads();
-  if (sl == 0 && e < q.elems) {
-#pragma unroll
-    for (int w2 = 1; w2 < 16; ++w2) v += red[w2 * 16 + threadIdx.x];
-    if (q.f32) {
-      float* o = (float*)q.out + e;
-      *o = accumulate ? *o + v : v;
-    } else {
-      bf16_t* o = (bf16_t*)q.out + e;
-      *o = f2bf(accumulate ? bf2f(*o) + v : v);
+    for (int s = sl; s < q.S; s += L) {
+      const float* r = q.part + (size_t)s * q.elems + e;
+      if (whole) v += *(const f32x4*)r;
+      else v += load4(r, n);
     }
   }
+  red[threadIdx.x] = v;
+  __syncthreads();
+  for (int h = L / 2; h > 0; h >>= 1) {
+    if (sl < h) red[threadIdx.x] += red[threadIdx.x + h * E];
+    __syncthreads();
+  }
+  if (sl == 0) {
+    v = red[threadIdx.x];
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (k < n) {
+        if (q.f32) {
+          float* o = (float*)q.out + e + k;
+          *o = accumulate ? *o + v[k] : v[k];
+        } else {
+          bf16_t* o = (bf16_t*)q.out + e + k;
+          *o = f2bf(accumulate ? bf2f(*o) + v[k] : v[k]);
+        }
+      }
+  }
+}
+constexpr int FOLD_FEW = 32;      // slabs up to which 16 lanes per element do
+__global__ __launch_bounds__(256) void linear_fold_kernel(const FoldP w, const FoldP b, const int accumulate) {
+  __shared__ f32x4 red[256];
+  if ((int)blockIdx.x >= w.blocks) fold<4>(b, blockIdx.x - w.blocks, accumulate, red);
+  else if (w.S > FOLD_FEW) fold<4>(w, blockIdx.x, accumulate, red);
+  else fold<16>(w, blockIdx.x, accumulate, red);
 }
 
 // ------------------------------------------------------------------------------------------------ host side
@@ -722,7 +750,7 @@ BwdPlan bwd_plan(const plyolo_linear_desc* d) {
   const int es = half ? 2 : 4, bk = half ? BK : FK;
   b.dz_ld = (d->N + 7) & ~7;
   b.dz_bytes = d->act == PLYOLO_ACT_NONE ? 0 : up16((size_t)d->M * b.dz_ld * es);
-  b.dzrows = max(32, cdiv(d->M, 512));
+  b.dzrows = max(16, cdiv(d->M, 1024));
   b.dzblk = cdiv(d->M, b.dzrows);
   b.part_off = b.dz_bytes;
   b.part_bytes = up16((size_t)b.dzblk * d->N * 4);
@@ -750,12 +778,13 @@ int check_linear(const plyolo_linear_desc* d, const char* who) {
   return 0;
 }
 
-// tile grid of an I x J output; the column tiles of one row tile are neighbours, so that its rows are read from HBM once
-int tile_grid(LinP& p, int tile, const char* who) {
+// workgroups of an I x J output
+int tile_grid(LinP& p, int tile, int slabs, const char* who) {
   p.nj = cdiv(p.J, tile);
   const int64_t n = (int64_t)cdiv(p.I, tile) * p.nj;
-  PLY_CHECK_ARG(n < 2147483647, "%s: more than 2^31 tiles", who);
-  return (int)n;
+  PLY_CHECK_ARG(n * slabs < 2147483647, "%s: more than 2^31 workgroups", who);
+  p.tiles = (int)n;
+  return (int)n * slabs;
 }
 
 bool rows16(const void* p, int ld, int len) { return (size_t)p % 16 == 0 && ld % 8 == 0 && len % 8 == 0; }
@@ -764,37 +793,37 @@ template <int MODE, int TI, int TJ> size_t tile_lds(size_t stages) {
   const size_t out = MODE == MODE_DW ? 0 : out_bytes<TI, TJ>();
   return out > stages ? out : stages;
 }
-template <int MODE, int T, bool HEAVY> hipError_t launch_any(const LinP& p, int grid, int slabs, hipStream_t s) {
+template <int MODE, int T, bool HEAVY> hipError_t launch_any(const LinP& p, int grid, hipStream_t s) {
   const size_t lds = tile_lds<MODE, T, T>(2 * (size_t)(2 * T) * BK * 2);
   auto k = linear_bf16_any_kernel<MODE, T, T, HEAVY>;
   if (hipError_t e = plyolo::ensure_dynamic_lds((const void*)k, lds); e != hipSuccess) return e;
-  hipLaunchKernelGGL(k, dim3(grid, slabs), dim3(256), lds, s, p);
+  hipLaunchKernelGGL(k, dim3(grid), dim3(256), lds, s, p);
   return hipGetLastError();
 }
-template <int MODE, int NWI, int NWJ, int WI, int WJ, int K, int ST, bool HEAVY> hipError_t launch_direct(const LinP& p, int grid, int slabs, hipStream_t s) {
+template <int MODE, int NWI, int NWJ, int WI, int WJ, int K, int ST, bool HEAVY> hipError_t launch_direct(const LinP& p, int grid, hipStream_t s) {
   constexpr int TI = NWI * WI, TJ = NWJ * WJ;
   const size_t lds = tile_lds<MODE, TI, TJ>(ST * (size_t)(TI + TJ) * K * 2);
   auto k = linear_bf16_kernel<MODE, NWI, NWJ, WI, WJ, K, ST, HEAVY>;
   if (hipError_t e = plyolo::ensure_dynamic_lds((const void*)k, lds); e != hipSuccess) return e;
-  hipLaunchKernelGGL(k, dim3(grid, slabs), dim3(64 * NWI * NWJ), lds, s, p);
+  hipLaunchKernelGGL(k, dim3(grid), dim3(64 * NWI * NWJ), lds, s, p);
   return hipGetLastError();
 }
 // direct: both operands' granules are whole and 16-byte aligned
-template <int MODE, bool HEAVY> hipError_t launch_bf16(const LinP& p, int tile, int grid, int slabs, bool direct, hipStream_t s) {
+template <int MODE, bool HEAVY> hipError_t launch_bf16(const LinP& p, int tile, int grid, bool direct, hipStream_t s) {
   if (direct) {
-    if constexpr (MODE != MODE_DW) if (tile == 256) return launch_direct<MODE, 2, 4, 128, 64, 64, 2, HEAVY>(p, grid, slabs, s);
-    if (tile == 128) return launch_direct<MODE, 2, 2, 64, 64, 64, 2, HEAVY>(p, grid, slabs, s);
-    return launch_direct<MODE, 2, 2, 32, 32, 64, 3, HEAVY>(p, grid, slabs, s);
+    if constexpr (MODE != MODE_DW) if (tile == 256) return launch_direct<MODE, 2, 4, 128, 64, 64, 2, HEAVY>(p, grid, s);
+    if (tile == 128) return launch_direct<MODE, 2, 2, 64, 64, 64, 2, HEAVY>(p, grid, s);
+    return launch_direct<MODE, 2, 2, 32, 32, 64, 3, HEAVY>(p, grid, s);
   }
-  return tile == 128 ? launch_any<MODE, 128, HEAVY>(p, grid, slabs, s) : launch_any<MODE, 64, HEAVY>(p, grid, slabs, s);
+  return tile == 128 ? launch_any<MODE, 128, HEAVY>(p, grid, s) : launch_any<MODE, 64, HEAVY>(p, grid, s);
 }
-template <int MODE> hipError_t launch_gemm(int dtype, const LinP& p, int tile, int grid, int slabs, bool direct, hipStream_t s) {
+template <int MODE> hipError_t launch_gemm(int dtype, const LinP& p, int tile, int grid, bool direct, hipStream_t s) {
   if (dtype != PLYOLO_BF16) {
-    hipLaunchKernelGGL(linear_f32_kernel<MODE>, dim3(grid, slabs), dim3(256), 0, s, p);
+    hipLaunchKernelGGL(linear_f32_kernel<MODE>, dim3(grid), dim3(256), 0, s, p);
     return hipGetLastError();
   }
-  if (MODE == MODE_FWD && p.act > PLYOLO_ACT_LRELU) return launch_bf16<MODE, MODE == MODE_FWD>(p, tile, grid, slabs, direct, s);
-  return launch_bf16<MODE, false>(p, tile, grid, slabs, direct, s);
+  if (MODE == MODE_FWD && p.act > PLYOLO_ACT_LRELU) return launch_bf16<MODE, MODE == MODE_FWD>(p, tile, grid, direct, s);
+  return launch_bf16<MODE, false>(p, tile, grid, direct, s);
 }
 
 }  // namespace
@@ -825,7 +854,7 @@ int plyolo_linear_fwd(const plyolo_linear_desc* d, const void* x, const void* w,
   // 16 x 16 blocks re-read x once per 16 columns and w once per 16 rows; while that is little, they fill the chip where tiles would not
   const double again = (m * k * cdiv(d->N, 16) + n * k * cdiv(d->M, 16)) * es;
   if (again < 32e6) {
-    const int grid = tile_grid(p, 16, "linear_fwd");
+    const int grid = tile_grid(p, 16, 1, "linear_fwd");
     if (grid < 0) return -1;
     const int step = dtype == PLYOLO_BF16 ? 32 : 16;
     int waves = 1;
@@ -840,9 +869,9 @@ int plyolo_linear_fwd(const plyolo_linear_desc* d, const void* x, const void* w,
   }
   const bool direct = rows16(x, d->x_ld, d->K) && rows16(w, d->w_ld, d->K);
   const int tile = dtype == PLYOLO_BF16 ? pick_tile(d->M, d->N, d->K, direct) : FT;
-  const int grid = tile_grid(p, tile, "linear_fwd");
+  const int grid = tile_grid(p, tile, 1, "linear_fwd");
   if (grid < 0) return -1;
-  return plyolo::submit(stream, [=](hipStream_t s) -> hipError_t { return launch_gemm<MODE_FWD>(dtype, p, tile, grid, 1, direct, s); });
+  return plyolo::submit(stream, [=](hipStream_t s) -> hipError_t { return launch_gemm<MODE_FWD>(dtype, p, tile, grid, direct, s); });
 }
 
 int plyolo_linear_bwd(const plyolo_linear_desc* d, const void* dy, const void* z, const void* x, const void* w, void* dx, int dx_ld,
@@ -881,12 +910,12 @@ int plyolo_linear_bwd(const plyolo_linear_desc* d, const void* dy, const void* z
   const int g_len = has_act ? b.dz_ld : d->N;
   const bool dx_direct = rows16(g, g_ld, g_len) && rows16(w, d->w_ld, d->K), dw_direct = rows16(g, g_ld, g_len) && rows16(x, d->x_ld, d->K);
   const int tx = dtype == PLYOLO_BF16 ? pick_tile(d->M, d->K, d->N, dx_direct) : FT;
-  const int gx = tile_grid(px, tx, "linear_bwd"), gw = tile_grid(pw, b.tile, "linear_bwd");
+  const int gx = tile_grid(px, tx, 1, "linear_bwd"), gw = tile_grid(pw, b.tile, b.S, "linear_bwd");
   if (gx < 0 || gw < 0) return -1;
   FoldP fw{}, fb{};
   if (dw) {
     fw.part = (const float*)(ws + b.slab_off); fw.out = dw; fw.elems = (size_t)d->N * d->K; fw.S = b.S; fw.f32 = dw_dtype == PLYOLO_F32;
-    fw.blocks = (int)cdivz(fw.elems, 16);
+    fw.blocks = (int)cdivz(fw.elems, fw.S > FOLD_FEW ? 16 : 64);
   }
   if (db) {
     fb.part = q.part; fb.out = db; fb.elems = (size_t)d->N; fb.S = b.dzblk; fb.f32 = 1;
@@ -901,9 +930,9 @@ int plyolo_linear_bwd(const plyolo_linear_desc* d, const void* dy, const void* z
       else hipLaunchKernelGGL(linear_dz_kernel<float>, dim3(b.dzblk), dim3(256), 0, s, q);
     }
     if (dx)
-      if (hipError_t e = launch_gemm<MODE_DX>(dtype, px, tx, gx, 1, dx_direct, s); e != hipSuccess) return e;
+      if (hipError_t e = launch_gemm<MODE_DX>(dtype, px, tx, gx, dx_direct, s); e != hipSuccess) return e;
     if (dw)
-      if (hipError_t e = launch_gemm<MODE_DW>(dtype, pw, b.tile, gw, b.S, dw_direct, s); e != hipSuccess) return e;
+      if (hipError_t e = launch_gemm<MODE_DW>(dtype, pw, b.tile, gw, dw_direct, s); e != hipSuccess) return e;
     if (dw || db) hipLaunchKernelGGL(linear_fold_kernel, dim3((unsigned)(fw.blocks + fb.blocks)), dim3(256), 0, s, fw, fb, acc);
     return hipGetLastError();
   });
