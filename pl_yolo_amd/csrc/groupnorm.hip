@@ -7,8 +7,9 @@
 // Both directions are HBM streams around one reduction.
 //   resident   a workgroup owns (image, slice of whole groups) and holds its rows in registers across the reduction: one launch, every
 //              operand read once (gn_res_*_kernel).  Taken wherever the slice fits.
-//   streaming  two launches: the first leaves one partial per (image, chunk of rows) in the workspace, the second joins the partials of its
-//              image in a fixed order in its prologue (a few KB out of L2) and streams.
+//   streaming  three launches: partials per (image, chunk of rows) into the workspace, a join of the partials in a fixed order, the stream.
+//              (Joining in the stream's own prologue saves a launch and loses more: every workgroup then reads all partials of its image, and
+//              all of them the same lines at the same time -- 1 x 25600 x 64 forward 35 us at 400 chunks, 87 us at 800.)
 // A thread owns one vector of channels for the whole launch and walks down the rows, as in the BatchNorm kernels.
 //
 // The variance is never formed as E[x^2] - E[x]^2: a thread sums deviations from its own first value, (count, mean, M2) triples are joined
@@ -70,7 +71,7 @@ struct GnP {
   const float* beta;
   float* stats;        // [N][G][2]
   float2* gpart;       // [N][chunks][G]: forward (mean - origin, M2), backward (sum v, sum v xh)
-  float* origin;       // [N][G]: the forward's origins, kept because the second launch may write over x
+  float2* gmean;       // [N][G]: backward (mean v, mean v xh)
   float2* cpart;       // [N][chunks][C]: backward (sum du, sum du xh)
   float* dgamma;
   float* dbeta;
@@ -167,63 +168,67 @@ template <typename T, int V> __global__ __launch_bounds__(256) void gn_stats_ker
         m2 += o.y + d * d * (float)nr;
       }
     m2 = lane_sum(m2, L);
-    if (on && gl == 0) {
-      p.gpart[((size_t)n * p.chunks + j) * p.G + g] = make_float2(mean, m2);
-      if (j == 0) p.origin[(size_t)n * p.G + g] = gn_origin<T>(p, n, g);
-    }
+    if (on && gl == 0) p.gpart[((size_t)n * p.chunks + j) * p.G + g] = make_float2(mean, m2);
   }
 }
 
-// joins the chunk partials of image n: gm[2 g], gm[2 g + 1] = mean, rstd.  A lane requests its (up to) 16 partials before it uses the first:
-// the joins are one round trip to L2, not one per partial.
-DEVINL void gn_join_stats(const GnP& p, int n, float* gm) {
-  const int L = join_lanes(p.G), gl = threadIdx.x % L, gstep = 256 / L;
-  const float2* part = p.gpart + (size_t)n * p.chunks * p.G;
-  const double total = (double)p.HW * p.cg;
-  for (int g0 = 0; g0 < p.G; g0 += gstep) {
-    const int g = g0 + threadIdx.x / L;
-    const bool on = g < p.G;
-    const int gc = min(g, p.G - 1);
-    float2 o[16];
-    double sm = 0.0;
-    for (int j0 = gl; j0 < p.chunks; j0 += 16 * L) {
+// Joins: 32 items (groups of an image, or channels) x NT / 32 lanes per workgroup, a lane's partials requested sixteen at a time, lanes added
+// in a fixed order.  fp64: the two sums of a group are then enough, however far its mean lies from the origin.
+constexpr int JOIN_I = 32, JOIN_FEW = 128;      // up to that many partials eight lanes per item do (NT 256; beyond, 32 lanes)
+template <int JOIN_NT> DEVINL void join_sums(const float2* part, int stride, int count, bool live, double& a, double& b, const float full, const float tail) {
+  __shared__ double da[JOIN_NT], db[JOIN_NT];
+  const int lane = threadIdx.x / JOIN_I, last = count - 1;
+  a = b = 0.0;
+  if (live)
+    for (int j0 = lane; j0 < count; j0 += 16 * (JOIN_NT / JOIN_I)) {
+      float2 o[16];
+#pragma unroll
+      for (int k = 0; k < 16; ++k) o[k] = part[(size_t)min(j0 + k * (JOIN_NT / JOIN_I), last) * stride];
 #pragma unroll
       for (int k = 0; k < 16; ++k) {
-        const int j = j0 + k * L;
-        o[k] = part[min(j, p.chunks - 1) * p.G + gc];       // (no branch around a request: a chunk beyond the last has no rows, weight 0)
-      }
-#pragma unroll
-      for (int k = 0; k < 16; ++k) sm += (double)o[k].x * (double)max(min(p.HW - (j0 + k * L) * p.rows, p.rows), 0);
-    }
-    const double mean = lane_sum(sm, L) / (double)p.HW;
-    double m2 = 0.0;
-    for (int j0 = gl; j0 < p.chunks; j0 += 16 * L) {
-      if (p.chunks > 16 * L) {
-#pragma unroll
-        for (int k = 0; k < 16; ++k) {
-          const int j = j0 + k * L;
-          o[k] = part[min(j, p.chunks - 1) * p.G + gc];
+        const int j = j0 + k * (JOIN_NT / JOIN_I);
+        if (j > last) continue;
+        if (full > 0.f) {      // (mean - origin, M2) of `full` values (the last: `tail`) -> sum, sum of squares
+          const double w = j < last ? (double)full : (double)tail;
+          a += w * (double)o[k].x;
+          b += (double)o[k].y + w * (double)o[k].x * (double)o[k].x;
+        } else {
+          a += (double)o[k].x;
+          b += (double)o[k].y;
         }
       }
-#pragma unroll
-      for (int k = 0; k < 16; ++k) {
-        const double d = (double)o[k].x - mean;
-        const double m = (double)o[k].y + d * d * ((double)min(p.HW - (j0 + k * L) * p.rows, p.rows) * p.cg);
-        m2 += j0 + k * L < p.chunks ? m : 0.0;
-      }
     }
-    m2 = lane_sum(m2, L);
-    if (on && gl == 0) {
-      gm[2 * g] = (float)(mean + (double)p.origin[(size_t)n * p.G + g]);
-      gm[2 * g + 1] = (float)(1.0 / sqrt(m2 / total + (double)p.eps));
+  da[threadIdx.x] = a;
+  db[threadIdx.x] = b;
+  __syncthreads();
+  for (int h = JOIN_NT / 2; h >= JOIN_I; h >>= 1) {
+    if ((int)threadIdx.x < h) {
+      da[threadIdx.x] += da[threadIdx.x + h];
+      db[threadIdx.x] += db[threadIdx.x + h];
     }
+    __syncthreads();
+  }
+  a = da[threadIdx.x % JOIN_I];
+  b = db[threadIdx.x % JOIN_I];
+}
+
+template <typename T, int JOIN_NT> __global__ __launch_bounds__(JOIN_NT) void gn_join_fwd_kernel(const GnP p) {
+  const int gb = (p.G + JOIN_I - 1) / JOIN_I, n = blockIdx.x / gb, g = (blockIdx.x % gb) * JOIN_I + threadIdx.x % JOIN_I;
+  const bool live = g < p.G;
+  double s, q;
+  join_sums<JOIN_NT>(p.gpart + (size_t)n * p.chunks * p.G + g, p.G, p.chunks, live, s, q, (float)p.rows * (float)p.cg,
+            (float)(p.HW - (p.chunks - 1) * p.rows) * (float)p.cg);
+  if (live && (int)threadIdx.x < JOIN_I) {
+    const double total = (double)p.HW * p.cg, mean = s / total, m2 = q - s * mean;
+    float* st = p.stats + ((size_t)n * p.G + g) * 2;
+    st[0] = (float)(mean + (double)gn_origin<T>(p, n, g));
+    st[1] = (float)(1.0 / sqrt((m2 < 0.0 ? 0.0 : m2) / total + (double)p.eps));
   }
 }
 
 constexpr int GN_U = 4;    // rows a thread has in flight
 
 template <typename T, int V, int ACTC> __global__ __launch_bounds__(256) void gn_apply_kernel(const GnP p) {
-  extern __shared__ float gm[];                // [G][2]
   // last chunk first: what the statistics read last is still in the last-level cache
   const int blk = gridDim.x - 1 - blockIdx.x, n = blk / p.chunks, j = blk % p.chunks;
   const int r0 = j * p.rows, nr = min(p.HW - r0, p.rows);
@@ -234,7 +239,6 @@ template <typename T, int V, int ACTC> __global__ __launch_bounds__(256) void gn
   typedef typename Lane<T, V>::raw raw_t;
   raw_t rx[GN_U], rr[GN_U];
   const bool rows_mine = trow < rpb;
-  // the first rows and the affine pair are requested in front of the join, so that its round trips to L2 run beside them
   auto request = [&](const int col, const int r) {
     const T* px = (const T*)p.x + row0 * p.x_ld + (size_t)col * V;
     const T* pr = (const T*)p.res + row0 * p.r_ld + (size_t)col * V;
@@ -246,32 +250,16 @@ template <typename T, int V, int ACTC> __global__ __launch_bounds__(256) void gn
       }
   };
   float a[V], b[V], mu[V];
-  auto affine = [&](const int col) {
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      a[e] = p.gamma ? p.gamma[col * V + e] : 1.f;
-      b[e] = p.beta ? p.beta[col * V + e] : 0.f;
-    }
-  };
-  if (rows_mine) {
-    request(tcol, trow);
-    affine(tcol);
-  }
-  gn_join_stats(p, n, gm);
-  __syncthreads();
-  if (j == 0)
-    for (int t = threadIdx.x; t < 2 * p.G; t += 256) p.stats[(size_t)n * 2 * p.G + t] = gm[t];
   if (!rows_mine) return;
+  const float* st = p.stats + (size_t)n * 2 * p.G;
   for (int col = tcol; col < cv; col += cols) {
-    if (col != tcol) {
-      request(col, trow);
-      affine(col);
-    }
+    request(col, trow);
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-      const int g = (col * V + e) / p.cg;
-      mu[e] = gm[2 * g];
-      a[e] *= gm[2 * g + 1];
+      const int c = col * V + e, g = c / p.cg;
+      mu[e] = st[2 * g];
+      a[e] = st[2 * g + 1] * (p.gamma ? p.gamma[c] : 1.f);
+      b[e] = p.beta ? p.beta[c] : 0.f;
     }
     T* po = (T*)p.out + row0 * p.o_ld + (size_t)col * V;
     for (int r = trow; r < nr; r += GN_U * rpb) {
@@ -397,76 +385,36 @@ template <typename T, int V, int ACTC> __global__ __launch_bounds__(256) void gn
   }
 }
 
-constexpr int GN_PC = 32;    // channels per parameter workgroup
-
-// dgamma / dbeta of GN_PC channels from `parts` per-channel partials, in a fixed order (256 threads)
-DEVINL void gn_params(const GnP& p, int block, size_t parts) {
-  __shared__ double da[256], db[256];
-  const int c = block * GN_PC + threadIdx.x % GN_PC, lane = threadIdx.x / GN_PC;
-  double a = 0.0, b = 0.0;
-  if (c < p.C) {
-#pragma unroll 8
-    for (size_t i = lane; i < parts; i += 256 / GN_PC) {
-      const float2 o = p.cpart[i * p.C + c];
-      a += (double)o.x;
-      b += (double)o.y;
-    }
-  }
-  da[threadIdx.x] = a;
-  db[threadIdx.x] = b;
-  __syncthreads();
-  if (lane == 0 && c < p.C) {
-    for (int w = 1; w < 256 / GN_PC; ++w) {
-      a += da[w * GN_PC + threadIdx.x];
-      b += db[w * GN_PC + threadIdx.x];
-    }
-    if (p.dbeta) p.dbeta[c] = (float)(a + (p.acc_par ? (double)p.dbeta[c] : 0.0));
-    if (p.dgamma) p.dgamma[c] = (float)(b + (p.acc_par ? (double)p.dgamma[c] : 0.0));
-  }
-}
-__global__ __launch_bounds__(256) void gn_params_kernel(const GnP p) { gn_params(p, blockIdx.x, (size_t)p.N); }
-
-// workgroups [0, npar): dgamma / dbeta of GN_PC channels, summed over all chunks in a fixed order; the others: dx of one chunk of rows
-template <typename T, int V, int ACTC> __global__ __launch_bounds__(256) void gn_bwd_dx_kernel(const GnP p, const int npar) {
-  extern __shared__ float gm[];                // [G][2]: the two means of the group
-  const int act = ACTC >= 0 ? ACTC : p.act;
+// workgroups [0, npar): dgamma / dbeta of 32 channels from `parts` per-channel partials; the others: the two means of 32 groups of an image
+template <int JOIN_NT> __global__ __launch_bounds__(JOIN_NT) void gn_join_bwd_kernel(const GnP p, const int npar, const int parts) {
+  double a, b;
   if ((int)blockIdx.x < npar) {
-    gn_params(p, blockIdx.x, (size_t)p.N * p.chunks);
+    const int c = blockIdx.x * JOIN_I + threadIdx.x % JOIN_I;
+    join_sums<JOIN_NT>(p.cpart + c, p.C, parts, c < p.C, a, b, 0.f, 0.f);
+    if (c < p.C && (int)threadIdx.x < JOIN_I) {
+      if (p.dbeta) p.dbeta[c] = (float)(a + (p.acc_par ? (double)p.dbeta[c] : 0.0));
+      if (p.dgamma) p.dgamma[c] = (float)(b + (p.acc_par ? (double)p.dgamma[c] : 0.0));
+    }
     return;
   }
+  const int blk = blockIdx.x - npar, gb = (p.G + JOIN_I - 1) / JOIN_I, n = blk / gb, g = (blk % gb) * JOIN_I + threadIdx.x % JOIN_I;
+  join_sums<JOIN_NT>(p.gpart + (size_t)n * p.chunks * p.G + g, p.G, p.chunks, g < p.G, a, b, 0.f, 0.f);
+  if (g < p.G && (int)threadIdx.x < JOIN_I) {
+    const double inv = 1.0 / ((double)p.HW * p.cg);
+    p.gmean[(size_t)n * p.G + g] = make_float2((float)(a * inv), (float)(b * inv));
+  }
+}
+
+template <typename T, int V, int ACTC> __global__ __launch_bounds__(256) void gn_bwd_dx_kernel(const GnP p) {
+  const int act = ACTC >= 0 ? ACTC : p.act;
   const int blk = gridDim.x - 1 - blockIdx.x, n = blk / p.chunks, j = blk % p.chunks;      // last chunk first, as in gn_apply_kernel
   const int r0 = j * p.rows, nr = min(p.HW - r0, p.rows);
-  {
-    const int L = join_lanes(p.G), gl = threadIdx.x % L, gstep = 256 / L;
-    const float2* part = p.gpart + (size_t)n * p.chunks * p.G;
-    const double inv = 1.0 / ((double)p.HW * p.cg);
-    for (int g0 = 0; g0 < p.G; g0 += gstep) {
-      const int g = g0 + threadIdx.x / L;
-      double a = 0.0, b = 0.0;
-      for (int j0 = gl; j0 < p.chunks; j0 += 16 * L) {
-        float2 o[16];
-#pragma unroll
-        for (int k = 0; k < 16; ++k) o[k] = part[min(j0 + k * L, p.chunks - 1) * p.G + min(g, p.G - 1)];
-#pragma unroll
-        for (int k = 0; k < 16; ++k) {
-          a += j0 + k * L < p.chunks ? (double)o[k].x : 0.0;
-          b += j0 + k * L < p.chunks ? (double)o[k].y : 0.0;
-        }
-      }
-      a = lane_sum(a, L);
-      b = lane_sum(b, L);
-      if (g < p.G && gl == 0) {
-        gm[2 * g] = (float)(a * inv);
-        gm[2 * g + 1] = (float)(b * inv);
-      }
-    }
-  }
-  __syncthreads();
   const int cv = p.C / V, cols = min(cv, 256), rpb = 256 / cols;
   const int tcol = threadIdx.x % cols, trow = threadIdx.x / cols;
   if (trow >= rpb) return;
   const size_t row0 = (size_t)n * p.HW + r0;
   const float* st = p.stats + (size_t)n * 2 * p.G;
+  const float2* gm = p.gmean + (size_t)n * p.G;
   for (int col = tcol; col < cv; col += cols) {
     float mu[V], ga[V], be[V], k0[V], k1[V];      // dx = (rs gamma) du + k0 + k1 c with c = x - mean
 #pragma unroll
@@ -476,8 +424,8 @@ template <typename T, int V, int ACTC> __global__ __launch_bounds__(256) void gn
       mu[e] = st[2 * g];
       ga[e] = rs * (p.gamma ? p.gamma[c] : 1.f);
       be[e] = p.beta ? p.beta[c] : 0.f;
-      k0[e] = -rs * gm[2 * g];
-      k1[e] = -rs * rs * gm[2 * g + 1];
+      k0[e] = -rs * gm[g].x;
+      k1[e] = -rs * rs * gm[g].y;
     }
     const T* px = (const T*)p.x + row0 * p.x_ld + (size_t)col * V;
     const T* pd = (const T*)p.dout + row0 * p.d_ld + (size_t)col * V;
@@ -785,12 +733,12 @@ template <typename T, int V, int NV, int ACTC> __global__ __launch_bounds__(RES_
 
 // ------------------------------------------------------------------------------------------------ host side
 // Row chunks of one image in the streaming launches.  A function of the descriptor's sizes alone, so that the workspace does not depend on
-// addresses: four workgroups per compute unit over the whole batch (with eight the joins cost more than they hide: backward of
-// 8 x 25600 x 320 bf16 171 instead of 150 us), and at least 8192 values per chunk.
+// addresses: four workgroups per compute unit over the whole batch (eight: 8 x 6400 x 320 bf16 forward 49 instead of 38 us), and at least 8192
+// values per chunk (2048 where that would leave fewer than 128 workgroups).
 void gn_chunks(const plyolo_gn_desc* d, int* chunks, int* rows) {
   const int64_t all = (int64_t)d->N * d->HW;
   int64_t r = (all + 1023) / 1024;
-  const int64_t least = (8192 + d->C - 1) / d->C;
+  const int64_t values = all * d->C / 128, least = (min(max(values, (int64_t)2048), (int64_t)8192) + d->C - 1) / d->C;
   if (r < least) r = least;
   if (r > d->HW) r = d->HW;
   *rows = (int)r;
@@ -813,7 +761,7 @@ int check_gn(const plyolo_gn_desc* d, const char* who) {
 size_t gn_ws_bytes(const plyolo_gn_desc* d) {
   int chunks, rows;
   gn_chunks(d, &chunks, &rows);
-  return (size_t)d->N * (chunks * ((size_t)d->groups + d->C) * sizeof(float2) + d->groups * sizeof(float));
+  return (size_t)d->N * (chunks * ((size_t)d->groups + d->C) + d->groups) * sizeof(float2);
 }
 
 GnP gn_params(const plyolo_gn_desc* d, void* ws) {
@@ -823,7 +771,7 @@ GnP gn_params(const plyolo_gn_desc* d, void* ws) {
   gn_chunks(d, &p.chunks, &p.rows);
   p.gpart = (float2*)ws;
   p.cpart = p.gpart + (size_t)p.N * p.chunks * p.G;
-  p.origin = (float*)(p.cpart + (size_t)p.N * p.chunks * p.C);
+  p.gmean = p.cpart + (size_t)p.N * p.chunks * p.C;
   return p;
 }
 
@@ -870,6 +818,11 @@ ResPlan res_plan(const plyolo_gn_desc* d, int V, bool bwd) {
                                     : KERN<bf16_t, 1, -1>)                                                                      \
                           : ((wide) ? KERN<float, 4, -1> : KERN<float, 1, -1>))
 
+void join_bwd(const GnP& p, int npar, int nmean, int parts, hipStream_t s) {
+  if (parts <= JOIN_FEW) hipLaunchKernelGGL(gn_join_bwd_kernel<256>, dim3((unsigned)(npar + nmean)), dim3(256), 0, s, p, npar, parts);
+  else hipLaunchKernelGGL(gn_join_bwd_kernel<1024>, dim3((unsigned)(npar + nmean)), dim3(1024), 0, s, p, npar, parts);
+}
+
 }  // namespace
 
 extern "C" {
@@ -908,8 +861,12 @@ int plyolo_gn_act_fwd(const plyolo_gn_desc* d, const void* x, const float* gamma
     auto ks = dtype == PLYOLO_BF16 ? (wide ? gn_stats_kernel<bf16_t, 8> : gn_stats_kernel<bf16_t, 1>) : (wide ? gn_stats_kernel<float, 4> : gn_stats_kernel<float, 1>);
     auto ka = GN_DISPATCH(dtype, wide, act, gn_apply_kernel);
     const dim3 grid((unsigned)p.N * p.chunks), blk(256);
+    const bool few = p.chunks <= JOIN_FEW;
+    auto kj = dtype == PLYOLO_BF16 ? (few ? gn_join_fwd_kernel<bf16_t, 256> : gn_join_fwd_kernel<bf16_t, 1024>)
+                                   : (few ? gn_join_fwd_kernel<float, 256> : gn_join_fwd_kernel<float, 1024>);
     hipLaunchKernelGGL(ks, grid, blk, (size_t)p.C * sizeof(float2), s, p);
-    hipLaunchKernelGGL(ka, grid, blk, (size_t)p.G * sizeof(float2), s, p);
+    hipLaunchKernelGGL(kj, dim3((unsigned)p.N * cdiv(p.G, JOIN_I)), dim3(few ? 256 : 1024), 0, s, p);
+    hipLaunchKernelGGL(ka, grid, blk, 0, s, p);
     return hipGetLastError();
   });
 }
@@ -939,7 +896,7 @@ int plyolo_gn_act_bwd(const plyolo_gn_desc* d, const void* dout, int d_ld, const
     return plyolo::submit(stream, [=](hipStream_t s) -> hipError_t {
       auto k = GN_RES_DISPATCH(dtype, wide, act, GN_RES_BWD, gn_res_bwd_kernel, rp.nv);
       hipLaunchKernelGGL(k, dim3((unsigned)p.N * rp.slices), dim3(RES_NT), lds, s, q);
-      if (p.N > 1 && (p.dgamma || p.dbeta)) hipLaunchKernelGGL(gn_params_kernel, dim3((unsigned)((p.C + GN_PC - 1) / GN_PC)), dim3(256), 0, s, p);
+      if (p.N > 1 && (p.dgamma || p.dbeta)) join_bwd(p, cdiv(p.C, JOIN_I), 0, p.N, s);
       return hipGetLastError();
     });
   }
@@ -947,9 +904,10 @@ int plyolo_gn_act_bwd(const plyolo_gn_desc* d, const void* dout, int d_ld, const
     auto ks = GN_DISPATCH(dtype, wide, act, gn_bwd_sums_kernel);
     auto kd = GN_DISPATCH(dtype, wide, act, gn_bwd_dx_kernel);
     const unsigned nblk = (unsigned)p.N * p.chunks;
-    const int npar = (p.dgamma || p.dbeta) ? (p.C + GN_PC - 1) / GN_PC : 0;
+    const int npar = (p.dgamma || p.dbeta) ? cdiv(p.C, JOIN_I) : 0;
     hipLaunchKernelGGL(ks, dim3(nblk), dim3(256), (size_t)p.C * sizeof(float2), s, p);
-    hipLaunchKernelGGL(kd, dim3(nblk + npar), dim3(256), (size_t)p.G * sizeof(float2), s, p, npar);
+    join_bwd(p, npar, p.N * cdiv(p.G, JOIN_I), p.N * p.chunks, s);
+    hipLaunchKernelGGL(kd, dim3(nblk), dim3(256), 0, s, p);
     return hipGetLastError();
   });
 }

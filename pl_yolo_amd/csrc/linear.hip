@@ -50,6 +50,17 @@ DEVINL u32x4 load8(const bf16_t* p, int n) {
   return v;
 }
 
+// drops the first e (1 .. 7) of eight elements
+DEVINL u32x4 shift_out(u32x4 v, int e) {
+  uint64_t lo = (uint64_t)v[1] << 32 | v[0], hi = (uint64_t)v[3] << 32 | v[2];
+  if (e >= 4) { lo = hi; hi = 0; e -= 4; }
+  if (e > 0) {
+    lo = lo >> (16 * e) | hi << (64 - 16 * e);
+    hi >>= 16 * e;
+  }
+  return u32x4{(unsigned)lo, (unsigned)(lo >> 32), (unsigned)hi, (unsigned)(hi >> 32)};
+}
+
 DEVINL void store8(bf16_t* p, int n, u32x4 v) {
   if (n >= 8) {
     *(u32x4_any*)p = v;
@@ -78,7 +89,8 @@ template <int TI, int TJ> DEVINL Place place(const LinP& p) {
 // RC image: [K][T] elements, rows of T / 16 32-byte segments, segment s of row k at position s ^ f(k): the 16 rows that one transposed read
 // of a wave touches spread over all banks.
 // DIRECT: whole granules at 16-byte addresses go to LDS without passing registers (a lane's destination is fixed by the instruction, so the
-// swizzle is applied to its source); otherwise through registers, granule by granule, with tails element by element.
+// swizzle is applied to its source); otherwise through registers: a granule that a row's end cuts is fetched as the row's last eight elements
+// and shifted on its way to LDS, so that no request waits for another (rows of fewer than eight elements: one by one).
 template <bool RC, int T, int K, int NT, bool DIRECT> struct Tile {
   static constexpr int NG = T * K / 8 / NT;      // 16-byte granules per thread
   static constexpr int BYTES = T * K * 2, KG = K / 8, TG = T / 8;
@@ -89,8 +101,12 @@ template <bool RC, int T, int K, int NT, bool DIRECT> struct Tile {
   int kof[NG];               // its contraction offset inside a stage
   u32x4 v[DIRECT ? 1 : NG];
   int len[DIRECT ? 1 : NG];  // RC: elements of the granule that exist
+  int cut[DIRECT ? 1 : NG];  // of the granule in v: elements to shift out
+  bool few;                  // rows of fewer than eight elements
 
-  DEVINL void init(const bf16_t* base, int ld, int row0, int rows, int kbeg) {
+  // clen: contraction elements of the whole operand
+  DEVINL void init(const bf16_t* base, int ld, int row0, int rows, int kbeg, int clen) {
+    few = (RC ? rows : clen) < 8;
 #pragma unroll
     for (int u = 0; u < NG; ++u) {
       const int idx = threadIdx.x + u * NT;
@@ -120,15 +136,19 @@ template <bool RC, int T, int K, int NT, bool DIRECT> struct Tile {
         __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)g,
                                          (__attribute__((address_space(3))) void*)(img + (u * NT + wave * 64) * 16), 16, 0, 0);
       } else {
-        v[DIRECT ? 0 : u] = ok ? load8(q, RC ? len[DIRECT ? 0 : u] : left - kof[u]) : u32x4{0u, 0u, 0u, 0u};
+        const int w = DIRECT ? 0 : u, n = RC ? len[w] : left - kof[u];
+        cut[w] = ok && n < 8 && !few ? 8 - n : 0;
+        if (few) v[w] = ok ? load8(q, n) : u32x4{0u, 0u, 0u, 0u};
+        else v[w] = *(ok ? (const u32x4_any*)(q - cut[w]) : (const u32x4_any*)&zero_granule);
       }
     }
   }
-  DEVINL void commit(unsigned char* img) const {
+  DEVINL void commit(unsigned char* img) {
     if (DIRECT) return;
 #pragma unroll
     for (int u = 0; u < NG; ++u) {
       const int idx = threadIdx.x + u * NT;
+      if (cut[DIRECT ? 0 : u]) v[DIRECT ? 0 : u] = shift_out(v[DIRECT ? 0 : u], cut[DIRECT ? 0 : u]);
       if (RC) {
         const int k = idx / TG, g = idx % TG;
         *(u32x4*)(img + k * (T * 2) + (((g >> 1) ^ swz_k(k)) << 5) + ((g & 1) << 4)) = v[DIRECT ? 0 : u];
@@ -334,8 +354,8 @@ template <int MODE, int TI, int TJ, bool HEAVY> __global__ __launch_bounds__(256
   const Bias<MODE, FB> bias(p, j0 + wj);
   TA ta;
   TB tb;
-  ta.init((const bf16_t*)p.a, p.a_ld, i0, p.I, kbeg);
-  tb.init((const bf16_t*)p.b, p.b_ld, j0, p.J, kbeg);
+  ta.init((const bf16_t*)p.a, p.a_ld, i0, p.I, kbeg, p.Kc);
+  tb.init((const bf16_t*)p.b, p.b_ld, j0, p.J, kbeg, p.Kc);
   ta.request(smem, 0, p.a_ld, klen);
   tb.request(smem, 0, p.b_ld, klen);
   int buf = 0;
@@ -393,8 +413,8 @@ __global__ __launch_bounds__(64 * NWI * NWJ) void linear_bf16_kernel(const LinP 
   const Bias<MODE, FB> bias(p, j0 + wj);
   TA ta;
   TB tb;
-  ta.init((const bf16_t*)p.a, p.a_ld, i0, p.I, kbeg);
-  tb.init((const bf16_t*)p.b, p.b_ld, j0, p.J, kbeg);
+  ta.init((const bf16_t*)p.a, p.a_ld, i0, p.I, kbeg, p.Kc);
+  tb.init((const bf16_t*)p.b, p.b_ld, j0, p.J, kbeg, p.Kc);
   for (int s = 0; s < ST - 1 && s * K < klen; ++s) {
     ta.request(smem + s * STAGE, s * K, p.a_ld, klen - s * K);
     tb.request(smem + s * STAGE + TA::BYTES, s * K, p.b_ld, klen - s * K);
@@ -743,11 +763,26 @@ int pick_tile(int64_t I, int64_t J, int64_t Kc, bool direct) {
   return 64;
 }
 
-// Slabs of dw: enough row ranges to give every compute unit a workgroup, at least four stages each.
+// Tile and slabs of dw: enough row ranges to give every compute unit a workgroup, as long as the slabs are not more to move than the operands;
+// a layer that does not get there with 128 x 128 tiles takes small ones.
+void dw_plan(const plyolo_linear_desc* d, int tile, BwdPlan* b) {
+  const bool half = d->dtype == PLYOLO_BF16;
+  const int64_t tiles = (int64_t)cdiv(d->N, tile) * cdiv(d->K, tile);
+  const int steps = cdiv(d->M, half ? BK : FK);
+  const double slab = 4.0 * d->N * d->K, operands = (half ? 2.0 : 4.0) * d->M * ((double)d->N + d->K);
+  int64_t s = (256 + tiles - 1) / tiles;
+  if (s > operands / slab) s = (int64_t)(operands / slab);
+  if (s > steps) s = steps;
+  if (s < 1) s = 1;
+  b->tile = tile;
+  b->ksteps = (int)((steps + s - 1) / s);
+  b->S = (steps + b->ksteps - 1) / b->ksteps;
+}
+
 BwdPlan bwd_plan(const plyolo_linear_desc* d) {
   BwdPlan b{};
   const bool half = d->dtype == PLYOLO_BF16;
-  const int es = half ? 2 : 4, bk = half ? BK : FK;
+  const int es = half ? 2 : 4;
   b.dz_ld = (d->N + 7) & ~7;
   b.dz_bytes = d->act == PLYOLO_ACT_NONE ? 0 : up16((size_t)d->M * b.dz_ld * es);
   b.dzrows = max(16, cdiv(d->M, 1024));
@@ -755,14 +790,12 @@ BwdPlan bwd_plan(const plyolo_linear_desc* d) {
   b.part_off = b.dz_bytes;
   b.part_bytes = up16((size_t)b.dzblk * d->N * 4);
   b.slab_off = b.part_off + b.part_bytes;
-  b.tile = half ? (d->N > 64 && d->K > 64 ? 128 : 64) : FT;
-  const int64_t tiles = (int64_t)cdiv(d->N, b.tile) * cdiv(d->K, b.tile);
-  const int steps = cdiv(d->M, bk);
-  int64_t s = (256 + tiles - 1) / tiles;
-  if (s > (steps + 3) / 4) s = (steps + 3) / 4;
-  if (s < 1) s = 1;
-  b.ksteps = (int)((steps + s - 1) / s);
-  b.S = (steps + b.ksteps - 1) / b.ksteps;
+  if (half) {
+    dw_plan(d, 128, &b);
+    if ((int64_t)b.S * cdiv(d->N, 128) * cdiv(d->K, 128) < 128) dw_plan(d, 64, &b);
+  } else {
+    dw_plan(d, FT, &b);
+  }
   b.slab_bytes = up16((size_t)b.S * d->N * d->K * 4);
   b.total = b.slab_off + b.slab_bytes;
   return b;
