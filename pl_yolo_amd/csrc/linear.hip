@@ -79,8 +79,8 @@ DEVINL int xcd_contiguous(int id, int n) {      // hardware deals workgroup ids 
 // Output tile and (MODE_DW) contraction slab of a workgroup.  Neighbours read the same rows, so they get neighbouring ids on one XCD and its L2
 // serves all but the first of them: column tiles of one row tile, and all tiles of one slab.
 struct Place { int i0, j0, slab; };
-template <int TI, int TJ> DEVINL Place place(const LinP& p) {
-  const int id = xcd_contiguous(blockIdx.x, gridDim.x), tile = id % p.tiles;
+template <int TI, int TJ> DEVINL Place place(const LinP& p, int block, int blocks) {
+  const int id = xcd_contiguous(block, blocks), tile = id % p.tiles;
   return Place{tile / p.nj * TI, tile % p.nj * TJ, id / p.tiles};
 }
 
@@ -335,13 +335,13 @@ template <int WI, int WJ> DEVINL void slab_out(const LinP& p, int slab, int i0, 
 
 // Any size, pitch and alignment: TI x TJ tile, four waves of TI / 2 x TJ / 2, operands through registers into two LDS images, one barrier per
 // stage: stage s + 1 is requested behind the barrier of stage s and lands under its MFMAs.
-template <int MODE, int TI, int TJ, bool HEAVY> __global__ __launch_bounds__(256) void linear_bf16_any_kernel(const LinP p) {
+template <int MODE, int TI, int TJ, bool HEAVY> DEVINL void any_tile(const LinP& p, int block, int blocks) {
   constexpr bool ARC = MODE == MODE_DW, BRC = MODE != MODE_FWD;
   typedef Tile<ARC, TI, BK, 256, false> TA;
   typedef Tile<BRC, TJ, BK, 256, false> TB;
   constexpr int FA = TI / 32, FB = TJ / 32, STAGE = TA::BYTES + TB::BYTES;
   extern __shared__ __align__(16) unsigned char smem[];
-  const Place at = place<TI, TJ>(p);
+  const Place at = place<TI, TJ>(p, block, blocks);
   const int i0 = at.i0, j0 = at.j0;
   const int wave = threadIdx.x >> 6, wi = (wave >> 1) * (TI / 2), wj = (wave & 1) * (TJ / 2);
   const int kbeg = at.slab * p.ksteps * BK;
@@ -391,8 +391,7 @@ template <int MODE, int TI, int TJ, bool HEAVY> __global__ __launch_bounds__(256
 // free for the youngest request.
 template <int N> DEVINL void wait_and_meet() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory"); }
 
-template <int MODE, int NWI, int NWJ, int WI, int WJ, int K, int ST, bool HEAVY>
-__global__ __launch_bounds__(64 * NWI * NWJ) void linear_bf16_kernel(const LinP p) {
+template <int MODE, int NWI, int NWJ, int WI, int WJ, int K, int ST, bool HEAVY> DEVINL void direct_tile(const LinP& p, int block, int blocks) {
   constexpr bool ARC = MODE == MODE_DW, BRC = MODE != MODE_FWD;
   constexpr int NT = 64 * NWI * NWJ, TI = NWI * WI, TJ = NWJ * WJ, FA = WI / 16, FB = WJ / 16;
   typedef Tile<ARC, TI, K, NT, true> TA;
@@ -400,7 +399,7 @@ __global__ __launch_bounds__(64 * NWI * NWJ) void linear_bf16_kernel(const LinP 
   constexpr int STAGE = TA::BYTES + TB::BYTES, LOADS = TA::NG + TB::NG;
   static_assert(ST >= 2 && ST <= 4, "the waits below");
   extern __shared__ __align__(16) unsigned char smem[];
-  const Place at = place<TI, TJ>(p);
+  const Place at = place<TI, TJ>(p, block, blocks);
   const int i0 = at.i0, j0 = at.j0;
   const int wave = threadIdx.x >> 6, wi = wave / NWJ * WI, wj = wave % NWJ * WJ;
   const int kbeg = at.slab * p.ksteps * BK;
@@ -456,6 +455,27 @@ __global__ __launch_bounds__(64 * NWI * NWJ) void linear_bf16_kernel(const LinP 
   }
   if (MODE == MODE_DW) slab_out<WI, WJ>(p, at.slab, i0 + wi, j0 + wj, acc);
   else tile_out<MODE, TI, TJ, NT, WI, WJ, HEAVY>(p, smem, i0, j0, wi, wj, acc, bias);
+}
+
+template <int MODE, int T, bool HEAVY> __global__ __launch_bounds__(256) void linear_bf16_any_kernel(const LinP p) {
+  any_tile<MODE, T, T, HEAVY>(p, blockIdx.x, gridDim.x);
+}
+template <int MODE, int NWI, int NWJ, int WI, int WJ, int K, int ST, bool HEAVY>
+__global__ __launch_bounds__(64 * NWI * NWJ) void linear_bf16_kernel(const LinP p) {
+  direct_tile<MODE, NWI, NWJ, WI, WJ, K, ST, HEAVY>(p, blockIdx.x, gridDim.x);
+}
+// Both products of the backward in one launch: workgroups [0, nw) form dw (few and long), the others dx (many and short) beside them.  Alone,
+// neither keeps the memory system busy: 51200 x 256 x 256 19 + 20 us one after the other, 30 us together.
+template <int T, bool DIRECT> __global__ __launch_bounds__(256) void linear_bf16_bwd_kernel(const LinP px, const LinP pw, const int nw) {
+  const bool first = (int)blockIdx.x < nw;
+  const int block = first ? blockIdx.x : blockIdx.x - nw, blocks = first ? nw : gridDim.x - nw;
+  if constexpr (DIRECT) {
+    if (first) direct_tile<MODE_DW, 2, 2, T / 2, T / 2, 64, 2, false>(pw, block, blocks);
+    else direct_tile<MODE_DX, 2, 2, T / 2, T / 2, 64, 2, false>(px, block, blocks);
+  } else {
+    if (first) any_tile<MODE_DW, T, T, false>(pw, block, blocks);
+    else any_tile<MODE_DX, T, T, false>(px, block, blocks);
+  }
 }
 
 // Few output values: one workgroup per 16 x 16 block, the contraction split over its waves (forward only: both operands run along the
@@ -538,7 +558,7 @@ template <int MODE> DEVINL void f32_store(const LinP& p, int slab, int i, int j,
 template <int MODE> __global__ __launch_bounds__(256) void linear_f32_kernel(const LinP p) {
   constexpr bool ARC = MODE == MODE_DW, BRC = MODE != MODE_FWD;
   __shared__ float smem[2][2 * FK * FP];
-  const Place at = place<FT, FT>(p);
+  const Place at = place<FT, FT>(p, blockIdx.x, gridDim.x);
   const int i0 = at.i0, j0 = at.j0;
   const int wave = threadIdx.x >> 6, wi = (wave >> 1) * 32, wj = (wave & 1) * 32, lane = threadIdx.x & 63;
   const int kbeg = at.slab * p.ksteps * FK;
@@ -738,7 +758,7 @@ template <int E> DEVINL void fold(const FoldP& q, int block, int accumulate, f32
       }
   }
 }
-constexpr int FOLD_FEW = 32;      // slabs up to which 16 lanes per element do
+constexpr int FOLD_FEW = 64;      // slabs up to which 16 lanes per element do
 __global__ __launch_bounds__(256) void linear_fold_kernel(const FoldP w, const FoldP b, const int accumulate) {
   __shared__ f32x4 red[256];
   if ((int)blockIdx.x >= w.blocks) fold<4>(b, blockIdx.x - w.blocks, accumulate, red);
@@ -815,7 +835,7 @@ int check_linear(const plyolo_linear_desc* d, const char* who) {
 int tile_grid(LinP& p, int tile, int slabs, const char* who) {
   p.nj = cdiv(p.J, tile);
   const int64_t n = (int64_t)cdiv(p.I, tile) * p.nj;
-  PLY_CHECK_ARG(n * slabs < 2147483647, "%s: more than 2^31 workgroups", who);
+  PLY_CHECK_ARG(n * slabs < 1073741824, "%s: more than 2^30 workgroups", who);
   p.tiles = (int)n;
   return (int)n * slabs;
 }
@@ -828,7 +848,7 @@ template <int MODE, int TI, int TJ> size_t tile_lds(size_t stages) {
 }
 template <int MODE, int T, bool HEAVY> hipError_t launch_any(const LinP& p, int grid, hipStream_t s) {
   const size_t lds = tile_lds<MODE, T, T>(2 * (size_t)(2 * T) * BK * 2);
-  auto k = linear_bf16_any_kernel<MODE, T, T, HEAVY>;
+  auto k = linear_bf16_any_kernel<MODE, T, HEAVY>;
   if (hipError_t e = plyolo::ensure_dynamic_lds((const void*)k, lds); e != hipSuccess) return e;
   hipLaunchKernelGGL(k, dim3(grid), dim3(256), lds, s, p);
   return hipGetLastError();
@@ -849,6 +869,13 @@ template <int MODE, bool HEAVY> hipError_t launch_bf16(const LinP& p, int tile, 
     return launch_direct<MODE, 2, 2, 32, 32, 64, 3, HEAVY>(p, grid, s);
   }
   return tile == 128 ? launch_any<MODE, 128, HEAVY>(p, grid, s) : launch_any<MODE, 64, HEAVY>(p, grid, s);
+}
+template <int T, bool DIRECT> hipError_t launch_both(const LinP& px, const LinP& pw, int gx, int gw, hipStream_t s) {
+  const size_t lds = tile_lds<MODE_DX, T, T>(2 * (size_t)(2 * T) * 64 * 2);
+  auto k = linear_bf16_bwd_kernel<T, DIRECT>;
+  if (hipError_t e = plyolo::ensure_dynamic_lds((const void*)k, lds); e != hipSuccess) return e;
+  hipLaunchKernelGGL(k, dim3((unsigned)gx + (unsigned)gw), dim3(256), lds, s, px, pw, gw);
+  return hipGetLastError();
 }
 template <int MODE> hipError_t launch_gemm(int dtype, const LinP& p, int tile, int grid, bool direct, hipStream_t s) {
   if (dtype != PLYOLO_BF16) {
@@ -962,10 +989,16 @@ int plyolo_linear_bwd(const plyolo_linear_desc* d, const void* dy, const void* z
       if (dtype == PLYOLO_BF16) hipLaunchKernelGGL(linear_dz_kernel<bf16_t>, dim3(b.dzblk), dim3(256), 0, s, q);
       else hipLaunchKernelGGL(linear_dz_kernel<float>, dim3(b.dzblk), dim3(256), 0, s, q);
     }
-    if (dx)
-      if (hipError_t e = launch_gemm<MODE_DX>(dtype, px, tx, gx, dx_direct, s); e != hipSuccess) return e;
-    if (dw)
-      if (hipError_t e = launch_gemm<MODE_DW>(dtype, pw, b.tile, gw, dw_direct, s); e != hipSuccess) return e;
+    if (dx && dw && dtype == PLYOLO_BF16 && tx == b.tile && dx_direct == dw_direct) {
+      const hipError_t e = tx == 128 ? (dx_direct ? launch_both<128, true>(px, pw, gx, gw, s) : launch_both<128, false>(px, pw, gx, gw, s))
+                                     : (dx_direct ? launch_both<64, true>(px, pw, gx, gw, s) : launch_both<64, false>(px, pw, gx, gw, s));
+      if (e != hipSuccess) return e;
+    } else {
+      if (dx)
+        if (hipError_t e = launch_gemm<MODE_DX>(dtype, px, tx, gx, dx_direct, s); e != hipSuccess) return e;
+      if (dw)
+        if (hipError_t e = launch_gemm<MODE_DW>(dtype, pw, b.tile, gw, dw_direct, s); e != hipSuccess) return e;
+    }
     if (dw || db) hipLaunchKernelGGL(linear_fold_kernel, dim3((unsigned)(fw.blocks + fb.blocks)), dim3(256), 0, s, fw, fb, acc);
     return hipGetLastError();
   });
