@@ -476,16 +476,16 @@ DEVINL int xcd_contiguous(int id, int n) {      // hardware deals workgroup ids 
 }
 
 // lanes that share the reduction of one of n items: a power of two, whole waves at most
-DEVINL int res_lanes(int n) {
+DEVINL int res_lanes(int n, int nt) {
   int l = 64;
-  while (l > 1 && l * n > RES_NT) l >>= 1;
+  while (l > 1 && l * n > nt) l >>= 1;
   return l;
 }
 
-template <typename T, int V, int NV, int ACTC> __global__ __launch_bounds__(RES_NT) void gn_res_fwd_kernel(const ResP q) {
+template <typename T, int V, int NV, int ACTC, int NT> __global__ __launch_bounds__(NT) void gn_res_fwd_kernel(const ResP q) {
   const GnP& p = q.g;
-  __shared__ float2 red[V * RES_NT];           // [channel of the vector][thread]: (mean, M2) of the thread's values
-  extern __shared__ float2 chan[];             // [channels of the slice] (mean - origin, M2), behind them [groups][2] mean, rstd
+  extern __shared__ float2 red[];              // [channel of the vector][thread]: (mean, M2) of the thread's values
+  float2* chan = red + V * NT;                 // [channels of the slice] (mean - origin, M2), behind them [groups][2] mean, rstd
   float* gm = (float*)(chan + q.sv * V);
   const int id = xcd_contiguous(blockIdx.x, gridDim.x), n = id / q.slices, c0 = (id % q.slices) * q.sv * V;
   const int tid = threadIdx.x, col = tid % q.sv, row = tid / q.sv, act = ACTC >= 0 ? ACTC : p.act;
@@ -520,19 +520,19 @@ template <typename T, int V, int NV, int ACTC> __global__ __launch_bounds__(RES_
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         const float o = gn_origin<T>(p, n, (c0 + col * V + e) / p.cg), v = m2[e] - s[e] * s[e] * inv;
-        red[e * RES_NT + tid] = make_float2((k[e] - o) + s[e] * inv, v < 0.f ? 0.f : v);
+        red[e * NT + tid] = make_float2((k[e] - o) + s[e] * inv, v < 0.f ? 0.f : v);
       }
     }
   }
   __syncthreads();
-  // row lanes -> channels (a channel's partials are res_lanes(nch) lanes' work, about V each) -> groups
+  // row lanes -> channels (a channel's partials are res_lanes(nch, NT) lanes' work, about V each) -> groups
   const int nch = q.sv * V, nrow = min(q.rpb, p.HW);
   {
-    const int L = res_lanes(nch), lane = tid % L;
-    for (int k = 0; k < nch; k += RES_NT / L) {
+    const int L = res_lanes(nch, NT), lane = tid % L;
+    for (int k = 0; k < nch; k += NT / L) {
       const int c = k + tid / L;
       const bool live = c < nch;
-      const float2* e = red + (live ? (c % V) * RES_NT + c / V : 0);
+      const float2* e = red + (live ? (c % V) * NT + c / V : 0);
       float mean = 0.f, m2 = 0.f;
       if (live)
         for (int r = lane; r < nrow; r += L) mean = fmaf(e[r * q.sv].x, (float)(per + (r < extra ? 1 : 0)), mean);
@@ -550,8 +550,8 @@ template <typename T, int V, int NV, int ACTC> __global__ __launch_bounds__(RES_
   __syncthreads();
   const int gs = nch / p.cg;
   {
-    const int L = res_lanes(gs), lane = tid % L;
-    for (int k = 0; k < gs; k += RES_NT / L) {
+    const int L = res_lanes(gs, NT), lane = tid % L;
+    for (int k = 0; k < gs; k += NT / L) {
       const int g = k + tid / L;
       const bool live = g < gs;
       float mean = 0.f, m2 = 0.f;
@@ -655,7 +655,7 @@ template <typename T, int V, int NV, int ACTC> __global__ __launch_bounds__(RES_
   __syncthreads();
   const int nrow = min(q.rpb, p.HW);
   {
-    const int L = res_lanes(nch), lane = tid % L;
+    const int L = res_lanes(nch, RES_NT), lane = tid % L;
     for (int k = 0; k < nch; k += RES_NT / L) {
       const int c = k + tid / L;
       const bool live = c < nch;
@@ -684,7 +684,7 @@ template <typename T, int V, int NV, int ACTC> __global__ __launch_bounds__(RES_
   __syncthreads();
   const int gs = nch / p.cg;
   {
-    const int L = res_lanes(gs), lane = tid % L;
+    const int L = res_lanes(gs, RES_NT), lane = tid % L;
     for (int k = 0; k < gs; k += RES_NT / L) {
       const int g = k + tid / L;
       float a = 0.f, b = 0.f;
@@ -782,7 +782,7 @@ GnP gn_params(const plyolo_gn_desc* d, void* ws) {
 // beyond 12 vectors (1 x 6400 x 128, nv 13: 20 / 15).  The backward holds two operands and has nothing to hide narrow row pieces behind: 16
 // vectors in pieces of 64 bytes and more (32 x 1600 x 256, sv 4: 31 / 44; 16 x 1600 x 640, sv 5: 39 / 51), 8 in narrower ones
 // (32 x 6400 x 128, sv 1, nv 13: 91 / 72) and on few workgroups.
-struct ResPlan { int sv, slices, rpb, nv; };
+struct ResPlan { int sv, slices, rpb, nv, nt; };
 ResPlan res_plan(const plyolo_gn_desc* d, int V, bool bwd) {
   ResPlan r{};
   const int cg = d->C / d->groups;
@@ -799,19 +799,27 @@ ResPlan res_plan(const plyolo_gn_desc* d, int V, bool bwd) {
     if (sv > least && wgs < 256) break;
     r.sv = sv; r.slices = cv / sv; r.rpb = rpb; r.nv = nv;
   }
+  r.nt = RES_NT;
+  if (!bwd && r.nv > 16) {      // twice the threads with half the vectors each
+    r.nt = 2 * RES_NT;
+    r.rpb = r.nt / r.sv;
+    r.nv = (d->HW + r.rpb - 1) / r.rpb;
+  }
   return r;
 }
 
 #define GN_RES_FWD(T, V, nv, ACT)                                                                      \
-  ((nv) <= 2 ? gn_res_fwd_kernel<T, V, 2, ACT> : (nv) <= 4 ? gn_res_fwd_kernel<T, V, 4, ACT>           \
-   : (nv) <= 8 ? gn_res_fwd_kernel<T, V, 8, ACT> : (nv) <= 16 ? gn_res_fwd_kernel<T, V, 16, ACT> : gn_res_fwd_kernel<T, V, 32, ACT>)
+  (rp.nt != RES_NT ? gn_res_fwd_kernel<T, V, 16, ACT, 2 * RES_NT> : (nv) <= 2 ? gn_res_fwd_kernel<T, V, 2, ACT, RES_NT> : (nv) <= 4 ? gn_res_fwd_kernel<T, V, 4, ACT, RES_NT>           \
+   : (nv) <= 8 ? gn_res_fwd_kernel<T, V, 8, ACT, RES_NT> : gn_res_fwd_kernel<T, V, 16, ACT, RES_NT>)
 #define GN_RES_BWD(T, V, nv, ACT) \
   ((nv) <= 2 ? gn_res_bwd_kernel<T, V, 2, ACT> : (nv) <= 4 ? gn_res_bwd_kernel<T, V, 4, ACT>           \
    : (nv) <= 8 ? gn_res_bwd_kernel<T, V, 8, ACT> : gn_res_bwd_kernel<T, V, 16, ACT>)
-#define GN_RES_DISPATCH(dtype, wide, act, NAME, KERN, nv)                                                                                   \
-  ((dtype) == PLYOLO_BF16 ? ((wide) ? ((act) == PLYOLO_ACT_SILU ? NAME(bf16_t, 8, nv, PLYOLO_ACT_SILU) : NAME(bf16_t, 8, nv, -1))            \
-                                    : KERN<bf16_t, 1, 16, -1>)                                                                             \
-                          : ((wide) ? NAME(float, 4, nv, -1) : KERN<float, 1, 16, -1>))
+#define GN_RES_DISPATCH(dtype, wide, act, NAME, ELEM, nv)                                                                        \
+  ((dtype) == PLYOLO_BF16 ? ((wide) ? ((act) == PLYOLO_ACT_SILU ? NAME(bf16_t, 8, nv, PLYOLO_ACT_SILU) : NAME(bf16_t, 8, nv, -1)) \
+                                    : ELEM(bf16_t))                                                                             \
+                          : ((wide) ? NAME(float, 4, nv, -1) : ELEM(float)))
+#define GN_RES_FWD1(T) gn_res_fwd_kernel<T, 1, 16, -1, RES_NT>
+#define GN_RES_BWD1(T) gn_res_bwd_kernel<T, 1, 16, -1>
 
 #define GN_DISPATCH(dtype, wide, act, KERN)                                                                                     \
   ((dtype) == PLYOLO_BF16 ? ((wide) ? ((act) == PLYOLO_ACT_SILU ? KERN<bf16_t, 8, PLYOLO_ACT_SILU> : KERN<bf16_t, 8, -1>)         \
@@ -850,10 +858,11 @@ int plyolo_gn_act_fwd(const plyolo_gn_desc* d, const void* x, const float* gamma
     ResP q{};
     q.g = p; q.sv = rp.sv; q.slices = rp.slices; q.rpb = rp.rpb;
     const int nch = rp.sv * (wide ? V : 1);
-    const size_t lds = (size_t)(nch + nch / p.cg) * sizeof(float2);
+    const size_t lds = (size_t)(rp.nt * (wide ? V : 1) + nch + nch / p.cg) * sizeof(float2);
     return plyolo::submit(stream, [=](hipStream_t s) -> hipError_t {
-      auto k = GN_RES_DISPATCH(dtype, wide, act, GN_RES_FWD, gn_res_fwd_kernel, rp.nv);
-      hipLaunchKernelGGL(k, dim3((unsigned)p.N * rp.slices), dim3(RES_NT), lds, s, q);
+      auto k = GN_RES_DISPATCH(dtype, wide, act, GN_RES_FWD, GN_RES_FWD1, rp.nv);
+      if (hipError_t e = plyolo::ensure_dynamic_lds((const void*)k, lds); e != hipSuccess) return e;
+      hipLaunchKernelGGL(k, dim3((unsigned)p.N * rp.slices), dim3(rp.nt), lds, s, q);
       return hipGetLastError();
     });
   }
@@ -894,7 +903,7 @@ int plyolo_gn_act_bwd(const plyolo_gn_desc* d, const void* dout, int d_ld, const
     const int nch = rp.sv * (wide ? V : 1);
     const size_t lds = (size_t)(nch + nch / p.cg) * sizeof(float2);
     return plyolo::submit(stream, [=](hipStream_t s) -> hipError_t {
-      auto k = GN_RES_DISPATCH(dtype, wide, act, GN_RES_BWD, gn_res_bwd_kernel, rp.nv);
+      auto k = GN_RES_DISPATCH(dtype, wide, act, GN_RES_BWD, GN_RES_BWD1, rp.nv);
       hipLaunchKernelGGL(k, dim3((unsigned)p.N * rp.slices), dim3(RES_NT), lds, s, q);
       if (p.N > 1 && (p.dgamma || p.dbeta)) join_bwd(p, cdiv(p.C, JOIN_I), 0, p.N, s);
       return hipGetLastError();
