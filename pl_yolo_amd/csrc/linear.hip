@@ -512,104 +512,153 @@ template <bool HEAVY> __global__ __launch_bounds__(1024) void linear_bf16_narrow
 }
 
 // ------------------------------------------------------------------------------------------------ fp32 (parity mode)
-// 64 x 64 tile, four waves of 32 x 32 (2 x 2 fragments of v_mfma_f32_16x16x4_f32), 16 contraction elements per stage; both LDS images are
-// [k][row] with a pitch of 80 floats: the four k rows of one fragment read start 16 banks apart.
-constexpr int FT = 64, FK = 16, FP = 80;
+typedef f32x4 __attribute__((aligned(4))) f32x4_any;     // 16 bytes at any element address
 
-template <bool RC> DEVINL void f32_request(float (&v)[4], const float* base, int ld, int row0, int rows, int k0, int kend) {
-#pragma unroll
-  for (int u = 0; u < 4; ++u) {
-    const int idx = threadIdx.x + u * 256;
-    const int k = k0 + (RC ? idx / FT : idx % FK), r = row0 + (RC ? idx % FT : idx / FK);
-    v[u] = (k < kend && r < rows) ? base[RC ? (size_t)k * ld + r : (size_t)r * ld + k] : 0.f;
-  }
-}
-template <bool RC> DEVINL void f32_commit(const float (&v)[4], float* img) {
-#pragma unroll
-  for (int u = 0; u < 4; ++u) {
-    const int idx = threadIdx.x + u * 256;
-    img[(RC ? idx / FT : idx % FK) * FP + (RC ? idx % FT : idx / FK)] = v[u];
-  }
-}
-
-template <int MODE> DEVINL void f32_store(const LinP& p, int slab, int i, int j, const f32x4 acc) {
-  if (i >= p.I) return;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    if (j + e >= p.J) continue;
-    float v = acc[e];
-    if (MODE == MODE_DW) {
-      ((float*)p.out)[((size_t)slab * p.I + i) * p.J + j + e] = v;
-      continue;
-    }
-    float* o = (float*)p.out + (size_t)i * p.o_ld + j + e;
-    if (MODE == MODE_FWD) {
-      if (p.bias) v += p.bias[j + e];
-      if (p.z) ((float*)p.z)[(size_t)i * p.z_ld + j + e] = v;
-      v = act_fwd_precise(v, p.act);
-      if (p.res) v += ((const float*)p.res)[(size_t)i * p.r_ld + j + e];
-    } else if (p.accumulate) {
-      v += *o;
-    }
-    *o = v;
-  }
-}
-
-template <int MODE> __global__ __launch_bounds__(256) void linear_f32_kernel(const LinP p) {
-  constexpr bool ARC = MODE == MODE_DW, BRC = MODE != MODE_FWD;
-  __shared__ float smem[2][2 * FK * FP];
-  const Place at = place<FT, FT>(p, blockIdx.x, gridDim.x);
-  const int i0 = at.i0, j0 = at.j0;
-  const int wave = threadIdx.x >> 6, wi = (wave >> 1) * 32, wj = (wave & 1) * 32, lane = threadIdx.x & 63;
-  const int kbeg = at.slab * p.ksteps * FK;
-  const int kend = MODE == MODE_DW ? min(p.Kc, kbeg + p.ksteps * FK) : p.Kc;
-  f32x4 acc[2][2];
-#pragma unroll
-  for (int a = 0; a < 2; ++a)
-#pragma unroll
-    for (int b = 0; b < 2; ++b) acc[a][b] = f32x4{0.f, 0.f, 0.f, 0.f};
-  float va[4], vb[4];
-  f32_request<ARC>(va, (const float*)p.a, p.a_ld, i0, p.I, kbeg, kend);
-  f32_request<BRC>(vb, (const float*)p.b, p.b_ld, j0, p.J, kbeg, kend);
-  int buf = 0;
-  for (int k0 = kbeg; k0 < kend; k0 += FK, buf ^= 1) {
-    float *ia = smem[buf], *ib = smem[buf] + FK * FP;
-    f32_commit<ARC>(va, ia);
-    f32_commit<BRC>(vb, ib);
-    __syncthreads();
-    if (k0 + FK < kend) {
-      f32_request<ARC>(va, (const float*)p.a, p.a_ld, i0, p.I, k0 + FK, kend);
-      f32_request<BRC>(vb, (const float*)p.b, p.b_ld, j0, p.J, k0 + FK, kend);
-    }
-#pragma unroll
-    for (int kk = 0; kk < FK / 4; ++kk) {
-      const int ro = (kk * 4 + (lane >> 4)) * FP + (lane & 15);
-      float fa[2], fb[2];
-#pragma unroll
-      for (int a = 0; a < 2; ++a) fa[a] = ia[ro + wi + a * 16];
-#pragma unroll
-      for (int b = 0; b < 2; ++b) fb[b] = ib[ro + wj + b * 16];
-#pragma unroll
-      for (int a = 0; a < 2; ++a)
-#pragma unroll
-        for (int b = 0; b < 2; ++b) acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x4f32(fb[b], fa[a], acc[a][b], 0, 0, 0);
-    }
-  }
-#pragma unroll
-  for (int a = 0; a < 2; ++a)
-#pragma unroll
-    for (int b = 0; b < 2; ++b) f32_store<MODE>(p, at.slab, i0 + wi + a * 16 + (lane & 15), j0 + wj + b * 16 + 4 * (lane >> 4), acc[a][b]);
-}
-
-// Few output values, fp32: as linear_bf16_narrow_kernel; a lane takes four consecutive k and feeds them to four MFMAs in turn (both operands
-// in the same order, which is all a sum needs).
+// four consecutive elements of which n >= 1 exist (the others are zero)
 DEVINL f32x4 load4(const float* p, int n) {
-  typedef f32x4 __attribute__((aligned(4))) f32x4_any;
   if (n >= 4) return *(const f32x4_any*)p;
   const float a = p[0], b = p[min(1, n - 1)], c = p[min(2, n - 1)];
   return f32x4{a, n > 1 ? b : 0.f, n > 2 ? c : 0.f, 0.f};
 }
 
+// One operand tile, as Tile: T rows x 32 contraction elements, 256 threads, 16-byte granules through registers.
+// KC image [T][32 + 4]: a lane's fragment is the four consecutive k of one 16-byte read, rows 36 floats apart on banks of their own.
+// RC image [32][T + 4]: four 4-byte reads, k rows 4 apart 16 banks apart.
+// Either way MFMA e of a group of four takes element e of both operands: the sum runs over all k, in whatever order.
+constexpr int FK = 32;
+template <bool RC, int T> struct F32Tile {
+  static constexpr int NG = T * FK / 4 / 256, PITCH = RC ? T + 4 : FK + 4, FLOATS = (RC ? FK : T) * PITCH, TG = T / 4, KG = FK / 4;
+  const float* src[NG];
+  int kof[NG], len[NG], cut[NG];
+  f32x4 v[NG];
+  bool few;
+
+  DEVINL void init(const float* base, int ld, int row0, int rows, int kbeg, int clen) {
+    few = (RC ? rows : clen) < 4;
+#pragma unroll
+    for (int u = 0; u < NG; ++u) {
+      const int idx = threadIdx.x + u * 256;
+      const int r = row0 + (RC ? idx % TG * 4 : idx / KG);
+      kof[u] = RC ? idx / TG : idx % KG * 4;
+      len[u] = rows - r;
+      src[u] = r >= rows ? nullptr : RC ? base + (size_t)(kbeg + kof[u]) * ld + r : base + (size_t)r * ld + kbeg + kof[u];
+    }
+  }
+  DEVINL void request(size_t k, int ld, int left) {
+#pragma unroll
+    for (int u = 0; u < NG; ++u) {
+      const bool ok = src[u] != nullptr && kof[u] < left;
+      const float* q = src[u] + (RC ? k * ld : k);
+      const int n = RC ? len[u] : left - kof[u];
+      cut[u] = ok && n < 4 && !few ? 4 - n : 0;
+      if (few) v[u] = ok ? load4(q, n) : f32x4{0.f, 0.f, 0.f, 0.f};
+      else v[u] = *(ok ? (const f32x4_any*)(q - cut[u]) : (const f32x4_any*)&zero_granule);
+    }
+  }
+  DEVINL void commit(float* img) {
+#pragma unroll
+    for (int u = 0; u < NG; ++u) {
+      const int idx = threadIdx.x + u * 256;
+      f32x4 t = v[u];
+      if (cut[u] == 1) t = f32x4{t[1], t[2], t[3], 0.f};
+      if (cut[u] == 2) t = f32x4{t[2], t[3], 0.f, 0.f};
+      if (cut[u] == 3) t = f32x4{t[3], 0.f, 0.f, 0.f};
+      *(f32x4*)(img + (RC ? idx / TG * PITCH + idx % TG * 4 : idx / KG * PITCH + idx % KG * 4)) = t;
+    }
+  }
+  // 16 rows from r0, contraction elements 16 kk .. 16 kk + 15
+  static DEVINL f32x4 frag(const float* img, int r0, int kk) {
+    const int lane = threadIdx.x & 63, k = kk * 16 + 4 * (lane >> 4), r = r0 + (lane & 15);
+    if (!RC) return *(const f32x4*)(img + r * PITCH + k);
+    f32x4 f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) f[e] = img[(k + e) * PITCH + r];
+    return f;
+  }
+};
+
+template <int MODE> DEVINL void f32_store(const LinP& p, int slab, int i, int j, f32x4 v) {
+  const int n = p.J - j;
+  if (i >= p.I || n <= 0) return;
+  float* o = MODE == MODE_DW ? (float*)p.out + ((size_t)slab * p.I + i) * p.J + j : (float*)p.out + (size_t)i * p.o_ld + j;
+  const float* r = MODE == MODE_FWD ? (p.res ? (const float*)p.res + (size_t)i * p.r_ld + j : nullptr) : MODE == MODE_DX && p.accumulate ? o : nullptr;
+  f32x4 add = {0.f, 0.f, 0.f, 0.f};
+  if (r) add = load4(r, n);
+  if (MODE == MODE_FWD) {
+    if (p.bias) v += load4(p.bias + j, n);
+    if (p.z) {
+      float* z = (float*)p.z + (size_t)i * p.z_ld + j;
+      if (n >= 4) *(f32x4_any*)z = v;
+      else
+#pragma unroll
+        for (int e = 0; e < 3; ++e)
+          if (e < n) z[e] = v[e];
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = act_fwd_precise(v[e], p.act);
+  }
+  if (r) v += add;
+  if (n >= 4) *(f32x4_any*)o = v;
+  else
+#pragma unroll
+    for (int e = 0; e < 3; ++e)
+      if (e < n) o[e] = v[e];
+}
+
+// T x T tile, four waves of T / 2 x T / 2, v_mfma_f32_16x16x4_f32, two LDS images per operand, one barrier per stage
+template <int MODE, int T> __global__ __launch_bounds__(256) void linear_f32_kernel(const LinP p) {
+  typedef F32Tile<MODE == MODE_DW, T> TA;
+  typedef F32Tile<MODE != MODE_FWD, T> TB;
+  constexpr int F = T / 32, STAGE = TA::FLOATS + TB::FLOATS;
+  extern __shared__ __align__(16) float fsmem[];
+  const Place at = place<T, T>(p, blockIdx.x, gridDim.x);
+  const int i0 = at.i0, j0 = at.j0;
+  const int wave = threadIdx.x >> 6, wi = (wave >> 1) * (T / 2), wj = (wave & 1) * (T / 2), lane = threadIdx.x & 63;
+  const int kbeg = at.slab * p.ksteps * FK;
+  const int klen = (MODE == MODE_DW ? min(p.Kc, kbeg + p.ksteps * FK) : p.Kc) - kbeg;
+  f32x4 acc[F][F];
+#pragma unroll
+  for (int a = 0; a < F; ++a)
+#pragma unroll
+    for (int b = 0; b < F; ++b) acc[a][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+  TA ta;
+  TB tb;
+  ta.init((const float*)p.a, p.a_ld, i0, p.I, kbeg, p.Kc);
+  tb.init((const float*)p.b, p.b_ld, j0, p.J, kbeg, p.Kc);
+  ta.request(0, p.a_ld, klen);
+  tb.request(0, p.b_ld, klen);
+  int buf = 0;
+  for (int k0 = 0; k0 < klen; k0 += FK, buf ^= 1) {
+    float *ia = fsmem + buf * STAGE, *ib = ia + TA::FLOATS;
+    ta.commit(ia);
+    tb.commit(ib);
+    __syncthreads();      // image `buf` is whole; image buf ^ 1 was last read before every wave came here
+    if (k0 + FK < klen) {
+      ta.request(k0 + FK, p.a_ld, klen - k0 - FK);
+      tb.request(k0 + FK, p.b_ld, klen - k0 - FK);
+    }
+#pragma unroll
+    for (int kk = 0; kk < FK / 16; ++kk) {
+      f32x4 fa[F], fb[F];
+#pragma unroll
+      for (int a = 0; a < F; ++a) fa[a] = TA::frag(ia, wi + a * 16, kk);
+#pragma unroll
+      for (int b = 0; b < F; ++b) fb[b] = TB::frag(ib, wj + b * 16, kk);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int a = 0; a < F; ++a)
+#pragma unroll
+          for (int b = 0; b < F; ++b) acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x4f32(fb[b][e], fa[a][e], acc[a][b], 0, 0, 0);
+    }
+  }
+#pragma unroll
+  for (int a = 0; a < F; ++a)
+#pragma unroll
+    for (int b = 0; b < F; ++b) f32_store<MODE>(p, at.slab, i0 + wi + a * 16 + (lane & 15), j0 + wj + b * 16 + 4 * (lane >> 4), acc[a][b]);
+}
+
+// Few output values, fp32: as linear_bf16_narrow_kernel; a lane takes four consecutive k and feeds them to four MFMAs in turn
 __global__ __launch_bounds__(1024) void linear_f32_narrow_kernel(const LinP p, const int kper) {
   __shared__ f32x4 part[16][64];
   const int waves = blockDim.x >> 6, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
@@ -776,7 +825,7 @@ size_t up16(size_t v) { return (v + 15) & ~(size_t)15; }
 
 // Tile edge of an I x J output (bf16): the larger the tile, the fewer LDS reads per MFMA and the fewer re-reads of the operands; the smaller,
 // the more of the chip a small output fills.
-int pick_tile(int64_t I, int64_t J, int64_t Kc, bool direct) {
+int pick_tile(int64_t I, int64_t J, int64_t Kc, bool direct) {      // (fp32: direct = false)
   auto tiles = [&](int a) { return ((I + a - 1) / a) * ((J + a - 1) / a); };
   if (direct && tiles(256) >= 128 && J > 128 && Kc >= 512) return 256;
   if (tiles(128) >= 192 && J > 64) return 128;
@@ -810,12 +859,8 @@ BwdPlan bwd_plan(const plyolo_linear_desc* d) {
   b.part_off = b.dz_bytes;
   b.part_bytes = up16((size_t)b.dzblk * d->N * 4);
   b.slab_off = b.part_off + b.part_bytes;
-  if (half) {
-    dw_plan(d, 128, &b);
-    if ((int64_t)b.S * cdiv(d->N, 128) * cdiv(d->K, 128) < 128) dw_plan(d, 64, &b);
-  } else {
-    dw_plan(d, FT, &b);
-  }
+  dw_plan(d, 128, &b);
+  if ((int64_t)b.S * cdiv(d->N, 128) * cdiv(d->K, 128) < 128) dw_plan(d, 64, &b);
   b.slab_bytes = up16((size_t)b.S * d->N * d->K * 4);
   b.total = b.slab_off + b.slab_bytes;
   return b;
@@ -825,7 +870,7 @@ int check_linear(const plyolo_linear_desc* d, const char* who) {
   PLY_CHECK_ARG(d != nullptr, "%s: null descriptor", who);
   PLY_CHECK_ARG(d->dtype == PLYOLO_BF16 || d->dtype == PLYOLO_F32, "%s: bad dtype %d", who, d->dtype);
   PLY_CHECK_ARG(d->M > 0 && d->N > 0 && d->K > 0, "%s: non-positive dimension (M %d, N %d, K %d)", who, d->M, d->N, d->K);
-  PLY_CHECK_ARG(d->N <= (1 << 20) && d->K <= (1 << 20) && d->M <= 2147483647 - 1024, "%s: dimension too large (M %d, N %d, K %d)", who, d->M, d->N, d->K);
+  PLY_CHECK_ARG(d->N <= (1 << 20) && d->K <= (1 << 20) && (double)d->N * d->K < 17179869184.0 && d->M <= 2147483647 - 1024, "%s: dimension too large (M %d, N %d, K %d)", who, d->M, d->N, d->K);
   PLY_CHECK_ARG(d->act >= PLYOLO_ACT_NONE && d->act <= PLYOLO_ACT_GELU, "%s: bad activation %d", who, d->act);
   PLY_CHECK_ARG(d->x_ld >= d->K && d->w_ld >= d->K, "%s: x_ld %d or w_ld %d < K %d", who, d->x_ld, d->w_ld, d->K);
   return 0;
@@ -861,6 +906,13 @@ template <int MODE, int NWI, int NWJ, int WI, int WJ, int K, int ST, bool HEAVY>
   hipLaunchKernelGGL(k, dim3(grid), dim3(64 * NWI * NWJ), lds, s, p);
   return hipGetLastError();
 }
+template <int MODE, int T> hipError_t launch_f32(const LinP& p, int grid, hipStream_t s) {
+  constexpr size_t lds = 2 * (size_t)(F32Tile<MODE == MODE_DW, T>::FLOATS + F32Tile<MODE != MODE_FWD, T>::FLOATS) * sizeof(float);
+  auto k = linear_f32_kernel<MODE, T>;
+  if (hipError_t e = plyolo::ensure_dynamic_lds((const void*)k, lds); e != hipSuccess) return e;
+  hipLaunchKernelGGL(k, dim3(grid), dim3(256), lds, s, p);
+  return hipGetLastError();
+}
 // direct: both operands' granules are whole and 16-byte aligned
 template <int MODE, bool HEAVY> hipError_t launch_bf16(const LinP& p, int tile, int grid, bool direct, hipStream_t s) {
   if (direct) {
@@ -878,10 +930,7 @@ template <int T, bool DIRECT> hipError_t launch_both(const LinP& px, const LinP&
   return hipGetLastError();
 }
 template <int MODE> hipError_t launch_gemm(int dtype, const LinP& p, int tile, int grid, bool direct, hipStream_t s) {
-  if (dtype != PLYOLO_BF16) {
-    hipLaunchKernelGGL(linear_f32_kernel<MODE>, dim3(grid), dim3(256), 0, s, p);
-    return hipGetLastError();
-  }
+  if (dtype != PLYOLO_BF16) return tile == 128 ? launch_f32<MODE, 128>(p, grid, s) : launch_f32<MODE, 64>(p, grid, s);
   if (MODE == MODE_FWD && p.act > PLYOLO_ACT_LRELU) return launch_bf16<MODE, MODE == MODE_FWD>(p, tile, grid, direct, s);
   return launch_bf16<MODE, false>(p, tile, grid, direct, s);
 }
@@ -911,9 +960,13 @@ int plyolo_linear_fwd(const plyolo_linear_desc* d, const void* x, const void* w,
   const int dtype = d->dtype;
   const double m = d->M, n = d->N, k = d->K;
   plyolo::annotate("linear_fwd", 2.0 * m * n * k, (m * k + n * k + m * n * (1.0 + (z ? 1 : 0) + (res ? 1 : 0))) * es);
-  // 16 x 16 blocks re-read x once per 16 columns and w once per 16 rows; while that is little, they fill the chip where tiles would not
+  // 16 x 16 blocks re-read x once per 16 columns and w once per 16 rows, out of L2 at about 9.6 bytes a nanosecond and block column; a tile walks
+  // its whole contraction by itself.  Microseconds, fitted over M 16 .. 51200, N 16 .. 2048, K 32 .. 2048, M x K x N here (bf16: 64 x 2048 x
+  // 1024 6.8 in blocks, 13.6 in tiles; 256 x 1024 x 1024 10.1 / 8.8; 12800 x 64 x 64 6.2 / 4.5.  fp32: 64 x 2048 x 1024 11.4 / 75; 400 x 512 x
+  // 512 10.6 / 23.6; 3200 x 512 x 512 49 / 37)
   const double again = (m * k * cdiv(d->N, 16) + n * k * cdiv(d->M, 16)) * es;
-  if (again < 32e6) {
+  const double blocks_us = 3.4 + again / 9.6e6, tiles_us = 4.0 + k * (dtype == PLYOLO_BF16 ? 0.31 / 64 : 1.0 / 29);
+  if (blocks_us < tiles_us) {
     const int grid = tile_grid(p, 16, 1, "linear_fwd");
     if (grid < 0) return -1;
     const int step = dtype == PLYOLO_BF16 ? 32 : 16;
@@ -928,7 +981,7 @@ int plyolo_linear_fwd(const plyolo_linear_desc* d, const void* x, const void* w,
     });
   }
   const bool direct = rows16(x, d->x_ld, d->K) && rows16(w, d->w_ld, d->K);
-  const int tile = dtype == PLYOLO_BF16 ? pick_tile(d->M, d->N, d->K, direct) : FT;
+  const int tile = pick_tile(d->M, d->N, d->K, direct && dtype == PLYOLO_BF16);
   const int grid = tile_grid(p, tile, 1, "linear_fwd");
   if (grid < 0) return -1;
   return plyolo::submit(stream, [=](hipStream_t s) -> hipError_t { return launch_gemm<MODE_FWD>(dtype, p, tile, grid, direct, s); });
@@ -969,7 +1022,7 @@ int plyolo_linear_bwd(const plyolo_linear_desc* d, const void* dy, const void* z
   // dz rows are padded to whole vectors of zeros, dy rows end at N
   const int g_len = has_act ? b.dz_ld : d->N;
   const bool dx_direct = rows16(g, g_ld, g_len) && rows16(w, d->w_ld, d->K), dw_direct = rows16(g, g_ld, g_len) && rows16(x, d->x_ld, d->K);
-  const int tx = dtype == PLYOLO_BF16 ? pick_tile(d->M, d->K, d->N, dx_direct) : FT;
+  const int tx = pick_tile(d->M, d->K, d->N, dx_direct && dtype == PLYOLO_BF16);
   const int gx = tile_grid(px, tx, 1, "linear_bwd"), gw = tile_grid(pw, b.tile, b.S, "linear_bwd");
   if (gx < 0 || gw < 0) return -1;
   FoldP fw{}, fb{};
