@@ -478,39 +478,6 @@ template <int T, bool DIRECT> __global__ __launch_bounds__(256) void linear_bf16
   }
 }
 
-// Few output values: one workgroup per 16 x 16 block, the contraction split over its waves (forward only: both operands run along the
-// contraction, so fragments come straight from memory; every load of a wave's range is in flight at once), partial blocks added in wave order.
-template <bool HEAVY> __global__ __launch_bounds__(1024) void linear_bf16_narrow_kernel(const LinP p, const int kper) {
-  __shared__ f32x4 part[16][64];
-  const int waves = blockDim.x >> 6, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int i0 = (int)(blockIdx.x / p.nj) * 16, j0 = (int)(blockIdx.x % p.nj) * 16;
-  const int i = i0 + (lane & 15), jr = j0 + (lane & 15), ko = 8 * (lane >> 4);
-  const bf16_t* pa = (const bf16_t*)p.a + (size_t)i * p.a_ld;
-  const bf16_t* pb = (const bf16_t*)p.b + (size_t)jr * p.b_ld;
-  const int k0 = wave * kper, k1 = min(p.Kc, k0 + kper);
-  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  for (int k = k0; k < k1; k += 128) {
-    u32x4 fa[4], fb[4];
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int kk = k + u * 32 + ko, n = k1 - kk;
-      fa[u] = i < p.I && n > 0 ? load8(pa + kk, n) : u32x4{0u, 0u, 0u, 0u};
-      fb[u] = jr < p.J && n > 0 ? load8(pb + kk, n) : u32x4{0u, 0u, 0u, 0u};
-    }
-#pragma unroll
-    for (int u = 0; u < 4; ++u) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*(const bf16x8*)&fb[u], *(const bf16x8*)&fa[u], acc, 0, 0, 0);
-  }
-  if (waves > 1) {
-    part[wave][lane] = acc;
-    __syncthreads();
-    if (wave) return;
-    acc = part[0][lane];
-    for (int w = 1; w < waves; ++w) acc += part[w][lane];
-  }
-  const int j = j0 + 4 * (lane >> 4);
-  store4<MODE_FWD, HEAVY>(p, i0 + (lane & 15), j, acc, bias4<MODE_FWD>(p, j));
-}
-
 // ------------------------------------------------------------------------------------------------ fp32 (parity mode)
 typedef f32x4 __attribute__((aligned(4))) f32x4_any;     // 16 bytes at any element address
 
@@ -524,9 +491,10 @@ DEVINL f32x4 load4(const float* p, int n) {
 // One operand tile, as Tile: T rows x 32 contraction elements, 256 threads, 16-byte granules through registers.
 // KC image [T][32 + 4]: a lane's fragment is the four consecutive k of one 16-byte read, rows 36 floats apart on banks of their own.
 // RC image [32][T + 4]: four 4-byte reads, k rows 4 apart 16 banks apart.
+// WHOLE: no granule is cut by the end of its row (ragged ones are fetched as the row's last four elements and shifted).
 // Either way MFMA e of a group of four takes element e of both operands: the sum runs over all k, in whatever order.
 constexpr int FK = 32;
-template <bool RC, int T> struct F32Tile {
+template <bool RC, int T, bool WHOLE> struct F32Tile {
   static constexpr int NG = T * FK / 4 / 256, PITCH = RC ? T + 4 : FK + 4, FLOATS = (RC ? FK : T) * PITCH, TG = T / 4, KG = FK / 4;
   const float* src[NG];
   int kof[NG], len[NG], cut[NG];
@@ -549,6 +517,10 @@ template <bool RC, int T> struct F32Tile {
     for (int u = 0; u < NG; ++u) {
       const bool ok = src[u] != nullptr && kof[u] < left;
       const float* q = src[u] + (RC ? k * ld : k);
+      if (WHOLE) {
+        v[u] = *(ok ? (const f32x4_any*)q : (const f32x4_any*)&zero_granule);
+        continue;
+      }
       const int n = RC ? len[u] : left - kof[u];
       cut[u] = ok && n < 4 && !few ? 4 - n : 0;
       if (few) v[u] = ok ? load4(q, n) : f32x4{0.f, 0.f, 0.f, 0.f};
@@ -560,6 +532,7 @@ template <bool RC, int T> struct F32Tile {
     for (int u = 0; u < NG; ++u) {
       const int idx = threadIdx.x + u * 256;
       f32x4 t = v[u];
+      if (WHOLE) cut[u] = 0;
       if (cut[u] == 1) t = f32x4{t[1], t[2], t[3], 0.f};
       if (cut[u] == 2) t = f32x4{t[2], t[3], 0.f, 0.f};
       if (cut[u] == 3) t = f32x4{t[3], 0.f, 0.f, 0.f};
@@ -606,10 +579,10 @@ template <int MODE> DEVINL void f32_store(const LinP& p, int slab, int i, int j,
 }
 
 // T x T tile, four waves of T / 2 x T / 2, v_mfma_f32_16x16x4_f32, two LDS images per operand, one barrier per stage
-template <int MODE, int T> __global__ __launch_bounds__(256) void linear_f32_kernel(const LinP p) {
-  typedef F32Tile<MODE == MODE_DW, T> TA;
-  typedef F32Tile<MODE != MODE_FWD, T> TB;
-  constexpr int F = T / 32, STAGE = TA::FLOATS + TB::FLOATS;
+template <int MODE, int T, bool WHOLE> __global__ __launch_bounds__(256) void linear_f32_kernel(const LinP p) {
+  typedef F32Tile<MODE == MODE_DW, T, WHOLE> TA;
+  typedef F32Tile<MODE != MODE_FWD, T, WHOLE> TB;
+  constexpr int F = T / 32, STAGE = TA::FLOATS + TB::FLOATS, AHEAD = WHOLE ? 2 : 1;
   extern __shared__ __align__(16) float fsmem[];
   const Place at = place<T, T>(p, blockIdx.x, gridDim.x);
   const int i0 = at.i0, j0 = at.j0;
@@ -621,35 +594,40 @@ template <int MODE, int T> __global__ __launch_bounds__(256) void linear_f32_ker
   for (int a = 0; a < F; ++a)
 #pragma unroll
     for (int b = 0; b < F; ++b) acc[a][b] = f32x4{0.f, 0.f, 0.f, 0.f};
-  TA ta;
-  TB tb;
-  ta.init((const float*)p.a, p.a_ld, i0, p.I, kbeg, p.Kc);
-  tb.init((const float*)p.b, p.b_ld, j0, p.J, kbeg, p.Kc);
-  ta.request(0, p.a_ld, klen);
-  tb.request(0, p.b_ld, klen);
-  int buf = 0;
-  for (int k0 = 0; k0 < klen; k0 += FK, buf ^= 1) {
-    float *ia = fsmem + buf * STAGE, *ib = ia + TA::FLOATS;
-    ta.commit(ia);
-    tb.commit(ib);
-    __syncthreads();      // image `buf` is whole; image buf ^ 1 was last read before every wave came here
-    if (k0 + FK < klen) {
-      ta.request(k0 + FK, p.a_ld, klen - k0 - FK);
-      tb.request(k0 + FK, p.b_ld, klen - k0 - FK);
-    }
+  TA ta[AHEAD];
+  TB tb[AHEAD];
 #pragma unroll
-    for (int kk = 0; kk < FK / 16; ++kk) {
-      f32x4 fa[F], fb[F];
+  for (int h = 0; h < AHEAD; ++h) {
+    ta[h].init((const float*)p.a, p.a_ld, i0, p.I, kbeg, p.Kc);
+    tb[h].init((const float*)p.b, p.b_ld, j0, p.J, kbeg, p.Kc);
+    ta[h].request(h * FK, p.a_ld, klen - h * FK);
+    tb[h].request(h * FK, p.b_ld, klen - h * FK);
+  }
+  for (int k = 0; k < klen; k += 2 * FK) {
 #pragma unroll
-      for (int a = 0; a < F; ++a) fa[a] = TA::frag(ia, wi + a * 16, kk);
+    for (int h = 0; h < 2; ++h) {
+      const int k0 = k + h * FK, next = k0 + AHEAD * FK;
+      if (k0 >= klen) break;
+      float *ia = fsmem + h * STAGE, *ib = ia + TA::FLOATS;
+      ta[h % AHEAD].commit(ia);
+      tb[h % AHEAD].commit(ib);
+      __syncthreads();      // image h is whole; image h ^ 1 was last read before every wave came here
+      ta[h % AHEAD].request(next, p.a_ld, klen - next);      // (past the end: zeros; a branch here would make every wait one for all loads)
+      tb[h % AHEAD].request(next, p.b_ld, klen - next);
 #pragma unroll
-      for (int b = 0; b < F; ++b) fb[b] = TB::frag(ib, wj + b * 16, kk);
+      for (int kk = 0; kk < FK / 16; ++kk) {
+        f32x4 fa[F], fb[F];
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
+        for (int a = 0; a < F; ++a) fa[a] = TA::frag(ia, wi + a * 16, kk);
 #pragma unroll
-        for (int a = 0; a < F; ++a)
+        for (int b = 0; b < F; ++b) fb[b] = TB::frag(ib, wj + b * 16, kk);
 #pragma unroll
-          for (int b = 0; b < F; ++b) acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x4f32(fb[b][e], fa[a][e], acc[a][b], 0, 0, 0);
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+          for (int a = 0; a < F; ++a)
+#pragma unroll
+            for (int b = 0; b < F; ++b) acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x4f32(fb[b][e], fa[a][e], acc[a][b], 0, 0, 0);
+      }
     }
   }
 #pragma unroll
@@ -658,37 +636,83 @@ template <int MODE, int T> __global__ __launch_bounds__(256) void linear_f32_ker
     for (int b = 0; b < F; ++b) f32_store<MODE>(p, at.slab, i0 + wi + a * 16 + (lane & 15), j0 + wj + b * 16 + 4 * (lane >> 4), acc[a][b]);
 }
 
-// Few output values, fp32: as linear_bf16_narrow_kernel; a lane takes four consecutive k and feeds them to four MFMAs in turn
-__global__ __launch_bounds__(1024) void linear_f32_narrow_kernel(const LinP p, const int kper) {
-  __shared__ f32x4 part[16][64];
-  const int waves = blockDim.x >> 6, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int i0 = (int)(blockIdx.x / p.nj) * 16, j0 = (int)(blockIdx.x % p.nj) * 16;
-  const int i = i0 + (lane & 15), jr = j0 + (lane & 15), ko = 4 * (lane >> 4);
-  const float* pa = (const float*)p.a + (size_t)i * p.a_ld;
-  const float* pb = (const float*)p.b + (size_t)jr * p.b_ld;
-  const int k0 = wave * kper, k1 = min(p.Kc, k0 + kper);
-  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  for (int k = k0; k < k1; k += 64) {
-    f32x4 fa[4], fb[4];
+// Few output values (forward only: both operands run along the contraction, so fragments come straight from memory): one workgroup per block of
+// 16 R x 16 R values, the contraction split over its waves with every load of a step in flight at once, partial blocks added in wave order.
+// Rows beyond the last are clamped to it; what they give is not stored.  fp32: a lane's four consecutive k feed four MFMAs in turn.
+DEVINL u32x4 load_granule(const bf16_t* p, int n) { return load8(p, n); }
+DEVINL u32x4 load_granule(const float* p, int n) {
+  const f32x4 v = load4(p, n);
+  return *(const u32x4*)&v;
+}
+DEVINL f32x4 granule_mma(const bf16_t*, const u32x4& a, const u32x4& b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(*(const bf16x8*)&b, *(const bf16x8*)&a, c, 0, 0, 0);
+}
+DEVINL f32x4 granule_mma(const float*, const u32x4& a, const u32x4& b, f32x4 c) {
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int kk = k + u * 16 + ko, n = k1 - kk;
-      fa[u] = i < p.I && n > 0 ? load4(pa + kk, n) : f32x4{0.f, 0.f, 0.f, 0.f};
-      fb[u] = jr < p.J && n > 0 ? load4(pb + kk, n) : f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(b[e]), __uint_as_float(a[e]), c, 0, 0, 0);
+  return c;
+}
+template <typename T, int R, bool HEAVY> __global__ __launch_bounds__(1024) void linear_blocks_kernel(const LinP p, const int kper) {
+  constexpr int E = 16 / (int)sizeof(T), STEP = 4 * E, U = sizeof(T) == 4 && R == 2 ? 2 : 4;      // (four would spill)
+  extern __shared__ f32x4 part[];       // [waves][R * R][64]
+  const int waves = blockDim.x >> 6, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int i0 = (int)(blockIdx.x / p.nj) * (16 * R), j0 = (int)(blockIdx.x % p.nj) * (16 * R), ko = E * (lane >> 4);
+  const T *pa[R], *pb[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    pa[r] = (const T*)p.a + (size_t)min(i0 + r * 16 + (lane & 15), p.I - 1) * p.a_ld + ko;
+    pb[r] = (const T*)p.b + (size_t)min(j0 + r * 16 + (lane & 15), p.J - 1) * p.b_ld + ko;
+  }
+  const int k0 = wave * kper, k1 = min(p.Kc, k0 + kper);
+  f32x4 acc[R][R];
+#pragma unroll
+  for (int a = 0; a < R; ++a)
+#pragma unroll
+    for (int b = 0; b < R; ++b) acc[a][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int k = k0; k < k1; k += U * STEP) {
+    u32x4 fa[U][R], fb[U][R];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int at = k + u * STEP, n = k1 - at - ko;
+      if (at + STEP <= k1) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          fa[u][r] = *(const u32x4_any*)(pa[r] + at);
+          fb[u][r] = *(const u32x4_any*)(pb[r] + at);
+        }
+      } else {
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          fa[u][r] = n > 0 ? load_granule(pa[r] + at, n) : u32x4{0u, 0u, 0u, 0u};
+          fb[u][r] = n > 0 ? load_granule(pb[r] + at, n) : u32x4{0u, 0u, 0u, 0u};
+        }
+      }
     }
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
+    for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(fb[u][e], fa[u][e], acc, 0, 0, 0);
+      for (int a = 0; a < R; ++a)
+#pragma unroll
+        for (int b = 0; b < R; ++b) acc[a][b] = granule_mma((const T*)nullptr, fa[u][a], fb[u][b], acc[a][b]);
   }
-  if (waves > 1) {
-    part[wave][lane] = acc;
-    __syncthreads();
-    if (wave) return;
-    acc = part[0][lane];
-    for (int w = 1; w < waves; ++w) acc += part[w][lane];
+  auto store = [&](int f, f32x4 v) {
+    const int i = i0 + f / R * 16 + (lane & 15), j = j0 + f % R * 16 + 4 * (lane >> 4);
+    if constexpr (sizeof(T) == 2) store4<MODE_FWD, HEAVY>(p, i, j, v, bias4<MODE_FWD>(p, j));
+    else f32_store<MODE_FWD>(p, 0, i, j, v);
+  };
+  if (waves == 1) {
+#pragma unroll
+    for (int f = 0; f < R * R; ++f) store(f, acc[f / R][f % R]);
+    return;
   }
-  f32_store<MODE_FWD>(p, 0, i0 + (lane & 15), j0 + 4 * (lane >> 4), acc);
+#pragma unroll
+  for (int f = 0; f < R * R; ++f) part[(wave * R * R + f) * 64 + lane] = acc[f / R][f % R];
+  __syncthreads();
+  for (int f = wave; f < R * R; f += waves) {
+    f32x4 v = part[f * 64 + lane];
+    for (int w = 1; w < waves; ++w) v += part[(w * R * R + f) * 64 + lane];
+    store(f, v);
+  }
 }
 
 // ------------------------------------------------------------------------------------------------ dz, db, slab sums
@@ -906,9 +930,19 @@ template <int MODE, int NWI, int NWJ, int WI, int WJ, int K, int ST, bool HEAVY>
   hipLaunchKernelGGL(k, dim3(grid), dim3(64 * NWI * NWJ), lds, s, p);
   return hipGetLastError();
 }
-template <int MODE, int T> hipError_t launch_f32(const LinP& p, int grid, hipStream_t s) {
-  constexpr size_t lds = 2 * (size_t)(F32Tile<MODE == MODE_DW, T>::FLOATS + F32Tile<MODE != MODE_FWD, T>::FLOATS) * sizeof(float);
-  auto k = linear_f32_kernel<MODE, T>;
+template <typename T, int R, bool HEAVY> hipError_t launch_blocks_of(const LinP& p, int grid, int waves, int kper, hipStream_t s) {
+  const size_t lds = waves > 1 ? (size_t)waves * R * R * 64 * sizeof(f32x4) : 0;
+  auto k = linear_blocks_kernel<T, R, HEAVY>;
+  hipLaunchKernelGGL(k, dim3(grid), dim3(64 * waves), lds, s, p, kper);
+  return hipGetLastError();
+}
+template <typename T, bool HEAVY> hipError_t launch_blocks(int R, const LinP& p, int grid, int waves, int kper, hipStream_t s) {
+  return R == 1 ? launch_blocks_of<T, 1, HEAVY>(p, grid, waves, kper, s)
+                : launch_blocks_of<T, 2, HEAVY>(p, grid, waves, kper, s);
+}
+template <int MODE, int T, bool WHOLE> hipError_t launch_f32(const LinP& p, int grid, hipStream_t s) {
+  constexpr size_t lds = 2 * (size_t)(F32Tile<MODE == MODE_DW, T, WHOLE>::FLOATS + F32Tile<MODE != MODE_FWD, T, WHOLE>::FLOATS) * sizeof(float);
+  auto k = linear_f32_kernel<MODE, T, WHOLE>;
   if (hipError_t e = plyolo::ensure_dynamic_lds((const void*)k, lds); e != hipSuccess) return e;
   hipLaunchKernelGGL(k, dim3(grid), dim3(256), lds, s, p);
   return hipGetLastError();
@@ -930,7 +964,11 @@ template <int T, bool DIRECT> hipError_t launch_both(const LinP& px, const LinP&
   return hipGetLastError();
 }
 template <int MODE> hipError_t launch_gemm(int dtype, const LinP& p, int tile, int grid, bool direct, hipStream_t s) {
-  if (dtype != PLYOLO_BF16) return tile == 128 ? launch_f32<MODE, 128>(p, grid, s) : launch_f32<MODE, 64>(p, grid, s);
+  if (dtype != PLYOLO_BF16) {
+    const bool whole = (MODE == MODE_DW ? p.I % 4 : p.Kc % 4) == 0 && (MODE == MODE_FWD ? p.Kc % 4 : p.J % 4) == 0;
+    if (whole) return tile == 128 ? launch_f32<MODE, 128, true>(p, grid, s) : launch_f32<MODE, 64, true>(p, grid, s);
+    return tile == 128 ? launch_f32<MODE, 128, false>(p, grid, s) : launch_f32<MODE, 64, false>(p, grid, s);
+  }
   if (MODE == MODE_FWD && p.act > PLYOLO_ACT_LRELU) return launch_bf16<MODE, MODE == MODE_FWD>(p, tile, grid, direct, s);
   return launch_bf16<MODE, false>(p, tile, grid, direct, s);
 }
@@ -960,24 +998,27 @@ int plyolo_linear_fwd(const plyolo_linear_desc* d, const void* x, const void* w,
   const int dtype = d->dtype;
   const double m = d->M, n = d->N, k = d->K;
   plyolo::annotate("linear_fwd", 2.0 * m * n * k, (m * k + n * k + m * n * (1.0 + (z ? 1 : 0) + (res ? 1 : 0))) * es);
-  // 16 x 16 blocks re-read x once per 16 columns and w once per 16 rows, out of L2 at about 9.6 bytes a nanosecond and block column; a tile walks
-  // its whole contraction by itself.  Microseconds, fitted over M 16 .. 51200, N 16 .. 2048, K 32 .. 2048, M x K x N here (bf16: 64 x 2048 x
-  // 1024 6.8 in blocks, 13.6 in tiles; 256 x 1024 x 1024 10.1 / 8.8; 12800 x 64 x 64 6.2 / 4.5.  fp32: 64 x 2048 x 1024 11.4 / 75; 400 x 512 x
-  // 512 10.6 / 23.6; 3200 x 512 x 512 49 / 37)
-  const double again = (m * k * cdiv(d->N, 16) + n * k * cdiv(d->M, 16)) * es;
-  const double blocks_us = 3.4 + again / 9.6e6, tiles_us = 4.0 + k * (dtype == PLYOLO_BF16 ? 0.31 / 64 : 1.0 / 29);
-  if (blocks_us < tiles_us) {
-    const int grid = tile_grid(p, 16, 1, "linear_fwd");
+  // Blocks of 16 R x 16 R re-read x once per 16 R columns and w once per 16 R rows, out of L2; a tile walks its whole contraction by itself.
+  // Estimated microseconds, fitted over M 16 .. 51200, N 16 .. 2048, K 32 .. 2048.  Measured, M x K x N, us with R = 1 / R = 2 / tiles:
+  //   bf16  64 x 2048 x 1024  6.8 / 10.4 / 13.6   256 x 1024 x 1024  10.2 /  7.4 /  9.0   12800 x 64 x 64  6.5 / 5.1 / 4.4
+  //   fp32  64 x 2048 x 1024 11.4 / 22.2 / 53.3   256 x 1024 x 1024  18.5 / 14.1 / 30.8   3200 x 512 x 512  54 / 37 / 27.8
+  const bool half = dtype == PLYOLO_BF16;
+  auto again = [&](int e) { return (m * k * cdiv(d->N, e) + n * k * cdiv(d->M, e)) * es; };
+  const double one_us = half ? 3.4 + again(16) / 9.6e6 : 6.0 + again(16) / 9.0e6, two_us = half ? 3.6 + again(32) / 8.0e6 : 5.0 + again(32) / 7.5e6;
+  const double tiles_us = half ? 4.0 + k * 0.31 / 64 : 6.5 + k / (d->K % 4 == 0 ? 43 : 29);
+  const bool fill = (int64_t)cdiv(d->M, 32) * cdiv(d->N, 32) >= 192;      // blocks of 32 leave too many of the 256 CUs without work below this
+  const int R = fill && two_us < one_us ? 2 : 1;
+  if ((R == 2 ? two_us : one_us) < tiles_us) {
+    const int grid = tile_grid(p, 16 * R, 1, "linear_fwd");
     if (grid < 0) return -1;
-    const int step = dtype == PLYOLO_BF16 ? 32 : 16;
+    const int step = half ? 32 : 16;
     int waves = 1;
     while (waves < 16 && waves * 2 * step <= d->K && (int64_t)grid * waves < 4096) waves *= 2;
     const int kper = cdiv(cdiv(d->K, waves), step) * step;
     return plyolo::submit(stream, [=](hipStream_t s) -> hipError_t {
-      if (dtype != PLYOLO_BF16) hipLaunchKernelGGL(linear_f32_narrow_kernel, dim3(grid), dim3(64 * waves), 0, s, p, kper);
-      else if (p.act > PLYOLO_ACT_LRELU) hipLaunchKernelGGL(linear_bf16_narrow_kernel<true>, dim3(grid), dim3(64 * waves), 0, s, p, kper);
-      else hipLaunchKernelGGL(linear_bf16_narrow_kernel<false>, dim3(grid), dim3(64 * waves), 0, s, p, kper);
-      return hipGetLastError();
+      return !half                       ? launch_blocks<float, false>(R, p, grid, waves, kper, s)
+             : p.act > PLYOLO_ACT_LRELU ? launch_blocks<bf16_t, true>(R, p, grid, waves, kper, s)
+                                        : launch_blocks<bf16_t, false>(R, p, grid, waves, kper, s);
     });
   }
   const bool direct = rows16(x, d->x_ld, d->K) && rows16(w, d->w_ld, d->K);
