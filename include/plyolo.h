@@ -513,7 +513,7 @@ int plyolo_lnw_act_bwd(int dtype, int N, int H, int W, int C, const void* dout, 
  * Statistics and gradient sums are formed in a fixed order (no atomics): results repeat bit for bit.  A NaN or infinity stays inside its
  * (image, group).  No operand may overlap another, except out == x and dx == dout (same pitch).
  * Workspace: plyolo_gn_workspace(d) bytes, 16-byte aligned, contents need not survive a call; calls that may run at the same time
- * (streams, captured graphs) need one each.  C <= 4096, N*HW and every pitch below 2^31. */
+ * (streams, captured graphs) need one each.  C <= 4096, N*HW and every pitch below 2^31, N * ceil(groups / 32) below 2^22 - 128. */
 typedef struct plyolo_gn_desc {
   int dtype, N, HW, C, groups, act;
   float eps;
@@ -538,7 +538,7 @@ int plyolo_gn_act_bwd(const plyolo_gn_desc* d, const void* dout, int d_ld, const
  * whose rows start on 16-byte boundaries with K and N multiples of 8 (bf16) take the wide path.  dy rows have pitch y_ld.
  * Every sum runs in a fixed order: results repeat bit for bit.  No operand may overlap another.
  * Workspace: plyolo_linear_workspace(d, backward) bytes, 16-byte aligned, one per call that may run at the same time (0 bytes: none
- * needed, pass NULL). */
+ * needed, pass NULL).  N, K <= 2^20, N * K < 2^30, at most 2^23 output tiles of 64 x 64. */
 typedef struct plyolo_linear_desc {
   int dtype, M, N, K, act;
   int x_ld, w_ld, y_ld, z_ld, r_ld;
@@ -556,6 +556,7 @@ int plyolo_linear_bwd(const plyolo_linear_desc* d, const void* dy, const void* z
  * counter = (low and high half of i / 4, low half of step, site), key = the halves of seed; it is kept when word >> 8 >= round(p * 2^24).
  * rng: device uint64[2] = {seed, step}, read by the launch (so a captured or replayed launch follows the state); `site` tells the
  * dropouts of one step apart.  0 <= p <= 1 (p = 1: nothing is kept).  A dropped infinity or NaN is 0.  x == out (same pitch) is allowed.
+ * M * C < 2^34.
  * plyolo_rng_next: out[0..1] = state[0..1]; state[1] += 1 -- one launch per step; forward and backward of the step read `out`. */
 int plyolo_rng_next(uint64_t* state, uint64_t* out, void* stream);
 int plyolo_dropout_fwd(int dtype, int M, int C, const void* x, int x_ld, float p, const uint64_t* rng, unsigned site, const void* res, int r_ld,

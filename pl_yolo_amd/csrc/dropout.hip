@@ -170,7 +170,7 @@ int dropout_submit(const char* who, int dtype, int M, int C, const void* x, int 
   const bool wide = aligned && C % V == 0 && x_ld % V == 0 && o_ld % V == 0 && (!res || r_ld % V == 0);
   const size_t per = (flat || wide) ? (size_t)V * 256 * DROP_U : (size_t)4 * 256;
   const size_t grid = cdivz(p.total, per);
-  PLY_CHECK_ARG(grid < 2147483647u, "%s: more than 2^31 workgroups", who);
+  PLY_CHECK_ARG(grid < 16777216u, "%s: more than 2^24 workgroups", who);
   plyolo::annotate(who, 0.0, (double)p.total * es * (res || accumulate ? 3.0 : 2.0));
   return plyolo::submit(stream, [=](hipStream_t s) -> hipError_t {
     const dim3 g((unsigned)grid), b(256);

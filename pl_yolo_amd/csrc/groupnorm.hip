@@ -752,8 +752,8 @@ int check_gn(const plyolo_gn_desc* d, const char* who) {
   PLY_CHECK_ARG(d->C % d->groups == 0, "%s: %d channels do not split into %d groups", who, d->C, d->groups);
   PLY_CHECK_ARG(d->C <= GN_MAXC, "%s: more than %d channels (%d)", who, GN_MAXC, d->C);
   PLY_CHECK_ARG((double)d->N * d->HW < 2147483648.0, "%s: more than 2^31 rows", who);
-  // workgroups of a launch: (image, slice or 32 groups), and at most 32 channel blocks more
-  PLY_CHECK_ARG((double)d->N * d->C < 17179869184.0 && (double)d->N * ((d->groups + 31) / 32 + 1) < 2147483000.0, "%s: too many images (%d)", who, d->N);
+  // a launch has fewer than 2^32 threads: 1024 for every JOIN_I groups of an image, and for at most 128 blocks of channels
+  PLY_CHECK_ARG((double)d->N * cdiv(d->groups, JOIN_I) < 4194304.0 - 128, "%s: too many images (%d)", who, d->N);
   PLY_CHECK_ARG(d->act >= PLYOLO_ACT_NONE && d->act <= PLYOLO_ACT_GELU, "%s: bad activation %d", who, d->act);
   PLY_CHECK_ARG(d->eps >= 0.f, "%s: eps must not be negative", who);
   PLY_CHECK_ARG(d->x_ld >= d->C, "%s: x_ld %d < C %d", who, d->x_ld, d->C);
@@ -796,7 +796,7 @@ ResPlan res_plan(const plyolo_gn_desc* d, int V, bool bwd) {
   for (int sv = least; sv <= cv && sv <= 8 * esz + least; sv += least) {
     if (cv % sv != 0 || sv > RES_NT) continue;
     const int64_t wgs = (int64_t)d->N * (cv / sv);
-    if (wgs > 2147483000) continue;
+    if (wgs >= 4194304) continue;      // (a launch has fewer than 2^32 threads)
     const int rpb = RES_NT / sv, nv = (d->HW + rpb - 1) / rpb;
     if (nv > (V == 1 ? 16 : wgs < 64 ? (bwd ? 8 : 12) : bwd ? (sv >= 4 ? 16 : 8) : 32)) continue;
     if (sv > least && wgs < 256) break;

@@ -5,8 +5,10 @@
 //
 // All three products are one kernel body over two operands that are either contiguous along the contraction (KC: x and w of the forward,
 // dz of dx) or along the output (RC: w of dx, dz and x of dw); an RC operand is transposed on its way out of LDS (ds_read_b64_tr_b16 in bf16).
-// The product is formed as D = B . A^T, so that a lane of the MFMA result holds four consecutive COLUMNS of one output row and the epilogue
-// moves 8- (bf16) or 16-byte (fp32) pieces of rows.
+// The product is formed as D = B . A^T, so that a lane of the MFMA result holds four consecutive COLUMNS of one output row: 8 bytes of bf16, put
+// together to whole row pieces in LDS, or 16 of fp32, stored as they are.
+//
+// bf16: dz is rounded to bf16 once, as the operand of both matrix products (db sums it unrounded); dw has that rounding's noise beside its own.
 //
 // dw contracts over the rows of the batch: the rows are split over workgroups, every range leaves a private fp32 slab and the slabs are
 // added in a fixed order.
@@ -27,12 +29,13 @@ struct LinP {
   int a_ld, b_ld, o_ld, z_ld, r_ld;
   int act, accumulate, vec4;
   int nj, tiles;       // column tiles, all tiles of the output
-  int ksteps;          // contraction steps per slab (MODE_DW), all of them otherwise
+  int ksteps;          // MODE_DW: contraction stages per slab
 };
 
 // ------------------------------------------------------------------------------------------------ bf16
 constexpr int BK = 64;           // contraction elements per stage (and the unit that dw's row ranges are counted in)
 typedef u32x4 __attribute__((aligned(2))) u32x4_any;     // 16 bytes at any element address
+typedef f32x4 __attribute__((aligned(4))) f32x4_any;
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 DEVINL s16x4 tr_read(const unsigned char* p) { return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p); }
 
@@ -183,26 +186,23 @@ template <bool HEAVY> DEVINL void act4(f32x4& v, int act) {
   }
 }
 
-// four consecutive columns j.. of output row i; nv of them exist
-template <int MODE, bool HEAVY> DEVINL void store4(const LinP& p, int i, int j, f32x4 v, const f32x4 bias) {
+// forward: four consecutive columns j.. of output row i; nv of them exist
+template <bool HEAVY> DEVINL void store4(const LinP& p, int i, int j, f32x4 v, const f32x4 bias) {
   const int nv = p.J - j;
   if (i >= p.I || nv <= 0) return;
   const bool whole = p.vec4 && nv >= 4;
-  if (MODE == MODE_FWD) {
+  v += bias;
+  if (p.z) {
+    bf16_t* z = (bf16_t*)p.z + (size_t)i * p.z_ld + j;
+    if (whole) *(uint2*)z = make_uint2(pack2bf(v[0], v[1]), pack2bf(v[2], v[3]));
+    else
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] += bias[e];
-    if (p.z) {
-      bf16_t* z = (bf16_t*)p.z + (size_t)i * p.z_ld + j;
-      if (whole) *(uint2*)z = make_uint2(pack2bf(v[0], v[1]), pack2bf(v[2], v[3]));
-      else
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (e < nv) z[e] = f2bf(v[e]);
-    }
-    act4<HEAVY>(v, p.act);
+      for (int e = 0; e < 4; ++e)
+        if (e < nv) z[e] = f2bf(v[e]);
   }
+  act4<HEAVY>(v, p.act);
   bf16_t* o = (bf16_t*)p.out + (size_t)i * p.o_ld + j;
-  const bf16_t* r = MODE == MODE_FWD ? (p.res ? (const bf16_t*)p.res + (size_t)i * p.r_ld + j : nullptr) : (p.accumulate ? o : nullptr);
+  const bf16_t* r = p.res ? (const bf16_t*)p.res + (size_t)i * p.r_ld + j : nullptr;
   if (whole) {
     if (r) {
       const uint2 t = *(const uint2*)r;
@@ -221,7 +221,6 @@ template <int MODE, bool HEAVY> DEVINL void store4(const LinP& p, int i, int j, 
 
 // the bias of columns j .. j + 3 (zeros where there is none)
 template <int MODE> DEVINL f32x4 bias4(const LinP& p, int j) {
-  typedef f32x4 __attribute__((aligned(4))) f32x4_any;
   f32x4 b = {0.f, 0.f, 0.f, 0.f};
   if (MODE == MODE_FWD && p.bias) {
     if (j + 4 <= p.J) {
@@ -479,8 +478,6 @@ template <int T, bool DIRECT> __global__ __launch_bounds__(256) void linear_bf16
 }
 
 // ------------------------------------------------------------------------------------------------ fp32 (parity mode)
-typedef f32x4 __attribute__((aligned(4))) f32x4_any;     // 16 bytes at any element address
-
 // four consecutive elements of which n >= 1 exist (the others are zero)
 DEVINL f32x4 load4(const float* p, int n) {
   if (n >= 4) return *(const f32x4_any*)p;
@@ -697,7 +694,7 @@ template <typename T, int R, bool HEAVY> __global__ __launch_bounds__(1024) void
   }
   auto store = [&](int f, f32x4 v) {
     const int i = i0 + f / R * 16 + (lane & 15), j = j0 + f % R * 16 + 4 * (lane >> 4);
-    if constexpr (sizeof(T) == 2) store4<MODE_FWD, HEAVY>(p, i, j, v, bias4<MODE_FWD>(p, j));
+    if constexpr (sizeof(T) == 2) store4<HEAVY>(p, i, j, v, bias4<MODE_FWD>(p, j));
     else f32_store<MODE_FWD>(p, 0, i, j, v);
   };
   if (waves == 1) {
@@ -894,17 +891,17 @@ int check_linear(const plyolo_linear_desc* d, const char* who) {
   PLY_CHECK_ARG(d != nullptr, "%s: null descriptor", who);
   PLY_CHECK_ARG(d->dtype == PLYOLO_BF16 || d->dtype == PLYOLO_F32, "%s: bad dtype %d", who, d->dtype);
   PLY_CHECK_ARG(d->M > 0 && d->N > 0 && d->K > 0, "%s: non-positive dimension (M %d, N %d, K %d)", who, d->M, d->N, d->K);
-  PLY_CHECK_ARG(d->N <= (1 << 20) && d->K <= (1 << 20) && (double)d->N * d->K < 17179869184.0 && d->M <= 2147483647 - 1024, "%s: dimension too large (M %d, N %d, K %d)", who, d->M, d->N, d->K);
+  PLY_CHECK_ARG(d->N <= (1 << 20) && d->K <= (1 << 20) && (double)d->N * d->K < 1073741824.0 && d->M <= 2147483647 - 1024, "%s: dimension too large (M %d, N %d, K %d)", who, d->M, d->N, d->K);
   PLY_CHECK_ARG(d->act >= PLYOLO_ACT_NONE && d->act <= PLYOLO_ACT_GELU, "%s: bad activation %d", who, d->act);
   PLY_CHECK_ARG(d->x_ld >= d->K && d->w_ld >= d->K, "%s: x_ld %d or w_ld %d < K %d", who, d->x_ld, d->w_ld, d->K);
   return 0;
 }
 
-// workgroups of an I x J output
+// workgroups of an I x J output (a launch has fewer than 2^32 threads: those of up to 512, two such grids in one launch, 64 for the many small ones)
 int tile_grid(LinP& p, int tile, int slabs, const char* who) {
   p.nj = cdiv(p.J, tile);
   const int64_t n = (int64_t)cdiv(p.I, tile) * p.nj;
-  PLY_CHECK_ARG(n * slabs < 1073741824, "%s: more than 2^30 workgroups", who);
+  PLY_CHECK_ARG(n * slabs < (tile < 64 ? 67108864 : 8388608), "%s: more than %d workgroups", who, tile < 64 ? 67108864 : 8388608);
   p.tiles = (int)n;
   return (int)n * slabs;
 }

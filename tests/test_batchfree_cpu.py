@@ -58,7 +58,8 @@ def gn_bwd(d, dout=P, d_ld=32, x=P, stats=P, dx=P, dx_ld=32, ws=P, n=1 << 30):
 
 
 @pytest.mark.parametrize("bad", [dict(dtype=2), dict(N=0), dict(HW=0), dict(HW=-4), dict(C=0), dict(groups=0), dict(groups=5), dict(C=8192, x_ld=8192, o_ld=8192),
-                                 dict(act=6), dict(act=-1), dict(eps=-1.0), dict(eps=float("nan")), dict(x_ld=31), dict(N=65536, HW=65536)])
+                                 dict(act=6), dict(act=-1), dict(eps=-1.0), dict(eps=float("nan")), dict(x_ld=31), dict(N=65536, HW=65536),
+                                 dict(N=1 << 22, HW=1)])
 def test_gn_refuses_descriptors(bad):
     d = gn_desc(**bad)
     assert _lib.lib().plyolo_gn_workspace(C.byref(d)) == 0
@@ -94,7 +95,8 @@ def lin_bwd(d, dy=P, z=P, x=P, w=P, dx=P, dx_ld=24, dw=P, dwt=0, db=P, ws=P, n=1
     call("plyolo_linear_bwd", C.byref(d) if d is not None else None, dy, z, x, w, dx, dx_ld, 0, dw, dwt, db, 0, ws, n, None)
 
 
-@pytest.mark.parametrize("bad", [dict(dtype=7), dict(M=0), dict(N=0), dict(K=-1), dict(act=9), dict(x_ld=23), dict(w_ld=23), dict(N=1 << 21, y_ld=1 << 21)])
+@pytest.mark.parametrize("bad", [dict(dtype=7), dict(M=0), dict(N=0), dict(K=-1), dict(act=9), dict(x_ld=23), dict(w_ld=23), dict(N=1 << 21, y_ld=1 << 21),
+                                 dict(N=1 << 15, K=1 << 15, x_ld=1 << 15, w_ld=1 << 15, y_ld=1 << 15)])
 def test_linear_refuses_descriptors(bad):
     d = lin_desc(**bad)
     with pytest.raises(PlyoloError, match="linear_fwd"):
@@ -117,6 +119,9 @@ def test_linear_refuses_operands():
                dict(ws=P + 8), dict(n=need - 1), dict(dy=P + 1), dict(dw=P + 2, dwt=1)):
         with pytest.raises(PlyoloError, match="linear_bwd"):
             lin_bwd(lin_desc(), **kw)
+    for f in (lin_fwd, lin_bwd):            # more tiles than one launch has room for
+        with pytest.raises(PlyoloError, match="workgroups"):
+            f(lin_desc(M=2147480000, N=64, K=1, y_ld=64, z_ld=64), z=P)
     with pytest.raises(PlyoloError, match="dw_dtype"):
         lin_bwd(lin_desc(dtype=1), dwt=0)      # bf16 weight gradients of an fp32 layer
 
@@ -126,7 +131,8 @@ def drop(M=4, Cc=8, x=P, x_ld=8, p=0.5, rng=P, res=None, r_ld=0, out=P, o_ld=8, 
 
 
 @pytest.mark.parametrize("kw", [dict(M=0), dict(Cc=0), dict(x=None), dict(rng=None), dict(out=None), dict(x_ld=7), dict(o_ld=7), dict(res=P, r_ld=7), dict(p=-0.1),
-                                dict(p=1.5), dict(p=float("nan")), dict(dt=4), dict(x=P + 1), dict(rng=P + 4)])
+                                dict(p=1.5), dict(p=float("nan")), dict(dt=4), dict(x=P + 1), dict(rng=P + 4),
+                                dict(M=2147483647, Cc=1024, x_ld=1024, o_ld=1024)])
 def test_dropout_refuses(kw):
     with pytest.raises(PlyoloError, match="dropout_fwd"):
         drop(**kw)

@@ -117,6 +117,8 @@ GN_SHAPES = [  # n, hw, c, groups, pad, off
     (1, 20011, 24, 8, 0, 0),        # one long image, ragged last chunk
     (33, 3, 16, 4, 0, 0),           # many short images
     (1, 130, 4096, 4096, 0, 0),     # as many groups as the largest channel count
+    (8, 9000, 64, 32, 0, 0),        # held in registers by 1024 threads
+    (13, 1500, 200, 5, 0, 0),       # ... by a slice of five vectors
 ]
 
 
@@ -363,6 +365,55 @@ def test_linear_forward_backward(shape, dt):
     y3, z3 = t.fwd()
     dx3, dw3, db3 = t.bwd(dy, z)
     assert torch.equal(y.v, y3.v) and torch.equal(z.v, z3.v) and torch.equal(dx.v, dx3.v) and torch.equal(dw, dw3) and torch.equal(db, db3)
+
+
+LIN_LARGE = [  # m, n, k, pad, off: each the smallest kind of layer that takes the tile
+    (8200, 1032, 520, 0, 0),        # 256 x 256 forward, ragged in every direction
+    (8200, 520, 1032, 8, 0),        # 256 x 256 dx
+    (12900, 264, 248, 0, 0),        # 128 x 128, dx and dw in one launch
+    (12900, 259, 251, 1, 0),        # ... through registers
+    (400, 512, 512, 0, 0),          # 32 x 32 blocks
+    (333, 515, 509, 0, 1),          # ... with cut rows
+    (3300, 500, 300, 0, 0),         # 64 x 64 tiles, rows of whole fp32 vectors but not of bf16 ones
+]
+
+
+@pytest.mark.parametrize("dt", [BF16, F32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("shape", LIN_LARGE, ids=lambda s: "m%d_n%d_k%d_p%d_o%d" % s)
+def test_linear_large(shape, dt):
+    m, n, k, pad, off = shape
+    t = Lin(dt, m, n, k, "silu", True, pad, off, pad)
+    res = t.rows(rnd(m, n, 8))
+    y, z = t.fwd(res)
+    t.check_fwd(y, z, res)
+    dy = t.rows(rnd(m, n, 9, 0.1))
+    base = Mat(m, k, dt, pad, off, rnd(m, k, 10, 0.1))
+    b64 = base.v.double().clone()
+    dx, dw, db = t.bwd(dy, z, dxm=base, acc_dx=1)
+    t.check_bwd(dy, z, dx, dw, db, base=b64)
+    y2, _ = t.fwd(res, z=False)
+    assert torch.equal(y.v, y2.v)
+    base.v.copy_(b64.to(base.v.dtype))
+    dx2, dw2, db2 = t.bwd(dy, z, dxm=base, acc_dx=1)
+    t.check_bwd(dy, z, dx2, None, None, base=b64)
+    assert torch.equal(dw, dw2) and torch.equal(db, db2)
+
+
+def test_linear_first_call_captured():
+    """The first launch of a kernel that needs more than 64 KiB of LDS may be a captured one."""
+    t = Lin(BF16, 8200, 1032, 520, "gelu")
+    y, z = t.rows(), t.rows()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=side):
+        call("plyolo_linear_fwd", C.byref(t.d), t.x.ptr, t.w.ptr, ptr(t.b), None, z.ptr, y.ptr, None, 0, torch.cuda.current_stream().cuda_stream)
+    for _ in range(3):
+        y.v.zero_()
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        t.check_fwd(y, z)
 
 
 @pytest.mark.parametrize("dt", [BF16, F32], ids=["bf16", "fp32"])
@@ -629,3 +680,45 @@ def test_two_streams_with_their_own_workspaces():
     torch.cuda.synchronize()
     for x, y, z in zip(a.results(), b.results(), want):
         assert torch.equal(x, z) and torch.equal(y, z)
+
+
+def test_rows_beyond_32_bit_offsets():
+    """Pitches that put the last rows more than 2^31 elements behind the first: bit for bit what packed rows give."""
+    m, c, ld = 70000, 16, 32000
+    big = torch.empty(m * ld, dtype=torch.bfloat16, device=DEV)
+
+    def col(i, data=None):
+        v = big.as_strided((m, c), (ld, 1), 64 * i)
+        if data is not None:
+            v.copy_(data)
+        return v
+    data = {s: rnd(m, c, s).bfloat16() for s in (1, 2, 3)}
+    w, b, ga, be = rnd(c, c, 4, 0.3).bfloat16(), rnd(1, c, 5).flatten(), rnd(1, c, 6).flatten(), rnd(1, c, 7).flatten()
+    rng = torch.tensor([77, 5], dtype=torch.int64, device=DEV)
+    lib, s = _lib.lib(), hu.stream()
+
+    def run(place, ld):
+        x, res, dy = place(0, data[1]), place(1, data[2]), place(2, data[3])
+        z, y, dx, o, dg, dd = (place(i) for i in range(3, 9))
+        d = LinearDesc()
+        d.dtype, d.M, d.N, d.K, d.act, d.x_ld, d.w_ld, d.y_ld, d.z_ld, d.r_ld = BF16, m, c, c, ACTS["silu"], ld, c, ld, ld, ld
+        nws = lib.plyolo_linear_workspace(C.byref(d), 1)
+        ws = torch.empty(nws, dtype=torch.uint8, device=DEV)
+        dw, db = torch.empty(c, c, dtype=torch.bfloat16, device=DEV), torch.empty(c, device=DEV)
+        call("plyolo_linear_fwd", C.byref(d), x.data_ptr(), w.data_ptr(), ptr(b), res.data_ptr(), z.data_ptr(), y.data_ptr(), None, 0, s)
+        call("plyolo_linear_bwd", C.byref(d), dy.data_ptr(), z.data_ptr(), x.data_ptr(), w.data_ptr(), dx.data_ptr(), ld, 0, dw.data_ptr(), BF16, ptr(db), 0,
+             ws.data_ptr(), nws, s)
+        g = GnDesc()
+        g.dtype, g.N, g.HW, g.C, g.groups, g.act, g.eps, g.x_ld, g.o_ld, g.r_ld = BF16, 2, m // 2, c, 4, ACTS["silu"], 1e-5, ld, ld, ld
+        nws = lib.plyolo_gn_workspace(C.byref(g))
+        ws2 = torch.empty(nws, dtype=torch.uint8, device=DEV)
+        st, dga, dbe = torch.empty(2, 4, 2, device=DEV), torch.empty(c, device=DEV), torch.empty(c, device=DEV)
+        call("plyolo_gn_act_fwd", C.byref(g), x.data_ptr(), ptr(ga), ptr(be), res.data_ptr(), o.data_ptr(), ptr(st), ws2.data_ptr(), nws, s)
+        call("plyolo_gn_act_bwd", C.byref(g), dy.data_ptr(), ld, x.data_ptr(), ptr(st), ptr(ga), ptr(be), dg.data_ptr(), ld, 0, ptr(dga), ptr(dbe), 0,
+             ws2.data_ptr(), nws, s)
+        call("plyolo_dropout_fwd", BF16, m, c, x.data_ptr(), ld, 0.25, rng.data_ptr(), 3, res.data_ptr(), ld, dd.data_ptr(), ld, s)
+        return [t.clone() for t in (z, y, dx, dw, db, o, st, dg, dga, dbe, dd)]
+    far = run(col, ld)
+    near = run(lambda i, v=None: v.clone() if v is not None else torch.empty(m, c, dtype=torch.bfloat16, device=DEV), c)
+    for name, a, e in zip(("z", "y", "dx", "dw", "db", "gn", "stats", "gn dx", "dgamma", "dbeta", "dropout"), far, near):
+        assert torch.equal(a, e), name
