@@ -95,9 +95,10 @@ template <int TI, int TJ> DEVINL Place place(const LinP& p, int block, int block
 // swizzle is applied to its source); otherwise through registers: a granule that a row's end cuts is fetched as the row's last eight elements
 // and shifted on its way to LDS, so that no request waits for another (rows of fewer than eight elements: one by one).
 template <bool RC, int T, int K, int NT, bool DIRECT> struct Tile {
-  static constexpr int NG = T * K / 8 / NT;      // 16-byte granules per thread
+  static constexpr int NG = (T * K / 8 + NT - 1) / NT;      // 16-byte granules per thread (the last of them: whole waves only)
   static constexpr int BYTES = T * K * 2, KG = K / 8, TG = T / 8;
-  static_assert(NG * NT * 8 == T * K, "whole granules per thread");
+  static_assert(T * K / 8 % (DIRECT ? 64 : NT) == 0, "a wave requests whole granules or none");
+  static DEVINL bool mine(int u) { return (u + 1) * NT * 8 <= T * K || (int)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 64 < T * K / 8 - u * NT; }
   static DEVINL int swz_k(int k) { return T >= 128 ? (k & 3) | ((k >> 1) & 4) : (k & 3); }
   static DEVINL int swz_r(int r) { return K == 64 ? r & 7 : (r >> 1) & 3; }
   const bf16_t* src[NG];     // granule u at contraction 0 of the workgroup (NULL: its row does not exist)
@@ -136,7 +137,7 @@ template <bool RC, int T, int K, int NT, bool DIRECT> struct Tile {
       const bool ok = src[u] != nullptr && kof[u] < left;
       if (DIRECT) {
         const void* g = ok ? (const void*)q : (const void*)&zero_granule;
-        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)g,
+        if (mine(u)) __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)g,
                                          (__attribute__((address_space(3))) void*)(img + (u * NT + wave * 64) * 16), 16, 0, 0);
       } else {
         const int w = DIRECT ? 0 : u, n = RC ? len[w] : left - kof[u];
@@ -396,7 +397,7 @@ template <int MODE, int NWI, int NWJ, int WI, int WJ, int K, int ST, bool HEAVY>
   typedef Tile<ARC, TI, K, NT, true> TA;
   typedef Tile<BRC, TJ, K, NT, true> TB;
   constexpr int STAGE = TA::BYTES + TB::BYTES, LOADS = TA::NG + TB::NG;
-  static_assert(ST >= 2 && ST <= 4, "the waits below");
+  static_assert(ST >= 2 && ST <= 3 && (ST == 2 || (TI * K / 8 % NT == 0 && TJ * K / 8 % NT == 0)), "the waits below count a wave's loads");
   extern __shared__ __align__(16) unsigned char smem[];
   const Place at = place<TI, TJ>(p, block, blocks);
   const int i0 = at.i0, j0 = at.j0;
@@ -421,8 +422,7 @@ template <int MODE, int NWI, int NWJ, int WI, int WJ, int K, int ST, bool HEAVY>
   for (int k0 = 0; k0 < klen; k0 += K, buf = buf + 1 == ST ? 0 : buf + 1) {
     unsigned char *ia = smem + buf * STAGE, *ib = ia + TA::BYTES;
     const int behind = klen - k0;                  // stages requested behind this one: as many as there are, ST - 2 at most
-    if (ST == 4 && behind > 2 * K) wait_and_meet<2 * LOADS>();
-    else if (ST >= 3 && behind > K) wait_and_meet<LOADS>();
+    if (ST == 3 && behind > K) wait_and_meet<LOADS>();
     else wait_and_meet<0>();
     if (behind > (ST - 1) * K) {
       unsigned char* na = smem + (buf == 0 ? ST - 1 : buf - 1) * STAGE;
@@ -844,12 +844,14 @@ struct BwdPlan {
 
 size_t up16(size_t v) { return (v + 15) & ~(size_t)15; }
 
-// Tile edge of an I x J output (bf16): the larger the tile, the fewer LDS reads per MFMA and the fewer re-reads of the operands; the smaller,
-// the more of the chip a small output fills.
-int pick_tile(int64_t I, int64_t J, int64_t Kc, bool direct) {      // (fp32: direct = false)
-  auto tiles = [&](int a) { return ((I + a - 1) / a) * ((J + a - 1) / a); };
-  if (direct && tiles(256) >= 128 && J > 128 && Kc >= 512) return 256;
-  if (tiles(128) >= 192 && J > 64) return 128;
+// Tile of an I x J output: the larger, the fewer LDS reads per MFMA and the fewer re-reads of the operands; the smaller, the more of the chip a
+// small output fills.  256 (x 256, eight waves: one workgroup per compute unit) becomes 224 x 256 where that is still one round of the 256
+// compute units: 12800 x 2048 x 1024 82 -> 77 us, 12800 x 1024 x 1024 45 -> 43 us (M x K x N, z and y written, inputs from HBM).
+// 128 x 128 in place of 256 x 256 costs a sixth there.  fp32 and operands that pass registers (direct false): 128 or 64.
+int pick_tile(int64_t I, int64_t J, int64_t Kc, bool direct) {
+  auto tiles = [&](int a, int b) { return ((I + a - 1) / a) * ((J + b - 1) / b); };
+  if (direct && tiles(256, 256) >= 128 && J > 128 && Kc >= 512) return tiles(224, 256) <= 256 ? 224 : 256;
+  if (tiles(128, 128) >= 192 && J > 64) return 128;
   return 64;
 }
 
@@ -899,7 +901,7 @@ int check_linear(const plyolo_linear_desc* d, const char* who) {
 
 // workgroups of an I x J output (a launch has fewer than 2^32 threads: those of up to 512, two such grids in one launch, 64 for the many small ones)
 int tile_grid(LinP& p, int tile, int slabs, const char* who) {
-  p.nj = cdiv(p.J, tile);
+  p.nj = cdiv(p.J, tile == 224 ? 256 : tile);
   const int64_t n = (int64_t)cdiv(p.I, tile) * p.nj;
   PLY_CHECK_ARG(n * slabs < (tile < 64 ? 67108864 : 8388608), "%s: more than %d workgroups", who, tile < 64 ? 67108864 : 8388608);
   p.tiles = (int)n;
@@ -947,7 +949,10 @@ template <int MODE, int T, bool WHOLE> hipError_t launch_f32(const LinP& p, int 
 // direct: both operands' granules are whole and 16-byte aligned
 template <int MODE, bool HEAVY> hipError_t launch_bf16(const LinP& p, int tile, int grid, bool direct, hipStream_t s) {
   if (direct) {
-    if constexpr (MODE != MODE_DW) if (tile == 256) return launch_direct<MODE, 2, 4, 128, 64, 64, 2, HEAVY>(p, grid, s);
+    if constexpr (MODE != MODE_DW) {
+      if (tile == 256) return launch_direct<MODE, 2, 4, 128, 64, 64, 2, HEAVY>(p, grid, s);
+      if (tile == 224) return launch_direct<MODE, 2, 4, 112, 64, 64, 2, HEAVY>(p, grid, s);
+    }
     if (tile == 128) return launch_direct<MODE, 2, 2, 64, 64, 64, 2, HEAVY>(p, grid, s);
     return launch_direct<MODE, 2, 2, 32, 32, 64, 3, HEAVY>(p, grid, s);
   }

@@ -368,8 +368,10 @@ def test_linear_forward_backward(shape, dt):
 
 
 LIN_LARGE = [  # m, n, k, pad, off: each the smallest kind of layer that takes the tile
-    (8200, 1032, 520, 0, 0),        # 256 x 256 forward, ragged in every direction
-    (8200, 520, 1032, 8, 0),        # 256 x 256 dx
+    (8200, 1032, 520, 0, 0),        # 224 x 256 forward, ragged in every direction
+    (8200, 520, 1032, 8, 0),        # 224 x 256 dx
+    (11600, 1288, 520, 0, 0),       # 256 x 256 forward
+    (11600, 520, 1288, 0, 0),       # 256 x 256 dx
     (12900, 264, 248, 0, 0),        # 128 x 128, dx and dw in one launch
     (12900, 259, 251, 1, 0),        # ... through registers
     (400, 512, 512, 0, 0),          # 32 x 32 blocks
