@@ -855,14 +855,15 @@ int pick_tile(int64_t I, int64_t J, int64_t Kc, bool direct) {
   return 64;
 }
 
-// Tile and slabs of dw: enough row ranges to give every compute unit a workgroup, as long as the slabs are not more to move than the operands;
-// a layer that does not get there with 128 x 128 tiles takes small ones.
+// Tile and slabs of dw: enough row ranges to give every compute unit a workgroup (bf16: three quarters of them, dx's workgroups of the same
+// launch take the rest; 51200 x 256 x 256 backward 62 us, 64 with 256 workgroups, 71 with 128 or 384), as long as the slabs are not more to
+// move than the operands; a layer that does not get there with 128 x 128 tiles takes small ones.
 void dw_plan(const plyolo_linear_desc* d, int tile, BwdPlan* b) {
   const bool half = d->dtype == PLYOLO_BF16;
   const int64_t tiles = (int64_t)cdiv(d->N, tile) * cdiv(d->K, tile);
   const int steps = cdiv(d->M, half ? BK : FK);
   const double slab = 4.0 * d->N * d->K, operands = (half ? 2.0 : 4.0) * d->M * ((double)d->N + d->K);
-  int64_t s = (256 + tiles - 1) / tiles;
+  int64_t s = ((half ? 192 : 256) + tiles - 1) / tiles;
   if (s > operands / slab) s = (int64_t)(operands / slab);
   if (s > steps) s = steps;
   if (s < 1) s = 1;

@@ -578,7 +578,8 @@ class Graph:
     def next_rng(self):
         """In front of a forward plan's ops: this step's (seed, step) for its dropouts, and the module's step counter moved on."""
         if self.rng is not None and self.training:
-            call("plyolo_rng_next", rng_state_of(self.root, self.device).data_ptr(), self.rng.data_ptr(), None)
+            self.rng_state = rng_state_of(self.root, self.device)      # (kept: the recorded launch holds its address)
+            call("plyolo_rng_next", self.rng_state.data_ptr(), self.rng.data_ptr(), None)
 
     def top_is(self, module):
         return self.root is module

@@ -163,7 +163,8 @@ def emit_pair(g, x, unit_a, unit_b):
     act_a = unit_a.act.act_name if unit_a.act is not None else None
     act_b = unit_b.act.act_name if unit_b.act is not None else None
     same = (g.pair_convs and ca.kernel_size == cb.kernel_size and unit_a.stride == unit_b.stride and act_a == act_b
-            and isinstance(na, nn.BatchNorm2d) and isinstance(nb, nn.BatchNorm2d) and not (getattr(unit_a, "drop", 0.0) or getattr(unit_b, "drop", 0.0)) and na.eps == nb.eps and na.momentum == nb.momentum
+            and isinstance(na, nn.BatchNorm2d) and isinstance(nb, nn.BatchNorm2d) and na.eps == nb.eps and na.momentum == nb.momentum
+            and not (getattr(unit_a, "drop", 0.0) or getattr(unit_b, "drop", 0.0))
             and ca.out_channels % g.vec == 0 and cb.out_channels % g.vec == 0)
     if not same:
         return unit_a.emit(g, x), unit_b.emit(g, x)
