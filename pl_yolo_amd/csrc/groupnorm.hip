@@ -79,8 +79,12 @@ struct GnP {
   int x_ld, d_ld, r_ld, o_ld;
   int chunks, rows;    // row chunks per image, rows per chunk
   int acc_dx, acc_par;
-  float eps;
+  float eps, inv_cg;   // 1 / cg
+  double inv_count;    // 1 / (HW cg)
 };
+// c / cg without an integer division: c + 1/2 is at least 1 / (2 cg) from every multiple of cg, relative 2^-13 at c <= 4096, and the product is
+// off by 2^-23
+DEVINL int group_of(const GnP& p, int c) { return (int)(((float)c + 0.5f) * p.inv_cg); }
 
 // lanes per group for the joins below: a power of two <= 64 with lanes * G <= 256 where that is possible
 DEVINL int join_lanes(int G) {
@@ -132,7 +136,7 @@ template <typename T, int V> __global__ __launch_bounds__(256) void gn_stats_ker
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         const float m2 = q[e] - s[e] * s[e] * inv;
-        const float from = k[e] - gn_origin<T>(p, n, (col * V + e) / p.cg);
+        const float from = k[e] - gn_origin<T>(p, n, group_of(p, col * V + e));
         red[(trow * cols + tcol) * V + e] = make_float2(from + s[e] * inv, m2 < 0.f ? 0.f : m2);   // (a NaN passes)
       }
     }
@@ -222,7 +226,7 @@ template <typename T, int JOIN_NT> __global__ __launch_bounds__(JOIN_NT) void gn
     const double total = (double)p.HW * p.cg, mean = s / total, m2 = q - s * mean;
     float* st = p.stats + ((size_t)n * p.G + g) * 2;
     st[0] = (float)(mean + (double)gn_origin<T>(p, n, g));
-    st[1] = (float)(1.0 / sqrt((m2 < 0.0 ? 0.0 : m2) / total + (double)p.eps));
+    st[1] = (float)rsqrt((m2 < 0.0 ? 0.0 : m2) * p.inv_count + (double)p.eps);
   }
 }
 
@@ -256,7 +260,7 @@ template <typename T, int V, int ACTC> __global__ __launch_bounds__(256) void gn
     request(col, trow);
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-      const int c = col * V + e, g = c / p.cg;
+      const int c = col * V + e, g = group_of(p, c);
       mu[e] = st[2 * g];
       a[e] = st[2 * g + 1] * (p.gamma ? p.gamma[c] : 1.f);
       b[e] = p.beta ? p.beta[c] : 0.f;
@@ -318,7 +322,7 @@ template <typename T, int V, int ACTC> __global__ __launch_bounds__(256) void gn
       float mu[V], rs[V], ga[V], be[V], sa[V], sb[V];
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        const int c = col * V + e, g = c / p.cg;
+        const int c = col * V + e, g = group_of(p, c);
         mu[e] = st[2 * g];
         rs[e] = st[2 * g + 1];
         ga[e] = rs[e] * (p.gamma ? p.gamma[c] : 1.f);
@@ -400,7 +404,7 @@ template <int JOIN_NT> __global__ __launch_bounds__(JOIN_NT) void gn_join_bwd_ke
   const int blk = blockIdx.x - npar, gb = (p.G + JOIN_I - 1) / JOIN_I, n = blk / gb, g = (blk % gb) * JOIN_I + threadIdx.x % JOIN_I;
   join_sums<JOIN_NT>(p.gpart + (size_t)n * p.chunks * p.G + g, p.G, p.chunks, g < p.G, a, b, 0.f, 0.f);
   if (g < p.G && (int)threadIdx.x < JOIN_I) {
-    const double inv = 1.0 / ((double)p.HW * p.cg);
+    const double inv = p.inv_count;
     p.gmean[(size_t)n * p.G + g] = make_float2((float)(a * inv), (float)(b * inv));
   }
 }
@@ -419,7 +423,7 @@ template <typename T, int V, int ACTC> __global__ __launch_bounds__(256) void gn
     float mu[V], ga[V], be[V], k0[V], k1[V];      // dx = (rs gamma) du + k0 + k1 c with c = x - mean
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-      const int c = col * V + e, g = c / p.cg;
+      const int c = col * V + e, g = group_of(p, c);
       const float rs = st[2 * g + 1];
       mu[e] = st[2 * g];
       ga[e] = rs * (p.gamma ? p.gamma[c] : 1.f);
@@ -476,10 +480,10 @@ DEVINL int xcd_contiguous(int id, int n) {      // hardware deals workgroup ids 
 }
 
 // lanes that share the reduction of one of n items: a power of two, whole waves at most
-DEVINL int res_lanes(int n, int nt) {
-  int l = 64;
-  while (l > 1 && l * n > nt) l >>= 1;
-  return l;
+DEVINL int res_shift(int n, int nt) {
+  int s = 6;
+  while (s > 0 && (n << s) > nt) --s;
+  return s;
 }
 
 template <typename T, int V, int NV, int ACTC, int NT> __global__ __launch_bounds__(NT) void gn_res_fwd_kernel(const ResP q) {
@@ -497,6 +501,23 @@ template <typename T, int V, int NV, int ACTC, int NT> __global__ __launch_bound
     const int r = row + i * q.rpb;
     if (on && r < p.HW) raw[i] = Lane<T, V>::get(px + (size_t)r * p.x_ld);
   }
+  float o[V], ga[V], be[V];       // what else comes from memory is requested before anything waits
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    const int c = c0 + col * V + e;
+    o[e] = gn_origin<T>(p, n, group_of(p, c));
+    ga[e] = p.gamma ? p.gamma[c] : 1.f;
+    be[e] = p.beta ? p.beta[c] : 0.f;
+  }
+  const T* pr = p.res ? (const T*)p.res + ((size_t)n * p.HW + row) * p.r_ld + c0 + (size_t)col * V : nullptr;
+  constexpr int NR = NV <= 4 ? NV : 1;     // (few rows: the shortcut's as well)
+  typename Lane<T, V>::raw rres[NR];
+  if (NV <= 4 && pr)
+#pragma unroll
+    for (int i = 0; i < NR; ++i) {
+      const int r = row + i * q.rpb;
+      if (on && r < p.HW) rres[i] = Lane<T, V>::get(pr + (size_t)i * q.rpb * p.r_ld);
+    }
   const int per = p.HW / q.rpb, extra = p.HW % q.rpb;      // rows of a row lane: per, one more in the first `extra` lanes
   const int cnt = on ? per + (row < extra ? 1 : 0) : 0;
   {
@@ -519,18 +540,18 @@ template <typename T, int V, int NV, int ACTC, int NT> __global__ __launch_bound
     if (cnt > 0) {
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        const float o = gn_origin<T>(p, n, (c0 + col * V + e) / p.cg), v = m2[e] - s[e] * s[e] * inv;
-        red[e * NT + tid] = make_float2((k[e] - o) + s[e] * inv, v < 0.f ? 0.f : v);
+        const float v = m2[e] - s[e] * s[e] * inv;
+        red[e * NT + tid] = make_float2((k[e] - o[e]) + s[e] * inv, v < 0.f ? 0.f : v);
       }
     }
   }
   __syncthreads();
-  // row lanes -> channels (a channel's partials are res_lanes(nch, NT) lanes' work, about V each) -> groups
+  // row lanes -> channels (a channel's partials are 2^res_shift(nch, NT) lanes' work, about V each) -> groups
   const int nch = q.sv * V, nrow = min(q.rpb, p.HW);
   {
-    const int L = res_lanes(nch, NT), lane = tid % L;
-    for (int k = 0; k < nch; k += NT / L) {
-      const int c = k + tid / L;
+    const int sh = res_shift(nch, NT), L = 1 << sh, lane = tid & (L - 1);
+    for (int k = 0; k < nch; k += NT >> sh) {
+      const int c = k + (tid >> sh);
       const bool live = c < nch;
       const float2* e = red + (live ? (c % V) * NT + c / V : 0);
       float mean = 0.f, m2 = 0.f;
@@ -550,9 +571,9 @@ template <typename T, int V, int NV, int ACTC, int NT> __global__ __launch_bound
   __syncthreads();
   const int gs = nch / p.cg;
   {
-    const int L = res_lanes(gs, NT), lane = tid % L;
-    for (int k = 0; k < gs; k += NT / L) {
-      const int g = k + tid / L;
+    const int sh = res_shift(gs, NT), L = 1 << sh, lane = tid & (L - 1);
+    for (int k = 0; k < gs; k += NT >> sh) {
+      const int g = k + (tid >> sh);
       const bool live = g < gs;
       float mean = 0.f, m2 = 0.f;
       if (live)
@@ -567,7 +588,7 @@ template <typename T, int V, int NV, int ACTC, int NT> __global__ __launch_bound
       if (live && lane == 0) {
         const int gg = c0 / p.cg + g;
         const float mu = (float)((double)mean + (double)gn_origin<T>(p, n, gg));
-        const float rs = (float)(1.0 / sqrt((double)m2 / ((double)p.HW * p.cg) + (double)p.eps));
+        const float rs = (float)rsqrt((double)m2 * p.inv_count + (double)p.eps);
         gm[2 * g] = mu;
         gm[2 * g + 1] = rs;
         p.stats[((size_t)n * p.G + gg) * 2] = mu;
@@ -577,26 +598,25 @@ template <typename T, int V, int NV, int ACTC, int NT> __global__ __launch_bound
   }
   __syncthreads();
   if (cnt == 0) return;
-  float mu[V], a[V], b[V];
+  float mu[V], a[V];
 #pragma unroll
   for (int e = 0; e < V; ++e) {
-    const int c = c0 + col * V + e, g = (col * V + e) / p.cg;
+    const int g = group_of(p, col * V + e);
     mu[e] = gm[2 * g];
-    a[e] = gm[2 * g + 1] * (p.gamma ? p.gamma[c] : 1.f);
-    b[e] = p.beta ? p.beta[c] : 0.f;
+    a[e] = gm[2 * g + 1] * ga[e];
   }
   const size_t row0 = (size_t)n * p.HW + row;
-  const T* pr = p.res ? (const T*)p.res + row0 * p.r_ld + c0 + (size_t)col * V : nullptr;
   T* po = (T*)p.out + row0 * p.o_ld + c0 + (size_t)col * V;
 #pragma unroll
   for (int i = 0; i < NV; ++i)
     if (i < cnt) {
       float f[V], t[V];
       Lane<T, V>::cvt(raw[i], f);
-      if (pr) lane_load<T, V>(pr + (size_t)i * q.rpb * p.r_ld, t);
+      if (NV <= 4 && pr) Lane<T, V>::cvt(rres[i < NR ? i : 0], t);
+      else if (pr) lane_load<T, V>(pr + (size_t)i * q.rpb * p.r_ld, t);
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        f[e] = gn_act<Vec<T>::precise>(fmaf(f[e] - mu[e], a[e], b[e]), act);
+        f[e] = gn_act<Vec<T>::precise>(fmaf(f[e] - mu[e], a[e], be[e]), act);
         if (pr) f[e] += t[e];
       }
       Lane<T, V>::store(po + (size_t)i * q.rpb * p.o_ld, f);
@@ -625,7 +645,7 @@ template <typename T, int V, int NV, int ACTC> __global__ __launch_bounds__(RES_
   float mu[V], ga[V], be[V];
 #pragma unroll
   for (int e = 0; e < V; ++e) {
-    const int c = c0 + col * V + e, g = (col * V + e) / p.cg;
+    const int c = c0 + col * V + e, g = group_of(p, col * V + e);
     mu[e] = st[2 * g];
     ga[e] = st[2 * g + 1] * (p.gamma ? p.gamma[c] : 1.f);
     be[e] = p.beta ? p.beta[c] : 0.f;
@@ -655,9 +675,9 @@ template <typename T, int V, int NV, int ACTC> __global__ __launch_bounds__(RES_
   __syncthreads();
   const int nrow = min(q.rpb, p.HW);
   {
-    const int L = res_lanes(nch, RES_NT), lane = tid % L;
-    for (int k = 0; k < nch; k += RES_NT / L) {
-      const int c = k + tid / L;
+    const int sh = res_shift(nch, RES_NT), L = 1 << sh, lane = tid & (L - 1);
+    for (int k = 0; k < nch; k += RES_NT >> sh) {
+      const int c = k + (tid >> sh);
       const bool live = c < nch;
       const float2* e = red + (live ? (c % V) * RES_NT + c / V : 0);
       float a = 0.f, b = 0.f;
@@ -670,7 +690,7 @@ template <typename T, int V, int NV, int ACTC> __global__ __launch_bounds__(RES_
       a = lane_sum(a, L);
       b = lane_sum(b, L);
       if (live && lane == 0) {
-        b *= st[2 * (c / p.cg) + 1];
+        b *= st[2 * group_of(p, c) + 1];
         chan[c] = make_float2(a, b);
         if (p.N > 1) {
           p.cpart[(size_t)n * p.C + c0 + c] = make_float2(a, b);
@@ -684,9 +704,9 @@ template <typename T, int V, int NV, int ACTC> __global__ __launch_bounds__(RES_
   __syncthreads();
   const int gs = nch / p.cg;
   {
-    const int L = res_lanes(gs, RES_NT), lane = tid % L;
-    for (int k = 0; k < gs; k += RES_NT / L) {
-      const int g = k + tid / L;
+    const int sh = res_shift(gs, RES_NT), L = 1 << sh, lane = tid & (L - 1);
+    for (int k = 0; k < gs; k += RES_NT >> sh) {
+      const int g = k + (tid >> sh);
       float a = 0.f, b = 0.f;
       if (g < gs)
         for (int c = g * p.cg + lane; c < (g + 1) * p.cg; c += L) {
@@ -697,7 +717,7 @@ template <typename T, int V, int NV, int ACTC> __global__ __launch_bounds__(RES_
       a = lane_sum(a, L);
       b = lane_sum(b, L);
       if (g < gs && lane == 0) {
-        const double inv = 1.0 / ((double)p.HW * p.cg);
+        const double inv = p.inv_count;
         gmean[g] = make_float2((float)(a * inv), (float)(b * inv));
       }
     }
@@ -707,7 +727,7 @@ template <typename T, int V, int NV, int ACTC> __global__ __launch_bounds__(RES_
   float k0[V], k1[V];
 #pragma unroll
   for (int e = 0; e < V; ++e) {
-    const int g = (col * V + e) / p.cg;
+    const int g = group_of(p, col * V + e);
     const float rs = st[2 * g + 1];
     k0[e] = -rs * gmean[g].x;
     k1[e] = -rs * rs * gmean[g].y;
@@ -770,6 +790,8 @@ GnP gn_params(const plyolo_gn_desc* d, void* ws) {
   GnP p{};
   p.N = d->N; p.HW = d->HW; p.C = d->C; p.G = d->groups; p.cg = d->C / d->groups; p.act = d->act;
   p.x_ld = d->x_ld; p.r_ld = d->r_ld; p.eps = d->eps;
+  p.inv_cg = 1.0f / (float)p.cg;
+  p.inv_count = 1.0 / ((double)p.HW * p.cg);
   gn_chunks(d, &p.chunks, &p.rows);
   p.gpart = (float2*)ws;
   p.cpart = p.gpart + (size_t)p.N * p.chunks * p.G;
