@@ -62,6 +62,7 @@ template <int V> DEVINL void drop_vec(const DropP& p, const Key& key, size_t v, 
 
 constexpr int DROP_U = 2;   // vectors in flight per thread
 
+// HBM's copy rate: 204800 x 128 bf16 with shortcut 30 us, 5.2 TB/s.
 // whole 16-byte vectors; FLAT: no pitch anywhere (one long row, any C), else C is a multiple of V
 template <typename T, bool FLAT> __global__ __launch_bounds__(256) void dropout_kernel(const DropP p) {
   constexpr int V = Vec<T>::N;
@@ -116,7 +117,29 @@ template <typename T, bool FLAT> __global__ __launch_bounds__(256) void dropout_
   }
 }
 
-// any C, pitch and alignment: one thread per counter, its four elements one by one
+// four consecutive elements
+template <typename T> struct Four;
+template <> struct Four<bf16_t> {
+  typedef unsigned type __attribute__((ext_vector_type(2)));
+  static DEVINL void cvt(const type v, float (&f)[4]) {
+    f[0] = __uint_as_float(v.x << 16);
+    f[1] = __uint_as_float(v.x & 0xffff0000u);
+    f[2] = __uint_as_float(v.y << 16);
+    f[3] = __uint_as_float(v.y & 0xffff0000u);
+  }
+  static DEVINL type pack(const float (&f)[4]) { return type{pack2bf(f[0], f[1]), pack2bf(f[2], f[3])}; }
+};
+template <> struct Four<float> {
+  typedef f32x4 type;
+  static DEVINL void cvt(const f32x4 v, float (&f)[4]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) f[e] = v[e];
+  }
+  static DEVINL f32x4 pack(const float (&f)[4]) { return f32x4{f[0], f[1], f[2], f[3]}; }
+};
+
+// any C, pitch and alignment: one thread per counter, one by one where its four elements are of two rows (20000 x 613 bf16 with shortcut, pitch
+// 616: 20 us; every element by itself 28; the same without a pitch, in whole vectors, 14)
 template <typename T> __global__ __launch_bounds__(256) void dropout_any_kernel(const DropP p) {
   const Key key = load_key(p.rng);
   const size_t q = (size_t)blockIdx.x * 256 + threadIdx.x;
@@ -125,6 +148,21 @@ template <typename T> __global__ __launch_bounds__(256) void dropout_any_kernel(
   philox4x32_7((unsigned)q, (unsigned)(q >> 32), key.step, p.site, key.k0, key.k1, w);
   size_t m = p.total <= 0xffffffffu ? (size_t)((unsigned)(q * 4) / (unsigned)p.C) : q * 4 / p.C;
   int c = (int)(q * 4 - m * p.C);
+  if (c + 4 <= p.C) {      // the whole counter in one row: 8 or 16 bytes at any element address
+    typedef typename Four<T>::type __attribute__((aligned(sizeof(T)))) any4;
+    T* o = (T*)p.out + m * p.o_ld + c;
+    float f[4], r[4];
+    Four<T>::cvt(*(const any4*)((const T*)p.x + m * p.x_ld + c), f);
+    if (p.res) Four<T>::cvt(*(const any4*)((const T*)p.res + m * p.r_ld + c), r);
+    else if (p.accumulate) Four<T>::cvt(*(const any4*)o, r);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      f[e] = (w[e] >= p.thr && !p.none) ? f[e] * p.scale : 0.f;
+      if (p.res || p.accumulate) f[e] += r[e];
+    }
+    *(any4*)o = Four<T>::pack(f);
+    return;
+  }
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     if (q * 4 + e < p.total) {

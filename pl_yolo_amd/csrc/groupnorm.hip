@@ -86,11 +86,11 @@ struct GnP {
 // off by 2^-23
 DEVINL int group_of(const GnP& p, int c) { return (int)(((float)c + 0.5f) * p.inv_cg); }
 
-// lanes per group for the joins below: a power of two <= 64 with lanes * G <= 256 where that is possible
-DEVINL int join_lanes(int G) {
-  int l = 64;
-  while (l > 1 && l * G > 256) l >>= 1;
-  return l;
+// 2^lane_shift lanes share the reduction of one of n items: as many as nt threads have for it, a wave at most
+DEVINL int lane_shift(int n, int nt) {
+  int s = 6;
+  while (s > 0 && (n << s) > nt) --s;
+  return s;
 }
 template <typename A> DEVINL A lane_sum(A v, int lanes) {
   for (int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor(v, o);
@@ -98,6 +98,23 @@ template <typename A> DEVINL A lane_sum(A v, int lanes) {
 }
 
 // ------------------------------------------------------------------------------------------------ forward
+// Vector `col` of a row of any C >= V channels (streaming kernels): the last one of a row that V does not divide is the row's last V channels,
+// of which the first `skip` are its neighbour's -- read, never summed or stored.  (Element by element instead: 16 x 6400 x 132 bf16 forward 44,
+// backward 138 us; this way 34 and 47.)
+template <int V> struct Col {
+  int c, skip;
+  DEVINL Col(const GnP& p, int col) : c(min(col * V, p.C - V)), skip(col * V - c) {}
+};
+template <typename T, int V> DEVINL void store_from(T* p, const float (&f)[V], int skip) {
+  if (skip == 0) {
+    Lane<T, V>::store(p, f);
+    return;
+  }
+#pragma unroll
+  for (int e = 1; e < V; ++e)
+    if (e >= skip) ActT<T>::st(p + e, f[e]);
+}
+
 // the value from which the means of (image, group) are counted
 template <typename T> DEVINL float gn_origin(const GnP& p, int n, int g) {
   return ActT<T>::ld((const T*)p.x + (size_t)n * p.HW * p.x_ld + (size_t)g * p.cg);
@@ -109,13 +126,14 @@ template <typename T, int V> __global__ __launch_bounds__(256) void gn_stats_ker
   __shared__ float2 red[256 * V];
   const int n = blockIdx.x / p.chunks, j = blockIdx.x % p.chunks;
   const int r0 = j * p.rows, nr = min(p.HW - r0, p.rows);
-  const int cv = p.C / V, cols = min(cv, 256), rpb = 256 / cols;
+  const int cv = (p.C + V - 1) / V, cols = min(cv, 256), rpb = 256 / cols;
   const int tcol = threadIdx.x % cols, trow = threadIdx.x / cols;
   const T* base = (const T*)p.x + ((size_t)n * p.HW + r0) * p.x_ld;
   for (int cb = 0; cb < cv; cb += cols) {
     const int col = cb + tcol;
     if (col < cv && trow < rpb) {
-      const T* px = base + (size_t)col * V;
+      const Col<V> at(p, col);
+      const T* px = base + at.c;
       float k[V], s[V], q[V], f[V];
 #pragma unroll
       for (int e = 0; e < V; ++e) k[e] = s[e] = q[e] = 0.f;
@@ -136,29 +154,35 @@ template <typename T, int V> __global__ __launch_bounds__(256) void gn_stats_ker
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         const float m2 = q[e] - s[e] * s[e] * inv;
-        const float from = k[e] - gn_origin<T>(p, n, group_of(p, col * V + e));
-        red[(trow * cols + tcol) * V + e] = make_float2(from + s[e] * inv, m2 < 0.f ? 0.f : m2);   // (a NaN passes)
+        const float from = k[e] - gn_origin<T>(p, n, group_of(p, at.c + e));
+        if (e >= at.skip) red[(trow * cols + tcol) * V + e - at.skip] = make_float2(from + s[e] * inv, m2 < 0.f ? 0.f : m2);   // (a NaN passes)
       }
     }
     __syncthreads();
-    const int nch = min(cols, cv - cb) * V, nrow = min(rpb, nr);
-    for (int t = threadIdx.x; t < nch; t += 256) {
+    const int nch = min(cols * V, p.C - cb * V), nrow = min(rpb, nr), per = nr / rpb, extra = nr % rpb;
+    const int sh = lane_shift(nch, 256), L = 1 << sh, lane = threadIdx.x & (L - 1);
+    for (int k = 0; k < nch; k += 256 >> sh) {
+      const int t = k + (threadIdx.x >> sh);
+      const bool live = t < nch;
       float mean = 0.f, m2 = 0.f;
-      for (int w = 0; w < nrow; ++w) mean = fmaf(red[w * cols * V + t].x, (float)((nr - w + rpb - 1) / rpb), mean);
-      mean /= (float)nr;
-      for (int w = 0; w < nrow; ++w) {
-        const float2 o = red[w * cols * V + t];
-        const float d = o.x - mean;
-        m2 += fmaf(d * d, (float)((nr - w + rpb - 1) / rpb), o.y);
-      }
-      chan[(size_t)cb * V + t] = make_float2(mean, m2);
+      if (live)
+        for (int w = lane; w < nrow; w += L) mean = fmaf(red[w * cols * V + t].x, (float)(per + (w < extra ? 1 : 0)), mean);
+      mean = lane_sum(mean, L) / (float)nr;
+      if (live)
+        for (int w = lane; w < nrow; w += L) {
+          const float2 o = red[w * cols * V + t];
+          const float d = o.x - mean;
+          m2 += fmaf(d * d, (float)(per + (w < extra ? 1 : 0)), o.y);
+        }
+      m2 = lane_sum(m2, L);
+      if (live && lane == 0) chan[cb * V + t] = make_float2(mean, m2);
     }
     __syncthreads();
   }
   // channels -> groups: equal counts, so the group's mean is the mean of means
-  const int L = join_lanes(p.G), gl = threadIdx.x % L, gstep = 256 / L;
+  const int sh = lane_shift(p.G, 256), L = 1 << sh, gl = threadIdx.x & (L - 1), gstep = 256 >> sh;
   for (int g0 = 0; g0 < p.G; g0 += gstep) {
-    const int g = g0 + threadIdx.x / L;
+    const int g = g0 + (threadIdx.x >> sh);
     const bool on = g < p.G;
     float sm = 0.f;
     const float first = on ? chan[g * p.cg].x : 0.f;      // the spread of the means about one of them: no digits lost to their size
@@ -237,15 +261,16 @@ template <typename T, int V, int ACTC> __global__ __launch_bounds__(256) void gn
   const int blk = gridDim.x - 1 - blockIdx.x, n = blk / p.chunks, j = blk % p.chunks;
   const int r0 = j * p.rows, nr = min(p.HW - r0, p.rows);
   const int act = ACTC >= 0 ? ACTC : p.act;
-  const int cv = p.C / V, cols = min(cv, 256), rpb = 256 / cols;
+  const int cv = (p.C + V - 1) / V, cols = min(cv, 256), rpb = 256 / cols;
   const int tcol = threadIdx.x % cols, trow = threadIdx.x / cols;
   const size_t row0 = (size_t)n * p.HW + r0;
   typedef typename Lane<T, V>::raw raw_t;
   raw_t rx[GN_U], rr[GN_U];
   const bool rows_mine = trow < rpb;
   auto request = [&](const int col, const int r) {
-    const T* px = (const T*)p.x + row0 * p.x_ld + (size_t)col * V;
-    const T* pr = (const T*)p.res + row0 * p.r_ld + (size_t)col * V;
+    const Col<V> at(p, col);
+    const T* px = (const T*)p.x + row0 * p.x_ld + at.c;
+    const T* pr = (const T*)p.res + row0 * p.r_ld + at.c;
 #pragma unroll
     for (int u = 0; u < GN_U; ++u)
       if (r + u * rpb < nr) {
@@ -257,15 +282,16 @@ template <typename T, int V, int ACTC> __global__ __launch_bounds__(256) void gn
   if (!rows_mine) return;
   const float* st = p.stats + (size_t)n * 2 * p.G;
   for (int col = tcol; col < cv; col += cols) {
+    const Col<V> at(p, col);
     request(col, trow);
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-      const int c = col * V + e, g = group_of(p, c);
+      const int c = at.c + e, g = group_of(p, c);
       mu[e] = st[2 * g];
       a[e] = st[2 * g + 1] * (p.gamma ? p.gamma[c] : 1.f);
       b[e] = p.beta ? p.beta[c] : 0.f;
     }
-    T* po = (T*)p.out + row0 * p.o_ld + (size_t)col * V;
+    T* po = (T*)p.out + row0 * p.o_ld + at.c;
     for (int r = trow; r < nr; r += GN_U * rpb) {
       raw_t cx[GN_U], cr[GN_U];
 #pragma unroll
@@ -285,7 +311,7 @@ template <typename T, int V, int ACTC> __global__ __launch_bounds__(256) void gn
             f[e] = gn_act<Vec<T>::precise>(fmaf(f[e] - mu[e], a[e], b[e]), act);
             if (p.res) f[e] += t[e];
           }
-          Lane<T, V>::store(po + (size_t)(r + u * rpb) * p.o_ld, f);
+          store_from<T, V>(po + (size_t)(r + u * rpb) * p.o_ld, f, at.skip);
         }
     }
   }
@@ -311,7 +337,7 @@ template <typename T, int V, int ACTC> __global__ __launch_bounds__(256) void gn
   const int n = blockIdx.x / p.chunks, j = blockIdx.x % p.chunks;
   const int r0 = j * p.rows, nr = min(p.HW - r0, p.rows);
   const int act = ACTC >= 0 ? ACTC : p.act;
-  const int cv = p.C / V, cols = min(cv, 256), rpb = 256 / cols;
+  const int cv = (p.C + V - 1) / V, cols = min(cv, 256), rpb = 256 / cols;
   const int tcol = threadIdx.x % cols, trow = threadIdx.x / cols;
   const size_t row0 = (size_t)n * p.HW + r0;
   const float* st = p.stats + (size_t)n * 2 * p.G;
@@ -319,18 +345,19 @@ template <typename T, int V, int ACTC> __global__ __launch_bounds__(256) void gn
   for (int cb = 0; cb < cv; cb += cols) {
     const int col = cb + tcol;
     if (col < cv && trow < rpb) {
+      const Col<V> at(p, col);
       float mu[V], rs[V], ga[V], be[V], sa[V], sb[V];
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        const int c = col * V + e, g = group_of(p, c);
+        const int c = at.c + e, g = group_of(p, c);
         mu[e] = st[2 * g];
         rs[e] = st[2 * g + 1];
         ga[e] = rs[e] * (p.gamma ? p.gamma[c] : 1.f);
         be[e] = p.beta ? p.beta[c] : 0.f;
         sa[e] = sb[e] = 0.f;
       }
-      const T* px = (const T*)p.x + row0 * p.x_ld + (size_t)col * V;
-      const T* pd = (const T*)p.dout + row0 * p.d_ld + (size_t)col * V;
+      const T* px = (const T*)p.x + row0 * p.x_ld + at.c;
+      const T* pd = (const T*)p.dout + row0 * p.d_ld + at.c;
       typename Lane<T, V>::raw rx[GN_BU], rd[GN_BU], cx[GN_BU], cd[GN_BU];
       gn_request<T, V>(rx, rd, px, pd, p, trow, nr, rpb);
       for (int r = trow; r < nr; r += GN_BU * rpb) {
@@ -356,26 +383,34 @@ template <typename T, int V, int ACTC> __global__ __launch_bounds__(256) void gn
           }
       }
 #pragma unroll
-      for (int e = 0; e < V; ++e) red[(trow * cols + tcol) * V + e] = make_float2(sa[e], sb[e] * rs[e]);
+      for (int e = 0; e < V; ++e)
+        if (e >= at.skip) red[(trow * cols + tcol) * V + e - at.skip] = make_float2(sa[e], sb[e] * rs[e]);
     }
     __syncthreads();
-    const int nch = min(cols, cv - cb) * V;
-    for (int t = threadIdx.x; t < nch; t += 256) {
+    const int nch = min(cols * V, p.C - cb * V), nrow = min(rpb, nr);
+    const int sh = lane_shift(nch, 256), L = 1 << sh, lane = threadIdx.x & (L - 1);
+    for (int k = 0; k < nch; k += 256 >> sh) {
+      const int t = k + (threadIdx.x >> sh), c = cb * V + t;
+      const bool live = t < nch;
       float a = 0.f, b = 0.f;
-      for (int w = 0; w < rpb && w < nr; ++w) {
-        const float2 o = red[w * cols * V + t];
-        a += o.x;
-        b += o.y;
+      if (live)
+        for (int w = lane; w < nrow; w += L) {
+          const float2 o = red[w * cols * V + t];
+          a += o.x;
+          b += o.y;
+        }
+      a = lane_sum(a, L);
+      b = lane_sum(b, L);
+      if (live && lane == 0) {
+        chan[c] = make_float2(a, b);
+        cp[c] = make_float2(a, b);
       }
-      const int c = cb * V + t;
-      chan[c] = make_float2(a, b);
-      cp[c] = make_float2(a, b);
     }
     __syncthreads();
   }
-  const int L = join_lanes(p.G), gl = threadIdx.x % L, gstep = 256 / L;
+  const int sh = lane_shift(p.G, 256), L = 1 << sh, gl = threadIdx.x & (L - 1), gstep = 256 >> sh;
   for (int g0 = 0; g0 < p.G; g0 += gstep) {
-    const int g = g0 + threadIdx.x / L;
+    const int g = g0 + (threadIdx.x >> sh);
     float a = 0.f, b = 0.f;
     if (g < p.G)
       for (int c = g * p.cg + gl; c < (g + 1) * p.cg; c += L) {
@@ -413,17 +448,18 @@ template <typename T, int V, int ACTC> __global__ __launch_bounds__(256) void gn
   const int act = ACTC >= 0 ? ACTC : p.act;
   const int blk = gridDim.x - 1 - blockIdx.x, n = blk / p.chunks, j = blk % p.chunks;      // last chunk first, as in gn_apply_kernel
   const int r0 = j * p.rows, nr = min(p.HW - r0, p.rows);
-  const int cv = p.C / V, cols = min(cv, 256), rpb = 256 / cols;
+  const int cv = (p.C + V - 1) / V, cols = min(cv, 256), rpb = 256 / cols;
   const int tcol = threadIdx.x % cols, trow = threadIdx.x / cols;
   if (trow >= rpb) return;
   const size_t row0 = (size_t)n * p.HW + r0;
   const float* st = p.stats + (size_t)n * 2 * p.G;
   const float2* gm = p.gmean + (size_t)n * p.G;
   for (int col = tcol; col < cv; col += cols) {
+    const Col<V> at(p, col);
     float mu[V], ga[V], be[V], k0[V], k1[V];      // dx = (rs gamma) du + k0 + k1 c with c = x - mean
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-      const int c = col * V + e, g = group_of(p, c);
+      const int c = at.c + e, g = group_of(p, c);
       const float rs = st[2 * g + 1];
       mu[e] = st[2 * g];
       ga[e] = rs * (p.gamma ? p.gamma[c] : 1.f);
@@ -431,9 +467,9 @@ template <typename T, int V, int ACTC> __global__ __launch_bounds__(256) void gn
       k0[e] = -rs * gm[g].x;
       k1[e] = -rs * rs * gm[g].y;
     }
-    const T* px = (const T*)p.x + row0 * p.x_ld + (size_t)col * V;
-    const T* pd = (const T*)p.dout + row0 * p.d_ld + (size_t)col * V;
-    T* po = (T*)p.out + row0 * p.o_ld + (size_t)col * V;
+    const T* px = (const T*)p.x + row0 * p.x_ld + at.c;
+    const T* pd = (const T*)p.dout + row0 * p.d_ld + at.c;
+    T* po = (T*)p.out + row0 * p.o_ld + at.c;
     typename Lane<T, V>::raw rx[GN_BU], rd[GN_BU], cx[GN_BU], cd[GN_BU];
     gn_request<T, V>(rx, rd, px, pd, p, trow, nr, rpb);
     for (int r = trow; r < nr; r += GN_BU * rpb) {
@@ -457,7 +493,7 @@ template <typename T, int V, int ACTC> __global__ __launch_bounds__(256) void gn
             const float g = fmaf(ga[e], du, fmaf(k1[e], c, k0[e]));
             d[e] = p.acc_dx ? o[e] + g : g;
           }
-          Lane<T, V>::store(po + (size_t)(r + u * rpb) * p.o_ld, d);
+          store_from<T, V>(po + (size_t)(r + u * rpb) * p.o_ld, d, at.skip);
         }
     }
   }
@@ -477,13 +513,6 @@ struct ResP {
 DEVINL int xcd_contiguous(int id, int n) {      // hardware deals workgroup ids round robin over the 8 XCDs: give each a contiguous range
   const int q = n >> 3, r = n & 7, x = id & 7;
   return (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + (id >> 3);
-}
-
-// lanes that share the reduction of one of n items: a power of two, whole waves at most
-DEVINL int res_shift(int n, int nt) {
-  int s = 6;
-  while (s > 0 && (n << s) > nt) --s;
-  return s;
 }
 
 template <typename T, int V, int NV, int ACTC, int NT> __global__ __launch_bounds__(NT) void gn_res_fwd_kernel(const ResP q) {
@@ -546,10 +575,10 @@ template <typename T, int V, int NV, int ACTC, int NT> __global__ __launch_bound
     }
   }
   __syncthreads();
-  // row lanes -> channels (a channel's partials are 2^res_shift(nch, NT) lanes' work, about V each) -> groups
+  // row lanes -> channels (a channel's partials are 2^lane_shift(nch, NT) lanes' work, about V each) -> groups
   const int nch = q.sv * V, nrow = min(q.rpb, p.HW);
   {
-    const int sh = res_shift(nch, NT), L = 1 << sh, lane = tid & (L - 1);
+    const int sh = lane_shift(nch, NT), L = 1 << sh, lane = tid & (L - 1);
     for (int k = 0; k < nch; k += NT >> sh) {
       const int c = k + (tid >> sh);
       const bool live = c < nch;
@@ -571,7 +600,7 @@ template <typename T, int V, int NV, int ACTC, int NT> __global__ __launch_bound
   __syncthreads();
   const int gs = nch / p.cg;
   {
-    const int sh = res_shift(gs, NT), L = 1 << sh, lane = tid & (L - 1);
+    const int sh = lane_shift(gs, NT), L = 1 << sh, lane = tid & (L - 1);
     for (int k = 0; k < gs; k += NT >> sh) {
       const int g = k + (tid >> sh);
       const bool live = g < gs;
@@ -675,7 +704,7 @@ template <typename T, int V, int NV, int ACTC> __global__ __launch_bounds__(RES_
   __syncthreads();
   const int nrow = min(q.rpb, p.HW);
   {
-    const int sh = res_shift(nch, RES_NT), L = 1 << sh, lane = tid & (L - 1);
+    const int sh = lane_shift(nch, RES_NT), L = 1 << sh, lane = tid & (L - 1);
     for (int k = 0; k < nch; k += RES_NT >> sh) {
       const int c = k + (tid >> sh);
       const bool live = c < nch;
@@ -704,7 +733,7 @@ template <typename T, int V, int NV, int ACTC> __global__ __launch_bounds__(RES_
   __syncthreads();
   const int gs = nch / p.cg;
   {
-    const int sh = res_shift(gs, RES_NT), L = 1 << sh, lane = tid & (L - 1);
+    const int sh = lane_shift(gs, RES_NT), L = 1 << sh, lane = tid & (L - 1);
     for (int k = 0; k < gs; k += RES_NT >> sh) {
       const int g = k + (tid >> sh);
       float a = 0.f, b = 0.f;
@@ -753,7 +782,7 @@ template <typename T, int V, int NV, int ACTC> __global__ __launch_bounds__(RES_
 
 // ------------------------------------------------------------------------------------------------ host side
 // Row chunks of one image in the streaming launches.  A function of the descriptor's sizes alone, so that the workspace does not depend on
-// addresses: four workgroups per compute unit over the whole batch (eight: 8 x 6400 x 320 bf16 forward 49 instead of 38 us), and at least 8192
+// addresses: four workgroups per compute unit over the whole batch (eight: 8 x 6400 x 320 bf16 forward 49 instead of 35 us), and at least 8192
 // values per chunk (2048 where that would leave fewer than 128 workgroups).
 void gn_chunks(const plyolo_gn_desc* d, int* chunks, int* rows) {
   const int64_t all = (int64_t)d->N * d->HW;
@@ -802,7 +831,7 @@ GnP gn_params(const plyolo_gn_desc* d, void* ws) {
 // The resident split of the descriptor, or nv = 0 for the streaming launches.  A slice is a multiple of the least run of vectors that holds
 // whole groups; it grows towards 128-byte row pieces as long as the batch still gives every compute unit a workgroup and the rows fit the
 // registers (nv vectors a thread).  Measured, resident / streaming: the forward keeps its lead to the register limit when there are
-// workgroups to fill the chip (32 x 6400 x 128 bf16, nv 25: 41 / 48 us; 32 x 1600 x 256: 20 / 37), one image on a few workgroups loses it
+// workgroups to fill the chip (32 x 6400 x 128 bf16, nv 25: 38 / 48 us; 32 x 1600 x 256: 19 / 37), one image on a few workgroups loses it
 // beyond 12 vectors (1 x 6400 x 128, nv 13: 20 / 15).  The backward holds two operands and has nothing to hide narrow row pieces behind: 16
 // vectors in pieces of 64 bytes and more (32 x 1600 x 256, sv 4: 31 / 44; 16 x 1600 x 640, sv 5: 39 / 51), 8 in narrower ones
 // (32 x 6400 x 128, sv 1, nv 13: 91 / 72) and on few workgroups.
@@ -876,16 +905,16 @@ int plyolo_gn_act_fwd(const plyolo_gn_desc* d, const void* x, const float* gamma
   GnP p = gn_params(d, workspace);
   p.x = x; p.res = res; p.out = out; p.gamma = gamma; p.beta = beta; p.stats = stats; p.o_ld = d->o_ld;
   const int V = d->dtype == PLYOLO_BF16 ? 8 : 4, dtype = d->dtype, act = d->act;
-  const bool wide = d->C % V == 0;
+  const bool wide = d->C >= V, whole = d->C % V == 0;
   plyolo::annotate("gn_act_fwd", 0.0, (double)p.N * p.HW * p.C * es * (res ? 3.0 : 2.0));
-  const ResPlan rp = res_plan(d, wide ? V : 1, false);
+  const ResPlan rp = res_plan(d, whole ? V : 1, false);
   if (rp.nv) {
     ResP q{};
     q.g = p; q.sv = rp.sv; q.slices = rp.slices; q.rpb = rp.rpb;
-    const int nch = rp.sv * (wide ? V : 1);
-    const size_t lds = (size_t)(rp.nt * (wide ? V : 1) + nch + nch / p.cg) * sizeof(float2);
+    const int nch = rp.sv * (whole ? V : 1);
+    const size_t lds = (size_t)(rp.nt * (whole ? V : 1) + nch + nch / p.cg) * sizeof(float2);
     return plyolo::submit(stream, [=](hipStream_t s) -> hipError_t {
-      auto k = GN_RES_DISPATCH(dtype, wide, act, GN_RES_FWD, GN_RES_FWD1, rp.nv);
+      auto k = GN_RES_DISPATCH(dtype, whole, act, GN_RES_FWD, GN_RES_FWD1, rp.nv);
       if (hipError_t e = plyolo::ensure_dynamic_lds((const void*)k, lds); e != hipSuccess) return e;
       hipLaunchKernelGGL(k, dim3((unsigned)p.N * rp.slices), dim3(rp.nt), lds, s, q);
       return hipGetLastError();
@@ -919,16 +948,16 @@ int plyolo_gn_act_bwd(const plyolo_gn_desc* d, const void* dout, int d_ld, const
   p.x = x; p.dout = dout; p.out = dx; p.gamma = gamma; p.beta = beta; p.stats = (float*)stats;
   p.dgamma = dgamma; p.dbeta = dbeta; p.d_ld = d_ld; p.o_ld = dx_ld; p.acc_dx = accumulate_dx ? 1 : 0; p.acc_par = accumulate_params ? 1 : 0;
   const int V = d->dtype == PLYOLO_BF16 ? 8 : 4, dtype = d->dtype, act = d->act;
-  const bool wide = d->C % V == 0;
+  const bool wide = d->C >= V, whole = d->C % V == 0;
   plyolo::annotate("gn_act_bwd", 0.0, (double)p.N * p.HW * p.C * es * (accumulate_dx ? 4.0 : 3.0));
-  const ResPlan rp = res_plan(d, wide ? V : 1, true);
+  const ResPlan rp = res_plan(d, whole ? V : 1, true);
   if (rp.nv) {
     ResP q{};
     q.g = p; q.sv = rp.sv; q.slices = rp.slices; q.rpb = rp.rpb;
-    const int nch = rp.sv * (wide ? V : 1);
+    const int nch = rp.sv * (whole ? V : 1);
     const size_t lds = (size_t)(nch + nch / p.cg) * sizeof(float2);
     return plyolo::submit(stream, [=](hipStream_t s) -> hipError_t {
-      auto k = GN_RES_DISPATCH(dtype, wide, act, GN_RES_BWD, GN_RES_BWD1, rp.nv);
+      auto k = GN_RES_DISPATCH(dtype, whole, act, GN_RES_BWD, GN_RES_BWD1, rp.nv);
       hipLaunchKernelGGL(k, dim3((unsigned)p.N * rp.slices), dim3(RES_NT), lds, s, q);
       if (p.N > 1 && (p.dgamma || p.dbeta)) join_bwd(p, cdiv(p.C, JOIN_I), 0, p.N, s);
       return hipGetLastError();

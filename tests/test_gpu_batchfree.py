@@ -119,6 +119,10 @@ GN_SHAPES = [  # n, hw, c, groups, pad, off
     (1, 130, 4096, 4096, 0, 0),     # as many groups as the largest channel count
     (8, 9000, 64, 32, 0, 0),        # held in registers by 1024 threads
     (13, 1500, 200, 5, 0, 0),       # ... by a slice of five vectors
+    (6, 6400, 132, 12, 0, 0),       # streamed, four channels behind the last bf16 vector
+    (2, 20000, 13, 13, 0, 0),       # ... five (one fp32)
+    (1, 30000, 9, 3, 3, 1),         # ... one, rows at odd addresses
+    (2, 9000, 15, 1, 0, 0),         # ... seven (three fp32)
 ]
 
 
@@ -169,6 +173,27 @@ def test_gn_activations_accumulation_and_in_place(act, dt):
     keep = out.v.clone()
     t.fwd(out=t.x)
     assert torch.equal(t.x.v, keep)
+
+
+@pytest.mark.parametrize("dt", [BF16, F32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("c,groups", [(13, 13), (132, 12), (10, 1)])
+def test_gn_streamed_in_place_with_a_ragged_last_vector(c, groups, dt):
+    """The last vector of a row overlaps its neighbour: in place, what is read there may be new already and must not count."""
+    n, hw = 2, 12000
+    t = Gn(dt, n, hw, c, groups, "gelu")
+    want, st = t.fwd()
+    t.check_fwd(want, st)
+    dout = t.mat(rnd(n * hw, c, 11, 0.1))
+    wdx = t.bwd(dout, st)
+    t.check_bwd(wdx, dout)
+    base = t.mat(rnd(n * hw, c, 12, 0.1))
+    b64 = base.v.double().clone()
+    t.bwd(dout, st, dx=base, acc=1)
+    t.check_bwd(base, dout, base=b64)
+    t.bwd(dout, st, dx=dout)
+    assert torch.equal(dout.v, wdx.v) and dout.untouched()
+    _, st2 = t.fwd(out=t.x)
+    assert torch.equal(t.x.v, want.v) and torch.equal(st, st2) and t.x.untouched()
 
 
 def test_gn_without_affine():
