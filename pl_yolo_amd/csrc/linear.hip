@@ -786,7 +786,7 @@ template <typename T> __global__ __launch_bounds__(256) void linear_dz_kernel(co
 }
 
 // out[e] (+)= sum over S slabs of part[s][e] in a fixed order: 4 E elements x 64 / E slab lanes per workgroup, eight slabs in flight per lane.
-// The weight gradient's workgroups (E = 16 or 4 by its slab count) come first, the bias gradient's (E = 4) behind them: one launch for both.
+// The weight gradient's workgroups (E by its slab count) come first, the bias gradient's (E = 4) behind them: one launch for both.
 struct FoldP {
   const float* part;
   void* out;
@@ -828,12 +828,16 @@ template <int E> DEVINL void fold(const FoldP& q, int block, int accumulate, f32
       }
   }
 }
-constexpr int FOLD_FEW = 64;      // slabs up to which 16 lanes per element do
+// 4 * fold_width elements per workgroup: by slab count, so that the lanes of an element have up to eight slabs each
+// (3 slabs of 1024 x 1024 by sixteen lanes 13 us, by one 5)
+__host__ __device__ __forceinline__ int fold_width(int slabs) { return slabs <= 8 ? 256 : slabs <= 32 ? 64 : slabs <= 64 ? 16 : 4; }
 __global__ __launch_bounds__(256) void linear_fold_kernel(const FoldP w, const FoldP b, const int accumulate) {
   __shared__ f32x4 red[256];
   if ((int)blockIdx.x >= w.blocks) fold<4>(b, blockIdx.x - w.blocks, accumulate, red);
-  else if (w.S > FOLD_FEW) fold<4>(w, blockIdx.x, accumulate, red);
-  else fold<16>(w, blockIdx.x, accumulate, red);
+  else if (fold_width(w.S) == 4) fold<4>(w, blockIdx.x, accumulate, red);
+  else if (fold_width(w.S) == 16) fold<16>(w, blockIdx.x, accumulate, red);
+  else if (fold_width(w.S) == 64) fold<64>(w, blockIdx.x, accumulate, red);
+  else fold<256>(w, blockIdx.x, accumulate, red);
 }
 
 // ------------------------------------------------------------------------------------------------ host side
@@ -855,15 +859,18 @@ int pick_tile(int64_t I, int64_t J, int64_t Kc, bool direct) {
   return 64;
 }
 
-// Tile and slabs of dw: enough row ranges to give every compute unit a workgroup (bf16: three quarters of them, dx's workgroups of the same
-// launch take the rest; 51200 x 256 x 256 backward 62 us, 64 with 256 workgroups, 71 with 128 or 384), as long as the slabs are not more to
-// move than the operands; a layer that does not get there with 128 x 128 tiles takes small ones.
+// Tile and slabs of dw: enough row ranges to give every compute unit a workgroup, as long as the slabs are not more to move than the operands; a
+// layer that does not get there with 128 x 128 tiles takes small ones, and so does one whose output fills half of them (K <= 64, where dx has
+// small tiles too and the two share a launch: 204800 x 64 x 64 bf16 66 -> 52 us; fp32, N <= 64 also: 204800 x 128 x 64 171 -> 156).  bf16: three quarters of the compute units where dx shares the launch
+// (51200 x 256 x 256 backward 62 us, 64 with all of them, 71 with half or one and a half), two workgroups each where dx has its own large tiles
+// (12800 x 2048 x 1024 196 us, 239 at three quarters, 214 at three; 12800 x 1024 x 1024 120, 157, 140).
 void dw_plan(const plyolo_linear_desc* d, int tile, BwdPlan* b) {
   const bool half = d->dtype == PLYOLO_BF16;
   const int64_t tiles = (int64_t)cdiv(d->N, tile) * cdiv(d->K, tile);
   const int steps = cdiv(d->M, half ? BK : FK);
   const double slab = 4.0 * d->N * d->K, operands = (half ? 2.0 : 4.0) * d->M * ((double)d->N + d->K);
-  int64_t s = ((half ? 192 : 256) + tiles - 1) / tiles;
+  const int want = !half ? 256 : pick_tile(d->M, d->K, d->N, true) > 128 ? 512 : 192;
+  int64_t s = (want + tiles - 1) / tiles;
   if (s > operands / slab) s = (int64_t)(operands / slab);
   if (s > steps) s = steps;
   if (s < 1) s = 1;
@@ -884,7 +891,8 @@ BwdPlan bwd_plan(const plyolo_linear_desc* d) {
   b.part_bytes = up16((size_t)b.dzblk * d->N * 4);
   b.slab_off = b.part_off + b.part_bytes;
   dw_plan(d, 128, &b);
-  if ((int64_t)b.S * cdiv(d->N, 128) * cdiv(d->K, 128) < 128) dw_plan(d, 64, &b);
+  const bool thin = d->K <= 64 || (!half && d->N <= 64);
+  if (thin || (int64_t)b.S * cdiv(d->N, 128) * cdiv(d->K, 128) < 128) dw_plan(d, 64, &b);
   b.slab_bytes = up16((size_t)b.S * d->N * d->K * 4);
   b.total = b.slab_off + b.slab_bytes;
   return b;
@@ -1072,7 +1080,7 @@ int plyolo_linear_bwd(const plyolo_linear_desc* d, const void* dy, const void* z
   FoldP fw{}, fb{};
   if (dw) {
     fw.part = (const float*)(ws + b.slab_off); fw.out = dw; fw.elems = (size_t)d->N * d->K; fw.S = b.S; fw.f32 = dw_dtype == PLYOLO_F32;
-    fw.blocks = (int)cdivz(fw.elems, fw.S > FOLD_FEW ? 16 : 64);
+    fw.blocks = (int)cdivz(fw.elems, 4 * fold_width(fw.S));
   }
   if (db) {
     fb.part = q.part; fb.out = db; fb.elems = (size_t)d->N; fb.S = b.dzblk; fb.f32 = 1;
