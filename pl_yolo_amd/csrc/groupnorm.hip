@@ -101,9 +101,10 @@ template <typename A> DEVINL A lane_sum(A v, int lanes) {
 // Vector `col` of a row of any C >= V channels (streaming kernels): the last one of a row that V does not divide is the row's last V channels,
 // of which the first `skip` are its neighbour's -- read, never summed or stored.  (Element by element instead: 16 x 6400 x 132 bf16 forward 44,
 // backward 138 us; this way 34 and 47.)
-template <int V> struct Col {
+// RAG: there is such a vector (8 x 25600 x 320 backward 153 us with the test for it, 151 without).
+template <int V, bool RAG> struct Col {
   int c, skip;
-  DEVINL Col(const GnP& p, int col) : c(min(col * V, p.C - V)), skip(col * V - c) {}
+  DEVINL Col(const GnP& p, int col) : c(RAG ? min(col * V, p.C - V) : col * V), skip(RAG ? col * V - c : 0) {}
 };
 template <typename T, int V> DEVINL void store_from(T* p, const float (&f)[V], int skip) {
   if (skip == 0) {
@@ -120,8 +121,8 @@ template <typename T> DEVINL float gn_origin(const GnP& p, int n, int g) {
   return ActT<T>::ld((const T*)p.x + (size_t)n * p.HW * p.x_ld + (size_t)g * p.cg);
 }
 
-// (mean - origin, M2) of every group over the rows of one chunk
-template <typename T, int V> __global__ __launch_bounds__(256) void gn_stats_kernel(const GnP p) {
+// (mean - origin, M2) of every group over the rows of one chunk: one read of x, a thread's deviations are taken from its own first value
+template <typename T, int V, bool RAG> __global__ __launch_bounds__(256) void gn_stats_kernel(const GnP p) {
   extern __shared__ float2 chan[];             // [C] (mean - origin, M2) of one channel over the chunk
   __shared__ float2 red[256 * V];
   const int n = blockIdx.x / p.chunks, j = blockIdx.x % p.chunks;
@@ -132,7 +133,7 @@ template <typename T, int V> __global__ __launch_bounds__(256) void gn_stats_ker
   for (int cb = 0; cb < cv; cb += cols) {
     const int col = cb + tcol;
     if (col < cv && trow < rpb) {
-      const Col<V> at(p, col);
+      const Col<V, RAG> at(p, col);
       const T* px = base + at.c;
       float k[V], s[V], q[V], f[V];
 #pragma unroll
@@ -256,7 +257,9 @@ template <typename T, int JOIN_NT> __global__ __launch_bounds__(JOIN_NT) void gn
 
 constexpr int GN_U = 4;    // rows a thread has in flight
 
-template <typename T, int V, int ACTC> __global__ __launch_bounds__(256) void gn_apply_kernel(const GnP p) {
+// the stream of the forward: GN_U rows requested ahead of the GN_U being formed (statistics, join and this: 32 x 6400 x 256 bf16 78 us, 2.7 TB/s
+// counting x once)
+template <typename T, int V, int ACTC, bool RAG> __global__ __launch_bounds__(256) void gn_apply_kernel(const GnP p) {
   // last chunk first: what the statistics read last is still in the last-level cache
   const int blk = gridDim.x - 1 - blockIdx.x, n = blk / p.chunks, j = blk % p.chunks;
   const int r0 = j * p.rows, nr = min(p.HW - r0, p.rows);
@@ -268,7 +271,7 @@ template <typename T, int V, int ACTC> __global__ __launch_bounds__(256) void gn
   raw_t rx[GN_U], rr[GN_U];
   const bool rows_mine = trow < rpb;
   auto request = [&](const int col, const int r) {
-    const Col<V> at(p, col);
+    const Col<V, RAG> at(p, col);
     const T* px = (const T*)p.x + row0 * p.x_ld + at.c;
     const T* pr = (const T*)p.res + row0 * p.r_ld + at.c;
 #pragma unroll
@@ -282,7 +285,7 @@ template <typename T, int V, int ACTC> __global__ __launch_bounds__(256) void gn
   if (!rows_mine) return;
   const float* st = p.stats + (size_t)n * 2 * p.G;
   for (int col = tcol; col < cv; col += cols) {
-    const Col<V> at(p, col);
+    const Col<V, RAG> at(p, col);
     request(col, trow);
 #pragma unroll
     for (int e = 0; e < V; ++e) {
@@ -330,8 +333,8 @@ DEVINL void gn_request(typename Lane<T, V>::raw (&rx)[GN_BU], typename Lane<T, V
     }
 }
 
-// per chunk: (sum du, sum du xh) of every channel, and (sum v, sum v xh) of every group
-template <typename T, int V, int ACTC> __global__ __launch_bounds__(256) void gn_bwd_sums_kernel(const GnP p) {
+// per chunk: (sum du, sum du xh) of every channel, and (sum v, sum v xh) of every group.  HBM: 8 x 25600 x 320 bf16 54 us, 4.8 TB/s of reads
+template <typename T, int V, int ACTC, bool RAG> __global__ __launch_bounds__(256) void gn_bwd_sums_kernel(const GnP p) {
   extern __shared__ float2 chan[];
   __shared__ float2 red[256 * V];
   const int n = blockIdx.x / p.chunks, j = blockIdx.x % p.chunks;
@@ -345,7 +348,7 @@ template <typename T, int V, int ACTC> __global__ __launch_bounds__(256) void gn
   for (int cb = 0; cb < cv; cb += cols) {
     const int col = cb + tcol;
     if (col < cv && trow < rpb) {
-      const Col<V> at(p, col);
+      const Col<V, RAG> at(p, col);
       float mu[V], rs[V], ga[V], be[V], sa[V], sb[V];
 #pragma unroll
       for (int e = 0; e < V; ++e) {
@@ -444,7 +447,8 @@ template <int JOIN_NT> __global__ __launch_bounds__(JOIN_NT) void gn_join_bwd_ke
   }
 }
 
-template <typename T, int V, int ACTC> __global__ __launch_bounds__(256) void gn_bwd_dx_kernel(const GnP p) {
+// the stream of the backward.  HBM: 8 x 25600 x 320 bf16 66 us, 6.0 TB/s (part of what the sums read last is still in the last-level cache)
+template <typename T, int V, int ACTC, bool RAG> __global__ __launch_bounds__(256) void gn_bwd_dx_kernel(const GnP p) {
   const int act = ACTC >= 0 ? ACTC : p.act;
   const int blk = gridDim.x - 1 - blockIdx.x, n = blk / p.chunks, j = blk % p.chunks;      // last chunk first, as in gn_apply_kernel
   const int r0 = j * p.rows, nr = min(p.HW - r0, p.rows);
@@ -455,7 +459,7 @@ template <typename T, int V, int ACTC> __global__ __launch_bounds__(256) void gn
   const float* st = p.stats + (size_t)n * 2 * p.G;
   const float2* gm = p.gmean + (size_t)n * p.G;
   for (int col = tcol; col < cv; col += cols) {
-    const Col<V> at(p, col);
+    const Col<V, RAG> at(p, col);
     float mu[V], ga[V], be[V], k0[V], k1[V];      // dx = (rs gamma) du + k0 + k1 c with c = x - mean
 #pragma unroll
     for (int e = 0; e < V; ++e) {
@@ -515,6 +519,8 @@ DEVINL int xcd_contiguous(int id, int n) {      // hardware deals workgroup ids 
   return (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + (id >> 3);
 }
 
+// The chip reads, reduces and writes one after the other: 32 x 6400 x 128 bf16 31 us for 105 MB (23 for its reads and writes alone); on one
+// 400 x 256 image it is a chain of latencies, 6.7 us.
 template <typename T, int V, int NV, int ACTC, int NT> __global__ __launch_bounds__(NT) void gn_res_fwd_kernel(const ResP q) {
   const GnP& p = q.g;
   extern __shared__ float2 red[];              // [channel of the vector][thread]: (mean, M2) of the thread's values
@@ -652,6 +658,7 @@ template <typename T, int V, int NV, int ACTC, int NT> __global__ __launch_bound
     }
 }
 
+// x and dout held across the reduction: 32 x 1600 x 256 bf16 31 us for 79 MB
 template <typename T, int V, int NV, int ACTC> __global__ __launch_bounds__(RES_NT) void gn_res_bwd_kernel(const ResP q) {
   const GnP& p = q.g;
   __shared__ float2 red[V * RES_NT];           // (sum du, sum du c) of the thread's rows, then [channel] totals
@@ -875,10 +882,13 @@ ResPlan res_plan(const plyolo_gn_desc* d, int V, bool bwd) {
 #define GN_RES_FWD1(T) gn_res_fwd_kernel<T, 1, 16, -1, RES_NT>
 #define GN_RES_BWD1(T) gn_res_bwd_kernel<T, 1, 16, -1>
 
-#define GN_DISPATCH(dtype, wide, act, KERN)                                                                                     \
-  ((dtype) == PLYOLO_BF16 ? ((wide) ? ((act) == PLYOLO_ACT_SILU ? KERN<bf16_t, 8, PLYOLO_ACT_SILU> : KERN<bf16_t, 8, -1>)         \
-                                    : KERN<bf16_t, 1, -1>)                                                                      \
-                          : ((wide) ? KERN<float, 4, -1> : KERN<float, 1, -1>))
+// rows of whole vectors, rows with a cut last vector, rows of fewer channels than a vector
+#define GN_DISPATCH(dtype, whole, wide, act, KERN)                                                                                       \
+  ((dtype) == PLYOLO_BF16                                                                                                                 \
+       ? ((whole)  ? ((act) == PLYOLO_ACT_SILU ? KERN<bf16_t, 8, PLYOLO_ACT_SILU, false> : KERN<bf16_t, 8, -1, false>)                      \
+          : (wide) ? ((act) == PLYOLO_ACT_SILU ? KERN<bf16_t, 8, PLYOLO_ACT_SILU, true> : KERN<bf16_t, 8, -1, true>)                        \
+                   : KERN<bf16_t, 1, -1, false>)                                                                                          \
+       : ((whole) ? KERN<float, 4, -1, false> : (wide) ? KERN<float, 4, -1, true> : KERN<float, 1, -1, false>))
 
 void join_bwd(const GnP& p, int npar, int nmean, int parts, hipStream_t s) {
   if (parts <= JOIN_FEW) hipLaunchKernelGGL(gn_join_bwd_kernel<256>, dim3((unsigned)(npar + nmean)), dim3(256), 0, s, p, npar, parts);
@@ -921,8 +931,9 @@ int plyolo_gn_act_fwd(const plyolo_gn_desc* d, const void* x, const float* gamma
     });
   }
   return plyolo::submit(stream, [=](hipStream_t s) -> hipError_t {
-    auto ks = dtype == PLYOLO_BF16 ? (wide ? gn_stats_kernel<bf16_t, 8> : gn_stats_kernel<bf16_t, 1>) : (wide ? gn_stats_kernel<float, 4> : gn_stats_kernel<float, 1>);
-    auto ka = GN_DISPATCH(dtype, wide, act, gn_apply_kernel);
+    auto ks = dtype == PLYOLO_BF16 ? (whole ? gn_stats_kernel<bf16_t, 8, false> : wide ? gn_stats_kernel<bf16_t, 8, true> : gn_stats_kernel<bf16_t, 1, false>)
+                                   : (whole ? gn_stats_kernel<float, 4, false> : wide ? gn_stats_kernel<float, 4, true> : gn_stats_kernel<float, 1, false>);
+    auto ka = GN_DISPATCH(dtype, whole, wide, act, gn_apply_kernel);
     const dim3 grid((unsigned)p.N * p.chunks), blk(256);
     const bool few = p.chunks <= JOIN_FEW;
     auto kj = dtype == PLYOLO_BF16 ? (few ? gn_join_fwd_kernel<bf16_t, 256> : gn_join_fwd_kernel<bf16_t, 1024>)
@@ -964,8 +975,8 @@ int plyolo_gn_act_bwd(const plyolo_gn_desc* d, const void* dout, int d_ld, const
     });
   }
   return plyolo::submit(stream, [=](hipStream_t s) -> hipError_t {
-    auto ks = GN_DISPATCH(dtype, wide, act, gn_bwd_sums_kernel);
-    auto kd = GN_DISPATCH(dtype, wide, act, gn_bwd_dx_kernel);
+    auto ks = GN_DISPATCH(dtype, whole, wide, act, gn_bwd_sums_kernel);
+    auto kd = GN_DISPATCH(dtype, whole, wide, act, gn_bwd_dx_kernel);
     const unsigned nblk = (unsigned)p.N * p.chunks;
     const int npar = (p.dgamma || p.dbeta) ? cdiv(p.C, JOIN_I) : 0;
     hipLaunchKernelGGL(ks, dim3(nblk), dim3(256), (size_t)p.C * sizeof(float2), s, p);
