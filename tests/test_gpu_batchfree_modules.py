@@ -358,6 +358,23 @@ def test_detector_with_group_norm_trains():
     assert copy.deepcopy(m) is not m
 
 
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_yolov7_with_group_norm(dtype):
+    """The other family: every BaseConv takes it, the RepConv blocks keep the BatchNorms their class builds; all parameters get gradients."""
+    with open(os.path.join(ROOT, "configs", "model", "yolov7", "yolov7_test.yaml")) as f:
+        cfg = yaml.safe_load(f)
+    for part in ("backbone", "neck", "head"):
+        cfg[part]["norm"] = "gn"
+    torch.manual_seed(1)
+    m = pl_yolo_amd.build_model(cfg, 3).to(DEV).train()
+    m.compute_dtype = dtype
+    assert any(isinstance(k, nn.GroupNorm) for k in m.modules())
+    imgs, labels = odet.synthetic_batch(2, 64, 3, num_gt=3, max_gt=8, seed=5)
+    m(imgs.to(DEV), labels.to(DEV))["loss"].sum().backward()
+    for n, p in m.named_parameters():
+        assert p.grad is not None and bool(torch.isfinite(p.grad).all()) and float(p.grad.abs().max()) > 0, n
+
+
 def test_linear_in_a_model_counts_its_operations():
     from pl_yolo_amd import graph as G, utils
     from pl_yolo_amd._lib import BF16
