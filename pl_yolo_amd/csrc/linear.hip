@@ -27,7 +27,8 @@ struct LinP {
   const float* bias;   // forward, or NULL
   int I, J, Kc;        // output rows, output columns, contraction length
   int a_ld, b_ld, o_ld, z_ld, r_ld;
-  int act, accumulate, vec4;
+  int act, accumulate;
+  int vec4;            // blocks of the forward, slabs: four columns leave at once
   int nj, tiles;       // column tiles, all tiles of the output
   int ksteps;          // MODE_DW: contraction stages per slab
 };
@@ -1070,7 +1071,6 @@ int plyolo_linear_bwd(const plyolo_linear_desc* d, const void* dy, const void* z
   px.a = g; px.b = w; px.out = dx; px.I = d->M; px.J = d->K;
   px.Kc = d->N;
   px.a_ld = g_ld; px.b_ld = d->w_ld; px.o_ld = dx_ld; px.accumulate = accumulate_dx ? 1 : 0;
-  px.vec4 = dx_ld % 4 == 0 && (size_t)dx % 8 == 0;
   pw.a = g; pw.b = x; pw.out = ws + b.slab_off; pw.I = d->N; pw.J = d->K; pw.Kc = d->M;
   pw.a_ld = g_ld; pw.b_ld = d->x_ld; pw.ksteps = b.ksteps;
   pw.vec4 = d->K % 4 == 0;
