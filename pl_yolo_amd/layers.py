@@ -50,6 +50,8 @@ class HipModule(nn.Module):
     callers that mix these modules with foreign ones, not the hot path.  Modules without an `emit` of that shape (the loss
     plugins: their `(list, labels) -> dict` has no caller outside OneStageD) refuse a direct call loudly."""
 
+    any_channels = False      # the input may have any channel count (convolutions read whole 16-byte channel vectors)
+
     def forward(self, *a, **k):
         if k or not hasattr(self, "emit") or type(self).__name__ in ("YOLOXLoss", "YOLOv7Loss"):
             raise PlyoloError(
@@ -83,6 +85,7 @@ class BaseConv(HipModule):
         self.act = get_activation(act, inplace=True)
         self.stride = stride
         self.drop = float(drop)
+        self.any_channels = self.linear
 
     def emit(self, g, x, residual=None, need_dgrad=True, cin_pad=None):
         if getattr(self, "drop", 0.0) > 0.0 and g.training:
@@ -175,6 +178,8 @@ def emit_pair(g, x, unit_a, unit_b):
 class Dropout(HipModule):
     """nn.Dropout(p) of a feature map: every element on its own, scaled by 1 / (1 - p), in training; the identity in eval mode.  The mask
     is a function of (seed, step, place in the network, element) and is never stored (csrc/dropout.hip); see dropout_state()."""
+
+    any_channels = True
 
     def __init__(self, p=0.5):
         super().__init__()

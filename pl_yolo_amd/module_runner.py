@@ -99,7 +99,7 @@ class ModuleRunner:
             ins.append(a)
         else:
             for (B, C_, H, W) in shapes:
-                if C_ % vec:
+                if C_ % vec and not getattr(m, "any_channels", False):
                     raise PlyoloError("sub-module input needs a channel count that is a multiple of %d in %s (got %d)" % (vec, dtype, C_))
                 ins.append(g.new_act(B, H, W, C_, "in"))
         s.ins = ins
