@@ -568,7 +568,8 @@ int plyolo_dropout_bwd(int dtype, int M, int C, const void* dout, int d_ld, floa
 /* Focus space-to-depth (network_blocks.py:50-65): NCHW fp32 image ->
  * NHWC [N,H/2,W/2,Cp] with channel blocks TL,BL,TR,BR (3 each) then zero pad. */
 int plyolo_focus_s2d(int dtype, const float* img, int N, int H, int W, void* out, int Cp, void* stream);
-/* out[m][0:C] (pitch o_ld) = (accumulate ? out : 0) + in[m][0:C] (pitch i_ld) */
+/* out[m][0:C] (pitch o_ld) = (accumulate ? out : 0) + in[m][0:C] (pitch i_ld); in NULL: zeros.  Any C, pitch and element-aligned
+ * address; rows of whole 16-byte-aligned vectors take the wide path. */
 int plyolo_copy_add(int dtype, int M, int C, const void* in, int i_ld, void* out, int o_ld, int accumulate,
                     void* stream);
 /* nearest x2 upsample (models/necks/pafpn_csp.py:22) fwd, and its bwd (2x2 sum) */

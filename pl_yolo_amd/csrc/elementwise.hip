@@ -58,6 +58,20 @@ __global__ void copy_add_kernel(size_t M, int C, const T* in, int i_ld, T* out, 
   }
 }
 
+// any C, pitch and element address, one element a thread (rows of whole aligned vectors take the kernel above)
+template <typename T>
+__global__ void copy_add_any_kernel(size_t M, int C, const T* in, int i_ld, T* out, int o_ld, int accumulate) {
+  const size_t total = M * C;
+  for (size_t idx = (size_t)blockIdx.x * blockDim.x + threadIdx.x; idx < total; idx += (size_t)gridDim.x * blockDim.x) {
+    const size_t m = total <= 0xffffffffu ? (size_t)((unsigned)idx / (unsigned)C) : idx / C;
+    const int c = (int)(idx - m * C);
+    float a = in ? ActT<T>::ld(in + m * i_ld + c) : 0.f;
+    T* o = out + m * o_ld + c;
+    if (accumulate) a += ActT<T>::ld(o);
+    ActT<T>::st(o, a);
+  }
+}
+
 template <typename T>
 __global__ void upsample2x_fwd_kernel(int N, int H, int W, int C, const T* in, int i_ld, T* out, int o_ld) {
   constexpr int V = Vec<T>::N;
@@ -918,13 +932,18 @@ int plyolo_focus_s2d(int dtype, const float* img, int N, int H, int W, void* out
 }
 
 int plyolo_copy_add(int dtype, int M, int C, const void* in, int i_ld, void* out, int o_ld, int accumulate, void* stream) {
-  plyolo::annotate("copy_add", 0.0, (double)M * C * (dtype == PLYOLO_BF16 ? 2.0 : 4.0) * (accumulate ? 3.0 : 2.0));
+  PLY_CHECK_ARG(dtype == PLYOLO_BF16 || dtype == PLYOLO_F32, "copy_add: bad dtype %d", dtype);
+  PLY_CHECK_ARG(M > 0 && C > 0 && out, "copy_add: non-positive dimension (M %d, C %d) or null out", M, C);
+  PLY_CHECK_ARG((!in || i_ld >= C) && o_ld >= C, "copy_add: a row pitch is smaller than C = %d", C);
+  const size_t es = dtype == PLYOLO_BF16 ? 2 : 4;
+  PLY_CHECK_ARG(((size_t)in | (size_t)out) % es == 0, "copy_add: misaligned operand");
+  plyolo::annotate("copy_add", 0.0, (double)M * C * es * (accumulate ? 3.0 : 2.0));
   const int V = dtype == PLYOLO_BF16 ? 8 : 4;
-  PLY_CHECK_ARG(C % V == 0 && i_ld % V == 0 && o_ld % V == 0, "copy_add: C/ld must be multiples of %d", V);
-  const size_t work = (size_t)M * (C / V);
+  const bool wide = C % V == 0 && (!in || i_ld % V == 0) && o_ld % V == 0 && ((size_t)in | (size_t)out) % 16 == 0;
+  const size_t work = (size_t)M * (wide ? C / V : C);
   return submit(stream, [=](hipStream_t s) -> hipError_t {
-    DISPATCH_T(dtype, hipLaunchKernelGGL(copy_add_kernel<T>, dim3(grid_for(work)), dim3(256), 0, s, (size_t)M, C, (const T*)in, i_ld,
-                                         (T*)out, o_ld, accumulate);)
+    DISPATCH_T(dtype, auto k = wide ? copy_add_kernel<T> : copy_add_any_kernel<T>;
+               hipLaunchKernelGGL(k, dim3(grid_for(work)), dim3(256), 0, s, (size_t)M, C, (const T*)in, i_ld, (T*)out, o_ld, accumulate);)
     return hipGetLastError();
   });
 }

@@ -659,7 +659,6 @@ class Graph:
                     e = c
                     while e < a.C and not flags[e]:
                         e += 1
-                    assert c % self.vec == 0 and (e - c) % self.vec == 0
                     call("plyolo_copy_add", self.dtype, a.M, e - c, None, 0,
                          self.grad_storage(st).data_ptr() + (a.c_off + c) * self.esize, st.ld, 0, None)
                     c = e

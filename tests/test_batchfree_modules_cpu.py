@@ -3,7 +3,8 @@ which calls are refused, and what a session is keyed by."""
 import pytest
 import torch
 
-from pl_yolo_amd.layers import BaseConv, Dropout
+from pl_yolo_amd._lib import PlyoloError, call
+from pl_yolo_amd.layers import BaseConv, Dropout, HipModule
 from pl_yolo_amd.module_runner import ModuleRunner
 
 CPU = torch.device("cpu")
@@ -26,7 +27,37 @@ def test_any_channel_count_enters_a_linear_layer_and_a_dropout(make, cin, cout, 
 
 
 def test_convolutions_keep_their_channel_vectors():
-    from pl_yolo_amd._lib import PlyoloError
     for m in (BaseConv(6, 16, 1, 1), BaseConv(6, 16, 3, 1, norm="gn")):
         with pytest.raises(PlyoloError, match="multiple of 8"):
             trace(m, (1, 6, 4, 4))
+
+
+class Residual(HipModule):
+    """x + unit(x)."""
+
+    any_channels = True
+
+    def __init__(self, unit):
+        super().__init__()
+        self.unit = unit
+
+    def emit(self, g, x):
+        return self.unit.emit(g, x, residual=x)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("make", [lambda: BaseConv(85, 85, 1, 1, bias=True, norm=None), lambda: Dropout(0.5),
+                                  lambda: BaseConv(85, 85, 1, 1, bias=True, norm=None, drop=0.5)])
+def test_a_shortcut_on_rows_of_any_channel_count_records_its_backward(make, dtype):
+    s = trace(Residual(make()), (2, 85, 4, 3), dtype)
+    assert s.bwd is not None and all(s.ins[0].storage.ginit)
+
+
+def copy_add(dt=0, M=4, C=5, src=0x10000, i_ld=5, out=0x10000, o_ld=5):
+    call("plyolo_copy_add", dt, M, C, src, i_ld, out, o_ld, 0, None)
+
+
+@pytest.mark.parametrize("kw", [dict(M=0), dict(C=0), dict(i_ld=4), dict(o_ld=4), dict(out=None), dict(src=0x10001), dict(out=0x10001), dict(dt=5)])
+def test_copy_add_refuses(kw):
+    with pytest.raises(PlyoloError, match="copy_add"):
+        copy_add(**kw)

@@ -7,8 +7,9 @@ import pytest
 import torch
 
 import hiputil as hu
-from batchfree import E32, UNIT, act64, act_grad64, assert_close, keep_mask
-from pl_yolo_amd.layers import BaseConv, Dropout, dropout_state
+from batchfree import E32, UNIT, Mat, act64, act_grad64, assert_close, keep_mask
+from pl_yolo_amd._lib import call
+from pl_yolo_amd.layers import BaseConv, Dropout, HipModule, dropout_state
 
 pytestmark = pytest.mark.gpu
 DEV = hu.DEV
@@ -81,3 +82,71 @@ def test_dropout_of_any_channel_count(c, dtype):
         for got, src, what in ((y.detach(), x, "y"), (xi.grad, r, "dx")):
             want = torch.where(keep, rows(src) / 0.7, torch.zeros((), dtype=torch.float64, device=DEV))
             assert_close(rows(got), want, (8 * E32 + u) * want.abs(), what)
+
+
+# ------------------------------------------------------------------------------------------------ shortcuts and slices on odd rows
+@pytest.mark.parametrize("dt", [0, 1], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("m,c,pad,off,ipad", [(1, 1, 0, 0, 0), (37, 85, 0, 0, 3), (1000, 7, 9, 5, 1), (64, 24, 8, 0, 0), (64, 24, 8, 1, 0), (5, 16, 3, 0, 8), (3, 70001, 0, 0, 0)])
+def test_copy_add_of_any_rows(m, c, pad, off, ipad, dt):
+    src, base = Mat(m, c, dt, ipad, off, rnd((m, c), 36)), rnd((m, c), 37)
+    for data, acc in ((None, 0), (base, 1)):
+        out = Mat(m, c, dt, pad, off, data)
+        want = src.v.float() + (out.v.float() if acc else 0.0)
+        call("plyolo_copy_add", dt, m, c, src.ptr, src.ld, out.ptr, out.ld, acc, hu.stream())
+        assert torch.equal(out.v, want.to(out.v.dtype)) and out.untouched()
+    call("plyolo_copy_add", dt, m, c, None, 0, out.ptr, out.ld, 0, hu.stream())
+    assert not bool(out.v.any()) and out.untouched()
+
+
+class Net(HipModule):
+    """A concatenation of two linear units' outputs with an odd boundary, one part of it read a second time, and a shortcut on odd rows:
+    t = [a(x), b(x)];  out = d(c(t)) + a(x) with dropout in front of the shortcut."""
+
+    any_channels = True
+
+    def __init__(self):
+        super().__init__()
+        self.a = BaseConv(13, 5, 1, 1, bias=True, norm=None, act="silu")
+        self.b = BaseConv(13, 11, 1, 1, bias=True, norm=None, act="gelu")
+        self.c = BaseConv(16, 9, 1, 1, bias=True, norm=None, act="silu")
+        self.d = BaseConv(9, 5, 1, 1, bias=True, norm=None, act=None, drop=0.25)
+
+    def emit(self, g, x):
+        a = self.a.emit(g, x)
+        t = g.concat([a, self.b.emit(g, x)])
+        return self.d.emit(g, self.c.emit(g, t), residual=a)
+
+
+def net64(m, w, x, keep):
+    p = {n: (w[n + ".conv.weight"].flatten(1), w[n + ".conv.bias"]) for n in "abcd"}
+    a = act64(x @ p["a"][0].t() + p["a"][1], "silu")
+    t = torch.cat([a, act64(x @ p["b"][0].t() + p["b"][1], "gelu")], 1)
+    u = act64(t @ p["c"][0].t() + p["c"][1], "silu") @ p["d"][0].t() + p["d"][1]
+    return a + keep * u / 0.75
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_shortcuts_and_concatenations_on_odd_rows(dtype):
+    torch.manual_seed(38)
+    m = Net().to(DEV).train()
+    m.compute_dtype = dtype
+    x, r = rnd((3, 13, 6, 5), 39, dtype), rnd((3, 5, 6, 5), 40, dtype)
+    w = {n: (hu.rnd_bf16(p) if dtype == "bf16" and n.endswith("weight") else p).detach().double().clone().requires_grad_(True) for n, p in m.named_parameters()}
+    seed = dropout_state(m).tolist()[0]
+    # fp32: chains of three layers of at most 90 rows and 16 channels, sums of mixed sign: (90 + 16 * 3 + 3 * 64) half steps, below 2e-5 of
+    # the largest value.  bf16: every stored tensor of the chain (three layers forward, their gradients back) is off by 2^-8 of its own size:
+    # 8 of them between the input and a gradient, 8 * 2^-8 of the largest value
+    tol = 2e-5 if dtype == "fp32" else 8 * UNIT[0]
+    for step in range(2):
+        keep = torch.from_numpy(keep_mask(seed, step, 0, 90, 5, 0.25)).to(DEV)
+        x64 = rows(x).requires_grad_(True)
+        for p in w.values():
+            p.grad = None
+        y = net64(m, w, x64, keep)
+        y.backward(rows(r))
+        xi = x.clone().requires_grad_(True)
+        m.zero_grad()
+        got = m(xi)
+        got.backward(r)
+        for a, b, what in [(rows(got.detach()), y.detach(), "y"), (rows(xi.grad), x64.grad, "dx")] + [(p.grad, w[n].grad, n) for n, p in m.named_parameters()]:
+            assert_close(a, b, tol * float(b.abs().max()), what)
