@@ -1451,6 +1451,16 @@ class BnOnlyOp:
         call("plyolo_copy_add", g.dtype, M, Cc, dz, Cc, g.gptr(x), x.ld, acc, None)
 
 
+def dropout_units(module):
+    """The units of a module tree that may drop (BaseConv, Dropout): `drop_p()` is baked into the launches a trace records, so a session
+    goes by the values (drop_key)."""
+    return [m for m in module.modules() if hasattr(m, "drop_p")]
+
+
+def drop_key(module, units):
+    return tuple(u.drop_p() for u in units) if module.training else ()
+
+
 def rng_state_of(module, device=None):
     """Device tensor (seed, step) of the dropouts of a traced module (layers.dropout_state)."""
     s = module.__dict__.get("_dropout_state")

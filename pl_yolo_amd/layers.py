@@ -62,12 +62,18 @@ class HipModule(nn.Module):
         return module_runner.run(self, *a)
 
 
+def check_probability(p):
+    if not 0.0 <= p <= 1.0:
+        raise ValueError("dropout probability has to be between 0 and 1, but got {}".format(p))
+    return p
+
+
 class BaseConv(HipModule):
     """A Convolution2d -> Normalization -> Activation (network_blocks.py:7-40).
 
     Beyond the reference's argument values: norm="gn" (get_normalization), bias=True on a 1x1 stride-1 unit without normalisation (the
     linear layer of csrc/linear.hip, trainable, any channel counts), and `drop`: dropout of the activated output with this probability
-    in training, in front of the shortcut where the unit has one (csrc/dropout.hip)."""
+    in training, in front of the shortcut where the unit has one (csrc/dropout.hip).  `drop` may be changed between steps."""
 
     def __init__(self, in_channels, out_channels, ksize, stride, padding=None, groups=1, bias=False, norm="bn", act="silu", drop=0.0):
         super().__init__()
@@ -78,8 +84,7 @@ class BaseConv(HipModule):
         if (groups != 1 and not self.depthwise) or (bias and not self.linear) or pad != (ksize - 1) // 2 or ksize not in (1, 3) or stride not in (1, 2):
             raise NotImplementedError("HIP conv supports k in {1,3}, stride in {1,2}, same padding, no bias (except 1x1 stride 1 with norm=None), "
                                       "groups=1 or depthwise 3x3 stride 1")
-        if not 0.0 <= drop <= 1.0:
-            raise ValueError("dropout probability has to be between 0 and 1, but got {}".format(drop))
+        check_probability(drop)
         self.conv = nn.Conv2d(in_channels, out_channels, kernel_size=ksize, stride=stride, padding=pad, groups=groups, bias=bias)
         self.norm = get_normalization(norm, out_channels)
         self.act = get_activation(act, inplace=True)
@@ -87,9 +92,13 @@ class BaseConv(HipModule):
         self.drop = float(drop)
         self.any_channels = self.linear
 
+    def drop_p(self):
+        return getattr(self, "drop", 0.0) if self.training else 0.0
+
     def emit(self, g, x, residual=None, need_dgrad=True, cin_pad=None):
-        if getattr(self, "drop", 0.0) > 0.0 and g.training:
-            return G.DropoutOp(g, self._emit_unit(g, x, None, need_dgrad, cin_pad), self.drop, residual).out
+        p = check_probability(self.drop_p()) if g.training else 0.0
+        if p > 0.0:
+            return G.DropoutOp(g, self._emit_unit(g, x, None, need_dgrad, cin_pad), p, residual).out
         return self._emit_unit(g, x, residual, need_dgrad, cin_pad)
 
     def _emit_unit(self, g, x, residual, need_dgrad, cin_pad):
@@ -176,19 +185,21 @@ def emit_pair(g, x, unit_a, unit_b):
 
 
 class Dropout(HipModule):
-    """nn.Dropout(p) of a feature map: every element on its own, scaled by 1 / (1 - p), in training; the identity in eval mode.  The mask
-    is a function of (seed, step, place in the network, element) and is never stored (csrc/dropout.hip); see dropout_state()."""
+    """nn.Dropout(p) of a feature map: every element on its own, scaled by 1 / (1 - p), in training; the identity in eval mode (its own,
+    or that of the module it is called in).  `p` may be changed between steps.  The mask is a function of (seed, step, place in the
+    network, element) and is never stored (csrc/dropout.hip); see dropout_state()."""
 
     any_channels = True
 
     def __init__(self, p=0.5):
         super().__init__()
-        if not 0.0 <= p <= 1.0:
-            raise ValueError("dropout probability has to be between 0 and 1, but got {}".format(p))
-        self.p = float(p)
+        self.p = float(check_probability(p))
+
+    def drop_p(self):
+        return self.p if self.training else 0.0
 
     def emit(self, g, x, residual=None):
-        p = self.p if g.training else 0.0
+        p = check_probability(self.drop_p()) if g.training else 0.0
         if p == 0.0 and residual is None and not g.top_is(self):
             return x
         return G.DropoutOp(g, x, p, residual).out

@@ -232,9 +232,10 @@ class ModuleRunner:
         # the recorded backward holds the gradient ADDRESS of every parameter that required a gradient at trace time (`grad_ptr_of`,
         # `used_params`): freezing / unfreezing a parameter afterwards is another session
         mask = tuple(p.requires_grad for p in self.m.parameters()) if want_grad else ()
-        key = (tuple(tuple(x.shape) for x in xs), image, in_is_list, dtype, training, want_grad, mask)
+        key = (tuple(tuple(x.shape) for x in xs), image, in_is_list, dtype, training, want_grad, mask, G.drop_key(self.m, G.dropout_units(self.m)))
         s = self.sessions.get(key)
         if s is None:
+            self.sessions = {k: v for k, v in self.sessions.items() if k[-1] in ((), key[-1])}     # a schedule of dropout probabilities does not pile up
             s = self._build([tuple(x.shape) for x in xs], image, in_is_list, dtype, training, want_grad, device)
             s.generation = 0
             self.sessions[key] = s

@@ -96,6 +96,10 @@ class DetectorRunner:
         self.flat = dict(device=device, params=params, offs=offs, w=w, g=gbuf, n=n, n_live=n_live, fbuf=bw, ibuf=iw,
                          off_of={id(p): o for p, o in zip(params, offs)})
         self.sessions = {}
+        self.drop_units = G.dropout_units(model)      # (collected once: walking the module tree would cost every step 0.25 ms of host time)
+
+    def drop_key(self):
+        return G.drop_key(self.model_ref, self.drop_units)
 
     def grad_ptr_of(self, p):
         if p is None or not p.requires_grad:
@@ -111,7 +115,8 @@ class DetectorRunner:
         if not self._adopted_ok(device):
             self.adopt(device)
         # use_l1 is baked into the recorded loss launches: flipping it on a live model (YOLOX's last epochs) traces a new session
-        key = (B, H, W, M, mode, self.dtype, self.model_ref.training, bool(getattr(self.model_ref.loss, "use_l1", False)))
+        # ... and so are the dropout probabilities
+        key = (B, H, W, M, mode, self.dtype, self.model_ref.training, bool(getattr(self.model_ref.loss, "use_l1", False)), self.drop_key())
         s = self.sessions.pop(key, None)
         if s is None:
             before = torch.cuda.memory_allocated(device)

@@ -3,11 +3,17 @@ rows, probabilities that change, several streams.
 
 Tolerances: bf16 stored values are off by half a step, 2^-8 relative (UNIT); the linear unit rounds x and W on their way in (the references
 here start from the rounded ones), z, dz and its outputs once each."""
+import os
+
 import pytest
 import torch
+import yaml
 
 import hiputil as hu
+import pl_yolo_amd
 from batchfree import E32, UNIT, Mat, act64, act_grad64, assert_close, keep_mask
+from conftest import ROOT
+from oracle import detector as odet
 from pl_yolo_amd._lib import call
 from pl_yolo_amd.layers import BaseConv, Dropout, HipModule, dropout_state
 
@@ -150,3 +156,49 @@ def test_shortcuts_and_concatenations_on_odd_rows(dtype):
         got.backward(r)
         for a, b, what in [(rows(got.detach()), y.detach(), "y"), (rows(xi.grad), x64.grad, "dx")] + [(p.grad, w[n].grad, n) for n, p in m.named_parameters()]:
             assert_close(a, b, tol * float(b.abs().max()), what)
+
+
+# ------------------------------------------------------------------------------------------------ probabilities that change
+def test_a_changed_probability_changes_rate_and_scale():
+    """Values between two calls of one shape, as in a schedule: each call follows the value it meets, backward included."""
+    m = Dropout(0.5).train()
+    m.compute_dtype = "fp32"
+    x = torch.ones(2, 64, 32, 32, device=DEV)
+    seed = dropout_state(m).tolist()[0]
+    for step, p in enumerate((0.5, 0.125, 0.0, 0.75, 1.0, 0.5)):
+        m.p = p
+        xi = x.clone().requires_grad_(True)
+        y = m(xi)
+        y.backward(x)
+        keep = torch.from_numpy(keep_mask(seed, step, 0, 2048, 64, p)).to(DEV)
+        want = keep.double() * (1.0 / (1.0 - p) if p < 1.0 else 0.0)
+        assert_close(rows(y.detach()), want, 8 * E32 * want, "y")
+        assert torch.equal(xi.grad, y.detach())
+    m.p = 0.5
+    m.eval()
+    with torch.no_grad():
+        assert torch.equal(m(x), x)
+
+
+def test_a_detector_follows_a_changed_probability():
+    with open(os.path.join(ROOT, "configs", "model", "yolox", "yolox_test.yaml")) as f:
+        cfg = yaml.safe_load(f)
+    torch.manual_seed(41)
+    m = pl_yolo_amd.build_model(cfg, 3).to(DEV).train()
+    m.compute_dtype = "fp32"
+    imgs, labels = odet.synthetic_batch(2, 64, 3, num_gt=3, max_gt=8, seed=6)
+    unit, losses = m.backbone.stage4[2].conv3, []
+
+    def step():
+        m.zero_grad()
+        out = m(imgs.to(DEV), labels.to(DEV))
+        out["loss"].backward()
+        assert all(bool(torch.isfinite(p.grad).all()) for p in m.parameters() if p.grad is not None)
+        losses.append(float(out["loss"].detach()))
+    state = dropout_state(m)
+    for drop, steps in ((0.0, 0), (0.5, 1), (0.0, 1), (0.5, 2)):
+        unit.drop = drop
+        step()
+        assert state.tolist()[1] == steps, (drop, state)
+    # batch statistics by atomics: the same arithmetic repeats to fp32 rounding; half the features dropped is far beyond it
+    assert abs(losses[2] - losses[0]) <= 1e-5 * abs(losses[0]) < abs(losses[1] - losses[0]) and losses[1] != losses[3]
