@@ -10,7 +10,7 @@ import yaml
 from conftest import ROOT
 from pl_yolo_amd import graph as G
 from pl_yolo_amd._lib import PlyoloError, call
-from pl_yolo_amd.layers import BaseConv, Dropout, HipModule
+from pl_yolo_amd.layers import BaseConv, Dropout, HipModule, get_normalization
 from pl_yolo_amd.module_runner import ModuleRunner
 
 CPU = torch.device("cpu")
@@ -139,3 +139,52 @@ def test_probabilities_set_later_are_checked():
     u.drop = float("nan")
     with pytest.raises(ValueError, match="between 0 and 1"):
         trace(u, (1, 16, 4, 4))
+
+
+# ------------------------------------------------------------------------------------------------ where `norm: gn` reaches
+def build(path, norm, **more):
+    import pl_yolo_amd
+    with open(os.path.join(ROOT, "configs", "model", path)) as f:
+        cfg = yaml.safe_load(f)
+    for part in ("backbone", "neck", "head"):
+        cfg[part]["norm"] = norm
+    return pl_yolo_amd.build_model(cfg, 3)
+
+
+def kinds(m, kind):
+    return sorted(n for n, k in m.named_modules() if isinstance(k, kind))
+
+
+YOLOX_FIXED = ["backbone.stage4.1.conv2.norm"] + ["head.stems.%d.norm" % i for i in range(3)]
+V7_FIXED = sorted(["backbone.stage%d.0.conv%d.norm" % (s, k) for s in (2, 3, 4) for k in (1, 2)] + ["backbone.stage4.1.conv2.norm"] +
+                  ["neck.spp.cv%d.norm" % k for k in range(1, 8)] + ["neck.downsample_conv%d.conv%d.norm" % (d, k) for d in (1, 2) for k in (1, 2)])
+
+
+@pytest.mark.parametrize("norm,kind", [("gn", nn.GroupNorm), ("ln", nn.LayerNorm)])
+@pytest.mark.parametrize("path,fixed", [("yolox/yolox_test.yaml", YOLOX_FIXED), ("yolox/yolox_s.yaml", YOLOX_FIXED), ("yolov7/yolov7_test.yaml", V7_FIXED),
+                                        ("yolov7/yolov7.yaml", V7_FIXED)])
+def test_norm_reaches_what_the_reference_forwards_it_to(path, fixed, norm, kind):
+    """These and no other units keep their BatchNorm whatever `norm` is, as the reference's blocks have it: SPP's second conv and the head's
+    stems (network_blocks.py:149, decoupled_head.py:29-31), the 1x1 units of the transitions and the SPP-CSP block (eelan.py:130-131,
+    yolov7_neck.py:153-154, network_blocks.py:158-175)."""
+    m = build(path, norm)
+    assert kinds(m, nn.BatchNorm2d) == fixed
+    assert sorted(fixed + kinds(m, kind)) == kinds(build(path, "bn"), nn.BatchNorm2d) and len(kinds(m, kind)) > 30
+
+
+@pytest.mark.parametrize("path", ["yolox/yolox_test.yaml", "yolov7/yolov7_test.yaml"])
+def test_group_norm_in_the_remaining_units(path):
+    """The documented way to a network without batch statistics."""
+    m = build(path, "gn")
+    for u in m.modules():
+        if isinstance(u, BaseConv) and isinstance(u.norm, nn.BatchNorm2d):
+            u.norm = get_normalization("gn", u.conv.out_channels)
+    assert kinds(m, nn.BatchNorm2d) == [] and not list(m.buffers())
+
+
+def test_repconv_keeps_its_batch_norms():
+    from pl_yolo_amd.necks import YOLOv7NECK, RepConv
+    m = YOLOv7NECK((1, 1, 1, 1), (32, 64, 64), norm="gn", repconv=True)
+    inside = sorted(n for n in kinds(m, nn.BatchNorm2d) if n.split(".")[0] in ("n3", "n4", "n5"))
+    assert len(kinds(m, RepConv)) == 3 and inside == sorted(n for k in ("n3", "n4", "n5") for n in
+                                                            (k + "." + q for q in kinds(getattr(m, k), nn.BatchNorm2d))) and len(inside) >= 6

@@ -15,7 +15,7 @@ from batchfree import E32, UNIT, Mat, act64, act_grad64, assert_close, keep_mask
 from conftest import ROOT
 from oracle import detector as odet
 from pl_yolo_amd._lib import call
-from pl_yolo_amd.layers import BaseConv, Dropout, HipModule, dropout_state
+from pl_yolo_amd.layers import BaseConv, Dropout, HipModule, dropout_state, get_normalization
 
 pytestmark = pytest.mark.gpu
 DEV = hu.DEV
@@ -202,3 +202,41 @@ def test_a_detector_follows_a_changed_probability():
         assert state.tolist()[1] == steps, (drop, state)
     # batch statistics by atomics: the same arithmetic repeats to fp32 rounding; half the features dropped is far beyond it
     assert abs(losses[2] - losses[0]) <= 1e-5 * abs(losses[0]) < abs(losses[1] - losses[0]) and losses[1] != losses[3]
+
+
+# ------------------------------------------------------------------------------------------------ whole detectors with group norm
+def gn_detector(path, dtype, nc=3):
+    with open(os.path.join(ROOT, "configs", "model", path)) as f:
+        cfg = yaml.safe_load(f)
+    for part in ("backbone", "neck", "head"):
+        cfg[part]["norm"] = "gn"
+    torch.manual_seed(42)
+    m = pl_yolo_amd.build_model(cfg, nc)
+    for u in m.modules():      # the units that `norm` does not reach
+        if isinstance(u, BaseConv) and isinstance(u.norm, torch.nn.BatchNorm2d):
+            u.norm = get_normalization("gn", u.conv.out_channels)
+    m = m.to(DEV).train()
+    m.compute_dtype = dtype
+    return m
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("path", ["yolox/yolox_test.yaml", "yolov7/yolov7_test.yaml"])
+def test_a_group_norm_detector_does_not_depend_on_its_batch(path, dtype):
+    """The maps of training and of inference are the same bit for bit, and an image's maps do not depend on the others of its batch: fp32 to
+    rounding (launches of another batch sum in another order; 1e-3 of the largest value is a thousand times that), where batch statistics
+    of these three images move them by their own size."""
+    m = gn_detector(path, dtype)
+    x = rnd((3, 3, 128, 128), 43, scale=50.0)
+    x[1] *= 3.0
+    x[2] += 100.0
+    with torch.no_grad():
+        train = [t.clone() for t in m(x)]
+        m.eval()
+        for a, b in zip(train, m(x)):
+            assert torch.equal(a, b)
+        m.train()
+        if dtype == "fp32":
+            for i in range(3):
+                for a, b in zip(train, m(x[i:i + 1])):
+                    assert hu.relerr(b[0], a[i]) <= 1e-3
