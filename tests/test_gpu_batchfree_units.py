@@ -240,3 +240,28 @@ def test_a_group_norm_detector_does_not_depend_on_its_batch(path, dtype):
             for i in range(3):
                 for a, b in zip(train, m(x[i:i + 1])):
                     assert hu.relerr(b[0], a[i]) <= 1e-3
+
+
+@pytest.mark.parametrize("path", ["yolox/yolox_test.yaml", "yolov7/yolov7_test.yaml"])
+def test_group_norm_detector_steps_repeat_on_any_lanes(path, monkeypatch):
+    """bf16 training steps with group norm everywhere and dropout in two units: loss and every gradient are the same bit for bit on several
+    streams, on one, and again."""
+    imgs, labels = odet.synthetic_batch(2, 96, 3, num_gt=3, max_gt=8, seed=77)
+    runs = []
+    for lanes in ("1", "0", "1"):
+        monkeypatch.setenv("PLYOLO_LANES", lanes)
+        m = gn_detector(path, "bf16")
+        units = [k for k in m.modules() if isinstance(k, BaseConv)]
+        units[5].drop, units[-4].drop = 0.25, 0.5
+        dropout_state(m).copy_(torch.tensor([12345, 0], device=DEV))
+        for _ in range(3):
+            m.zero_grad(set_to_none=True)
+            loss = m(imgs.to(DEV), labels.to(DEV))["loss"]
+            loss.sum().backward()
+            runs.append((lanes, loss.detach().clone(), {n: p.grad.clone() for n, p in m.named_parameters() if p.grad is not None}))
+    assert not torch.equal(runs[0][1], runs[1][1])            # another mask each step
+    for i in range(3, 9):
+        (_, l0, g0), (lanes, l1, g1) = runs[i % 3], runs[i]
+        assert torch.equal(l0, l1), (lanes, i)
+        off = [n for n in g0 if not torch.equal(g0[n], g1[n])]
+        assert set(g0) == set(g1) and len(g0) > 100 and not off, (lanes, i, len(off), off[:8])
