@@ -100,6 +100,7 @@ class Graph:
         self.root = None        # the module that is traced (rng_state_of: the dropouts' seed and step belong to it)
         self.rng, self.n_drop = None, 0     # this graph's copy of (seed, step) during one forward -> backward pair; dropouts so far
         self.post_unpack = []   # ops with work that must follow unpack_wgrads
+        self.param_written = set()      # ids of the linear layers' parameters whose gradient the backward recording has written
         self.plan = None        # the Plan being recorded (ops use it for lanes / events)
         self.cur_lane, self.cur_lane_fwd = 0, None
         self.side_lanes = []    # compute lanes besides lane 0 used by the plan being recorded (record_ops)
@@ -584,6 +585,27 @@ class Graph:
     def top_is(self, module):
         return self.root is module
 
+    def check_shared_params(self):
+        """Before a backward plan is recorded.  A linear layer adds to what an earlier launch of the plan left in its parameters' gradients
+        (LinearOp.bwd); the gradients of group norms and of packed convolutions have one writer each, so a group-norm unit whose
+        parameters appear twice, or a linear layer that shares its weights with a convolution, would lose all contributions but one."""
+        packed, own = {}, {}
+        for _, w, b in self.pack_entries:
+            for p in (w, b):
+                packed[id(p)] = packed.get(id(p), 0) + 1
+        for op in self.ops:
+            if isinstance(op, GnConvUnitOp):
+                for p in op.own_params:
+                    own[id(p)] = own.get(id(p), 0) + 1
+        for op in self.ops:
+            ps = [(p, 0) for p in op.own_params] if isinstance(op, LinearOp) else \
+                [(p, 1) for p in op.own_params + [op.pc.sources[0][0]]] if isinstance(op, GnConvUnitOp) else []
+            for p, most in ps:
+                if self.grad_ptr_of(p) is not None and packed.get(id(p), 0) + own.get(id(p), 0) > most:
+                    raise _lib.PlyoloError("a %s parameter of shape %s is used twice in one network: its gradient has one place, which the second "
+                                           "use would overwrite (freeze it, or give each use parameters of its own)"
+                                           % ("linear layer's" if isinstance(op, LinearOp) else "group-norm unit's", tuple(p.shape)))
+
     def zero_bwd_stats(self):
         call("plyolo_memset_async", self.bstat_arena.data_ptr(), 0, self.bstat_arena.numel() * 8, None)
 
@@ -721,7 +743,9 @@ def op_io(op):
         return [op.src], [op.dst]
     if isinstance(op, ConvPairOp):
         return [op.x], [op.out_a, op.out_b]
-    if isinstance(op, (ConvUnitOp, DwConvUnitOp, BnOnlyOp, LinearOp, DropoutOp)):
+    if isinstance(op, LinearOp):      # (backward: gradients of shared parameters are added to, one launch after the other)
+        return [op.x] + ([op.res] if op.res is not None else []) + [(("param", id(p)), 0, 1) for p in op.own_params], [op.out]
+    if isinstance(op, (ConvUnitOp, DwConvUnitOp, BnOnlyOp, DropoutOp)):
         return [op.x] + ([op.res] if op.res is not None else []), [op.out]
     if isinstance(op, (BicubicUpsampleOp, ActOp, LnWidthOp, UpsampleOp, MaxPool2x2Op)):
         return [op.x], [op.out]
@@ -1570,8 +1594,19 @@ class LinearOp:
         if not (self.need_dgrad or dw or db):
             return
         acc = g.grad_mode(self.x) if self.need_dgrad else 0
-        call("plyolo_linear_bwd", self._desc(), dy, self.z.tensor.data_ptr() if self.z is not None else None, g.aptr(self.x), self.wt.data_ptr(),
-             g.gptr(self.x) if self.need_dgrad else None, self.x.ld, acc, dw, F32, db, 0, self.ws.data_ptr(), self.ws.numel(), None)
+        # a layer that runs twice in one network adds to the gradients that its other use left
+        add_w, add_b = (int(id(p) in g.param_written) for p in (self.w, self.b))
+        g.param_written.update(id(p) for p in self.own_params)
+
+        def launch(dx, dw, db, add):
+            call("plyolo_linear_bwd", self._desc(), dy, self.z.tensor.data_ptr() if self.z is not None else None, g.aptr(self.x), self.wt.data_ptr(),
+                 dx, self.x.ld, acc, dw, F32, db, add, self.ws.data_ptr(), self.ws.numel(), None)
+        dx = g.gptr(self.x) if self.need_dgrad else None
+        if dw and db and add_w != add_b:      # only one of the two is shared
+            launch(dx, dw, None, add_w)
+            launch(None, None, db, add_b)
+        else:
+            launch(dx, dw, db, add_w if dw else add_b)
 
 
 class DropoutOp:

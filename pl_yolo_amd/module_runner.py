@@ -144,6 +144,7 @@ class ModuleRunner:
                 g.grad_storage(st)
                 for i in range(o.c_off, o.c_off + o.C):
                     st.ginit[i] = True
+            g.check_shared_params()
             s.bwd = G.Plan()
             with s.bwd:
                 g.plan = s.bwd

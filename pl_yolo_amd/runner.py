@@ -202,6 +202,7 @@ class DetectorRunner:
         s.bwd = None
         s.used_params = []
         if mode in ("train", "maps_grad"):
+            g.check_shared_params()
             s.bwd = G.Plan()
             with s.bwd:
                 g.plan = s.bwd

@@ -188,3 +188,35 @@ def test_repconv_keeps_its_batch_norms():
     inside = sorted(n for n in kinds(m, nn.BatchNorm2d) if n.split(".")[0] in ("n3", "n4", "n5"))
     assert len(kinds(m, RepConv)) == 3 and inside == sorted(n for k in ("n3", "n4", "n5") for n in
                                                             (k + "." + q for q in kinds(getattr(m, k), nn.BatchNorm2d))) and len(inside) >= 6
+
+
+# ------------------------------------------------------------------------------------------------ one unit used twice
+class Twice(HipModule):
+    def __init__(self, a, b):
+        super().__init__()
+        self.a, self.b = a, b
+
+    def emit(self, g, x):
+        return self.b.emit(g, self.a.emit(g, x))
+
+
+def test_a_group_norm_unit_used_twice_is_refused_in_training():
+    """A convolution's weight gradient has one place, which the second use would overwrite."""
+    a, b = BaseConv(16, 16, 3, 1, norm="gn"), BaseConv(16, 16, 3, 1, norm="gn")
+    assert trace(Twice(a, b), (1, 16, 6, 6)).bwd is not None
+    for other in (a, b):
+        if other is b:
+            b.norm = a.norm                         # the affine pair alone
+        with pytest.raises(PlyoloError, match="used twice"):
+            trace(Twice(a, other), (1, 16, 6, 6))
+        assert trace(Twice(a, other), (1, 16, 6, 6), want_grad=False).bwd is None
+    for p in a.parameters():
+        p.requires_grad_(False)                     # nothing to overwrite
+    assert trace(Twice(a, a), (1, 16, 6, 6)).bwd is not None
+
+
+def test_a_linear_layer_sharing_its_weights_with_a_convolution_is_refused_in_training():
+    a, b = BaseConv(16, 16, 1, 1, bias=True, norm=None), BaseConv(16, 16, 1, 1)
+    b.conv.weight = a.conv.weight
+    with pytest.raises(PlyoloError, match="used twice"):
+        trace(Twice(a, b), (1, 16, 6, 6))

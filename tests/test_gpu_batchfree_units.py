@@ -265,3 +265,54 @@ def test_group_norm_detector_steps_repeat_on_any_lanes(path, monkeypatch):
         assert torch.equal(l0, l1), (lanes, i)
         off = [n for n in g0 if not torch.equal(g0[n], g1[n])]
         assert set(g0) == set(g1) and len(g0) > 100 and not off, (lanes, i, len(off), off[:8])
+
+
+# ------------------------------------------------------------------------------------------------ one unit used twice
+class Twice(HipModule):
+    """a(x) + a(b(x)): the linear unit `a` runs twice in one trace, the second time on a lane of its own, and shares its weights (not its
+    bias) with `c`."""
+
+    any_channels = True
+
+    def __init__(self):
+        super().__init__()
+        self.a = BaseConv(12, 12, 1, 1, bias=True, norm=None, act="silu")
+        self.b = BaseConv(12, 12, 1, 1, bias=True, norm=None, act="gelu")
+        self.c = BaseConv(12, 12, 1, 1, bias=True, norm=None, act=None)
+        self.c.conv.weight = self.a.conv.weight
+
+    def emit(self, g, x):
+        y = self.a.emit(g, x)
+        with g.on_lane(2):
+            t = self.a.emit(g, self.b.emit(g, x))
+        return self.c.emit(g, t, residual=y)
+
+
+@pytest.mark.parametrize("frozen", [None, "weight", "bias"])
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_gradients_of_a_linear_unit_used_twice_add_up(dtype, frozen):
+    torch.manual_seed(44)
+    m = Twice().to(DEV).train()
+    m.compute_dtype = dtype
+    if frozen:
+        getattr(m.a.conv, frozen).requires_grad_(False)
+    x, r = rnd((2, 12, 9, 7), 45, dtype), rnd((2, 12, 9, 7), 46, dtype)
+    w = {n: (hu.rnd_bf16(p) if dtype == "bf16" and n.endswith("weight") else p).detach().double().clone().requires_grad_(True) for n, p in m.named_parameters()}
+    x64 = rows(x).requires_grad_(True)
+
+    def unit(t, n, act):
+        return act64(t @ w[("a" if n == "c" else n) + ".conv.weight"].view(12, 12).t() + w[n + ".conv.bias"], act)
+    y = unit(x64, "a", "silu") + unit(unit(unit(x64, "b", "gelu"), "a", "silu"), "c", "none")
+    y.backward(rows(r))
+    # as for the network above: 2e-5 of the largest value in fp32, eight stored roundings of it in bf16
+    tol = 2e-5 if dtype == "fp32" else 8 * UNIT[0]
+    for _ in range(3):
+        xi = x.clone().requires_grad_(True)
+        m.zero_grad()
+        got = m(xi)
+        got.backward(r)
+        for a, b, what in [(rows(got.detach()), y.detach(), "y"), (rows(xi.grad), x64.grad, "dx")] + \
+                [(p.grad, w[n].grad, n) for n, p in m.named_parameters() if p.requires_grad]:
+            assert_close(a, b, tol * float(b.abs().max()), what)
+    if frozen:
+        assert getattr(m.a.conv, frozen).grad is None
