@@ -204,7 +204,7 @@ template <typename T, int V, bool RAG> __global__ __launch_bounds__(256) void gn
 // Joins: 32 items (groups of an image, or channels) x NT / 32 lanes per workgroup, a lane's partials requested sixteen at a time, lanes added
 // in a fixed order.  fp64: the two sums of a group are then enough, however far its mean lies from the origin.
 constexpr int JOIN_I = 32, JOIN_FEW = 128;      // up to that many partials eight lanes per item do (NT 256; beyond, 32 lanes)
-template <int JOIN_NT> DEVINL void join_sums(const float2* part, int stride, int count, bool live, double& a, double& b, const float full, const float tail) {
+template <int JOIN_NT> DEVINL void join_sums(const float2* part, int stride, int count, bool live, double& a, double& b, const double full, const double tail) {
   __shared__ double da[JOIN_NT], db[JOIN_NT];
   const int lane = threadIdx.x / JOIN_I, last = count - 1;
   a = b = 0.0;
@@ -217,8 +217,8 @@ template <int JOIN_NT> DEVINL void join_sums(const float2* part, int stride, int
       for (int k = 0; k < 16; ++k) {
         const int j = j0 + k * (JOIN_NT / JOIN_I);
         if (j > last) continue;
-        if (full > 0.f) {      // (mean - origin, M2) of `full` values (the last: `tail`) -> sum, sum of squares
-          const double w = j < last ? (double)full : (double)tail;
+        if (full > 0.0) {      // (mean - origin, M2) of `full` values (the last: `tail`; more than a float counts) -> sum, sum of squares
+          const double w = j < last ? full : tail;
           a += w * (double)o[k].x;
           b += (double)o[k].y + w * (double)o[k].x * (double)o[k].x;
         } else {
@@ -245,8 +245,8 @@ template <typename T, int JOIN_NT> __global__ __launch_bounds__(JOIN_NT) void gn
   const int gb = (p.G + JOIN_I - 1) / JOIN_I, n = blockIdx.x / gb, g = (blockIdx.x % gb) * JOIN_I + threadIdx.x % JOIN_I;
   const bool live = g < p.G;
   double s, q;
-  join_sums<JOIN_NT>(p.gpart + (size_t)n * p.chunks * p.G + g, p.G, p.chunks, live, s, q, (float)p.rows * (float)p.cg,
-            (float)(p.HW - (p.chunks - 1) * p.rows) * (float)p.cg);
+  join_sums<JOIN_NT>(p.gpart + (size_t)n * p.chunks * p.G + g, p.G, p.chunks, live, s, q, (double)p.rows * p.cg,
+            (double)(p.HW - (p.chunks - 1) * p.rows) * p.cg);
   if (live && (int)threadIdx.x < JOIN_I) {
     const double total = (double)p.HW * p.cg, mean = s / total, m2 = q - s * mean;
     float* st = p.stats + ((size_t)n * p.G + g) * 2;
@@ -432,7 +432,7 @@ template <int JOIN_NT> __global__ __launch_bounds__(JOIN_NT) void gn_join_bwd_ke
   double a, b;
   if ((int)blockIdx.x < npar) {
     const int c = blockIdx.x * JOIN_I + threadIdx.x % JOIN_I;
-    join_sums<JOIN_NT>(p.cpart + c, p.C, parts, c < p.C, a, b, 0.f, 0.f);
+    join_sums<JOIN_NT>(p.cpart + c, p.C, parts, c < p.C, a, b, 0.0, 0.0);
     if (c < p.C && (int)threadIdx.x < JOIN_I) {
       if (p.dbeta) p.dbeta[c] = (float)(a + (p.acc_par ? (double)p.dbeta[c] : 0.0));
       if (p.dgamma) p.dgamma[c] = (float)(b + (p.acc_par ? (double)p.dgamma[c] : 0.0));
@@ -440,7 +440,7 @@ template <int JOIN_NT> __global__ __launch_bounds__(JOIN_NT) void gn_join_bwd_ke
     return;
   }
   const int blk = blockIdx.x - npar, gb = (p.G + JOIN_I - 1) / JOIN_I, n = blk / gb, g = (blk % gb) * JOIN_I + threadIdx.x % JOIN_I;
-  join_sums<JOIN_NT>(p.gpart + (size_t)n * p.chunks * p.G + g, p.G, p.chunks, g < p.G, a, b, 0.f, 0.f);
+  join_sums<JOIN_NT>(p.gpart + (size_t)n * p.chunks * p.G + g, p.G, p.chunks, g < p.G, a, b, 0.0, 0.0);
   if (g < p.G && (int)threadIdx.x < JOIN_I) {
     const double inv = p.inv_count;
     p.gmean[(size_t)n * p.G + g] = make_float2((float)(a * inv), (float)(b * inv));
@@ -790,12 +790,17 @@ template <typename T, int V, int NV, int ACTC> __global__ __launch_bounds__(RES_
 // ------------------------------------------------------------------------------------------------ host side
 // Row chunks of one image in the streaming launches.  A function of the descriptor's sizes alone, so that the workspace does not depend on
 // addresses: four workgroups per compute unit over the whole batch (eight: 8 x 6400 x 320 bf16 forward 49 instead of 35 us), and at least 8192
-// values per chunk (2048 where that would leave fewer than 128 workgroups).
+// values per chunk (2048 where that would leave fewer than 128 workgroups).  Beyond 2^29 values (bf16) there are more workgroups instead of
+// longer ones: a thread then sums THREAD_ROWS rows in fp32, and a chunk whose first value dwarfs the rest keeps its M2 to THREAD_ROWS^2 half
+// steps at worst (4e-3; with 8208 rows a thread 0.12 was measured).
+constexpr int THREAD_ROWS = 256;
 void gn_chunks(const plyolo_gn_desc* d, int* chunks, int* rows) {
   const int64_t all = (int64_t)d->N * d->HW;
   int64_t r = (all + 1023) / 1024;
   const int64_t values = all * d->C / 128, least = (min(max(values, (int64_t)2048), (int64_t)8192) + d->C - 1) / d->C;
   if (r < least) r = least;
+  const int V = d->dtype == PLYOLO_BF16 ? 8 : 4, cols = min(d->C >= V ? cdiv(d->C, V) : d->C, 256);
+  r = min(r, (int64_t)THREAD_ROWS * (256 / cols));
   if (r > d->HW) r = d->HW;
   *rows = (int)r;
   *chunks = (int)((d->HW + r - 1) / r);

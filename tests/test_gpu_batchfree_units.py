@@ -3,6 +3,7 @@ rows, probabilities that change, several streams.
 
 Tolerances: bf16 stored values are off by half a step, 2^-8 relative (UNIT); the linear unit rounds x and W on their way in (the references
 here start from the rounded ones), z, dz and its outputs once each."""
+import ctypes as C
 import os
 
 import pytest
@@ -11,10 +12,11 @@ import yaml
 
 import hiputil as hu
 import pl_yolo_amd
-from batchfree import E32, UNIT, Mat, act64, act_grad64, assert_close, keep_mask
+from batchfree import ACTS, E32, UNIT, Mat, act64, act_grad64, assert_close, keep_mask
 from conftest import ROOT
 from oracle import detector as odet
-from pl_yolo_amd._lib import call
+from pl_yolo_amd import _lib
+from pl_yolo_amd._lib import BF16, GnDesc, call
 from pl_yolo_amd.layers import BaseConv, Dropout, HipModule, dropout_state, get_normalization
 
 pytestmark = pytest.mark.gpu
@@ -316,3 +318,26 @@ def test_gradients_of_a_linear_unit_used_twice_add_up(dtype, frozen):
             assert_close(a, b, tol * float(b.abs().max()), what)
     if frozen:
         assert getattr(m.a.conv, frozen).grad is None
+
+
+# ------------------------------------------------------------------------------------------------ kernels at the ends of their ranges
+def test_group_norm_of_more_values_than_a_float_counts():
+    """One group of 1.7e10 values.  x is 1 but for its first value, 256: the mean lies 255 away from the origin of the partials, and counts that
+    are off by a rounding of fp32 (one part in 1.7e7) make a variance of 255^2 * 6e-8 = 4e-3 out of the true 255^2 / n = 3.8e-6.  A thread
+    sums 256 squares of 255 in fp32: each addition is off by at most half a step of the sum, 256 * 256 * 2^-24 = 4e-3 of M2 together, half
+    of which reaches rstd (less by eps).  The rest in closed form."""
+    c, hw = 1023, 1024 * 16417
+    x = torch.ones(hw, c, dtype=torch.bfloat16, device=DEV)
+    x[0, 0] = 256.0
+    d = GnDesc()
+    d.dtype, d.N, d.HW, d.C, d.groups, d.act, d.eps, d.x_ld, d.o_ld, d.r_ld = BF16, 1, hw, c, 1, ACTS["none"], 1e-5, c, c, c
+    nws = _lib.lib().plyolo_gn_workspace(C.byref(d))
+    ws, st = torch.empty(nws, dtype=torch.uint8, device=DEV), torch.empty(2, device=DEV)
+    call("plyolo_gn_act_fwd", C.byref(d), x.data_ptr(), None, None, None, x.data_ptr(), st.data_ptr(), ws.data_ptr(), nws, hu.stream())
+    n = float(hw) * c
+    mean, var = 1.0 + 255.0 / n, 255.0 ** 2 / n * (1.0 - 1.0 / n)
+    rstd = (var + 1e-5) ** -0.5
+    assert abs(float(st[0]) - mean) <= 2 * E32 and abs(float(st[1]) - rstd) <= 2e-3 * rstd, (st.tolist(), mean, rstd)
+    assert float(x[0, 0]) == float(torch.tensor(255.0 * float(st[1])).bfloat16())
+    for i in (1, hw // 2, hw - 1):      # (1 - mean) rstd, a rounding away from 0
+        assert float(x[i].float().abs().max()) <= 2 * E32 * rstd
