@@ -509,9 +509,11 @@ int plyolo_lnw_act_bwd(int dtype, int N, int H, int W, int C, const void* dout, 
  *             stats[N][groups][2] = (mean, rstd), fp32, for the backward
  *   backward  from dout, x, stats: dx (written, or added to when accumulate_dx), dgamma / dbeta [C] fp32 (either may be NULL; added to
  *             when accumulate_params).  The shortcut's gradient is dout itself.
- * gamma, beta: fp32 [C], NULL = 1 / 0.  Any C, pitch and element-aligned address; rows of 16-byte-aligned vectors take the wide path.
+ * gamma, beta: fp32 [C], NULL = 1 / 0.  Any C, pitch and element-aligned address; rows of at least one 16-byte vector of channels are read
+ * and written by vectors, whatever their alignment, and rows of whole vectors may stay in registers between the two passes.
  * Statistics and gradient sums are formed in a fixed order (no atomics): results repeat bit for bit.  A NaN or infinity stays inside its
- * (image, group).  No operand may overlap another, except out == x and dx == dout (same pitch).
+ * (image, group), whose outputs become NaN; as everywhere in this library relu is u > 0 ? u : 0, so it turns them into 0, and
+ * slopes that are chosen by comparisons stay finite (act'(NaN): relu 0, lrelu 0.1, hswish 0).  No operand may overlap another, except out == x and dx == dout (same pitch).
  * Workspace: plyolo_gn_workspace(d) bytes, 16-byte aligned, contents need not survive a call; calls that may run at the same time
  * (streams, captured graphs) need one each.  C <= 4096, N*HW and every pitch below 2^31, N * ceil(groups / 32) below 2^22 - 128. */
 typedef struct plyolo_gn_desc {
@@ -534,7 +536,8 @@ int plyolo_gn_act_bwd(const plyolo_gn_desc* d, const void* dout, int d_ld, const
  *             dw_dtype (PLYOLO_F32: the masters' type; or `dtype`);  db[n] = sum dz, fp32.  dx, dw, db may each be NULL; dw and db are
  *             added to when accumulate_params.  The shortcut's gradient is dy itself.
  * PLYOLO_BF16: bf16 operands, fp32 accumulation (MFMA), dz rounded to bf16 once for the two products (db sums it unrounded);
- * PLYOLO_F32: fp32 throughout.  y is formed from the unrounded z.  Any M, N, K >= 1, pitches and element-aligned addresses; operands
+ * PLYOLO_F32: fp32 throughout.  y is formed from the unrounded z.  A NaN or infinity of x reaches its row of y and z, one of w its column
+ * (relu and slopes at NaN as for group norm).  Any M, N, K >= 1, pitches and element-aligned addresses; operands
  * whose rows start on 16-byte boundaries with K and N multiples of 8 (bf16) take the wide path.  dy rows have pitch y_ld.
  * Every sum runs in a fixed order: results repeat bit for bit.  No operand may overlap another.
  * Workspace: plyolo_linear_workspace(d, backward) bytes, 16-byte aligned, one per call that may run at the same time (0 bytes: none

@@ -1,5 +1,6 @@
 """Group norm, linear layer and dropout as modules, without a GPU: what a traced session records (nothing runs: plans are only recorded),
 which calls are refused, and what a session is keyed by."""
+import copy
 import os
 
 import pytest
@@ -220,3 +221,30 @@ def test_a_linear_layer_sharing_its_weights_with_a_convolution_is_refused_in_tra
     b.conv.weight = a.conv.weight
     with pytest.raises(PlyoloError, match="used twice"):
         trace(Twice(a, b), (1, 16, 6, 6))
+
+
+# ------------------------------------------------------------------------------------------------ the dropouts' state
+def test_every_rank_draws_its_own_seed(monkeypatch):
+    dist, seeds = torch.distributed, []
+    for rank in (None, 0, 1, 2, 7):
+        torch.manual_seed(9)
+        if rank is not None:
+            monkeypatch.setattr(dist, "is_initialized", lambda: True)
+            monkeypatch.setattr(dist, "get_rank", lambda: rank)
+        seed, step = G.rng_state_of(Dropout(0.5), CPU).tolist()
+        assert step == 0 and 0 <= seed < 1 << 62
+        seeds.append(seed)
+    assert seeds[0] == seeds[1] and len(set(seeds[1:])) == 4          # rank 0 draws what a single process draws
+
+
+def test_a_copy_of_a_module_has_a_state_of_its_own():
+    m = BaseConv(16, 16, 1, 1, bias=True, norm=None, drop=0.5).train()
+    a = G.rng_state_of(m, CPU)
+    r = m.__dict__["_mrunner"] = ModuleRunner(m)
+    trace(m, (1, 16, 4, 4), runner=r)
+    c = copy.deepcopy(m)
+    b = G.rng_state_of(c, CPU)
+    assert b is not a and b.data_ptr() != a.data_ptr() and b.tolist() == a.tolist()
+    assert c.__dict__.get("_mrunner") is None and c.drop == 0.5
+    b[1] = 5
+    assert a.tolist()[1] == 0 and G.rng_state_of(m, CPU) is a

@@ -16,7 +16,7 @@ from batchfree import ACTS, E32, UNIT, Mat, act64, act_grad64, assert_close, kee
 from conftest import ROOT
 from oracle import detector as odet
 from pl_yolo_amd import _lib
-from pl_yolo_amd._lib import BF16, GnDesc, call
+from pl_yolo_amd._lib import BF16, F32, GnDesc, LinearDesc, call
 from pl_yolo_amd.layers import BaseConv, Dropout, HipModule, dropout_state, get_normalization
 
 pytestmark = pytest.mark.gpu
@@ -341,3 +341,126 @@ def test_group_norm_of_more_values_than_a_float_counts():
     assert float(x[0, 0]) == float(torch.tensor(255.0 * float(st[1])).bfloat16())
     for i in (1, hw // 2, hw - 1):      # (1 - mean) rstd, a rounding away from 0
         assert float(x[i].float().abs().max()) <= 2 * E32 * rstd
+
+
+# ------------------------------------------------------------------------------------------------ NaN and infinity through the linear layer
+LIN_SIZES = [(5, 24, 40), (300, 85, 179), (3300, 136, 264), (8200, 520, 1032)]      # blocks, cut rows, whole rows, the large tiles
+
+
+class Linear:
+    def __init__(self, dt, m, n, k, act):
+        self.dt, self.m, self.n, self.k = dt, m, n, k
+        self.x, self.w = Mat(m, k, dt, data=rnd((m, k), 51)), Mat(n, k, dt, data=rnd((n, k), 52, scale=k ** -0.5))
+        self.b = rnd((n,), 53)
+        d = LinearDesc()
+        d.dtype, d.M, d.N, d.K, d.act, d.x_ld, d.w_ld, d.y_ld, d.z_ld = dt, m, n, k, ACTS[act], k, k, n, n
+        self.d = d
+        self.nws = _lib.lib().plyolo_linear_workspace(C.byref(d), 1)
+        self.ws = torch.empty(self.nws, dtype=torch.uint8, device=DEV)
+
+    def fwd(self):
+        z, y = Mat(self.m, self.n, self.dt), Mat(self.m, self.n, self.dt)
+        call("plyolo_linear_fwd", C.byref(self.d), self.x.ptr, self.w.ptr, self.b.data_ptr(), None, z.ptr, y.ptr, None, 0, hu.stream())
+        return y, z
+
+    def bwd(self, dy, z):
+        dx, dw, db = Mat(self.m, self.k, self.dt), torch.empty(self.n, self.k, device=DEV), torch.empty(self.n, device=DEV)
+        call("plyolo_linear_bwd", C.byref(self.d), dy.ptr, z.ptr if z is not None else None, self.x.ptr, self.w.ptr, dx.ptr, dx.ld, 0, dw.data_ptr(),
+             F32, db.data_ptr(), 0, self.ws.data_ptr(), self.nws, hu.stream())
+        return dx.v, dw, db
+
+
+def only(a, b, rows_hit, cols_hit):
+    """b differs from a nowhere but in these rows and columns, and is not finite anywhere in them."""
+    hit = torch.zeros(a.shape, dtype=torch.bool, device=a.device)
+    hit[rows_hit] = True
+    hit[..., cols_hit] = True
+    return torch.equal(a[~hit], b[~hit]) and not bool(torch.isfinite(b[hit]).any())
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("dt", [0, 1], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("m,n,k", LIN_SIZES)
+def test_linear_keeps_nan_and_infinity_in_their_rows_and_columns(m, n, k, dt, bad):
+    """The last row, output and input column (what a tile's ragged end would spread): x[i] reaches y[i] and dw's column, w[o] reaches y's and
+    z's column and all of dx, dy[i, o] reaches dx[i], dw[o] and db[o]."""
+    t = Linear(dt, m, n, k, "none")
+    t.x.v.copy_(t.x.v.sign() * t.x.v.abs().clamp(min=0.01))        # (no zeros: 0 * infinity would be NaN beside the infinities, both not finite)
+    dy = Mat(m, n, dt, data=rnd((m, n), 54).sign() * rnd((m, n), 54).abs().clamp(min=0.01))
+    (y0, z0), g0 = t.fwd(), t.bwd(dy, None)
+    keep = t.x.v.clone()
+    t.x.v[-1, -1] = bad
+    y1, z1 = t.fwd()
+    dx, dw, db = t.bwd(dy, None)
+    assert only(y0.v, y1.v, [-1], []) and only(z0.v, z1.v, [-1], [])
+    assert torch.equal(dx, g0[0]) and only(g0[1], dw, [], [-1]) and torch.equal(db, g0[2])
+    t.x.v.copy_(keep)
+    keep = t.w.v.clone()
+    t.w.v[-1] = bad
+    y1, z1 = t.fwd()
+    dx, dw, db = t.bwd(dy, None)
+    assert only(y0.v, y1.v, [], [-1]) and only(z0.v, z1.v, [], [-1])
+    assert not bool(torch.isfinite(dx).any()) and torch.equal(dw, g0[1]) and torch.equal(db, g0[2])
+    t.w.v.copy_(keep)
+    dy.v[-1, -1] = bad
+    dx, dw, db = t.bwd(dy, None)
+    assert only(g0[0], dx, [-1], []) and only(g0[1], dw, [-1], []) and only(g0[2], db, [], [-1])
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu", "hswish", "lrelu"])
+@pytest.mark.parametrize("dt", [0, 1], ids=["bf16", "fp32"])
+def test_linear_backward_passes_a_nan_of_z(dt, act):
+    t = Linear(dt, 300, 85, 179, act)
+    dy = Mat(300, 85, dt, data=rnd((300, 85), 55) + 3.0)
+    _, z = t.fwd()
+    g0 = t.bwd(dy, z)
+    dy.v[7, 84] = float("nan")
+    dx, dw, db = t.bwd(dy, z)
+    assert only(g0[0], dx, [7], []) and only(g0[1], dw, [84], []) and only(g0[2], db, [], [84])
+    dy.v[7, 84] = 1.0
+    g0 = t.bwd(dy, z)
+    z.v[7, 84] = float("nan")
+    dx, dw, db = t.bwd(dy, z)
+    if act in ("silu", "gelu"):
+        assert only(g0[0], dx, [7], []) and only(g0[1], dw, [84], []) and only(g0[2], db, [], [84])
+    else:       # slopes that are chosen by comparisons: a NaN is not above zero (0.1), nor inside (-3, 3) (0)
+        assert all(bool(torch.isfinite(v).all()) for v in (dx, dw, db))
+
+
+def test_relu_clears_nan():
+    """The package's relu is u > 0 ? u : 0, in the new operators too: a NaN leaves as 0 (and has slope 0)."""
+    t = Linear(1, 20, 8, 16, "relu")
+    t.x.v[3] = float("nan")
+    y, z = t.fwd()
+    assert bool(torch.isnan(z.v[3]).all()) and bool((y.v[3] == 0).all())
+    x = rnd((2 * 50, 16), 56)
+    x[60, 3] = float("nan")
+    d = GnDesc()
+    d.dtype, d.N, d.HW, d.C, d.groups, d.act, d.eps, d.x_ld, d.o_ld, d.r_ld = F32, 2, 50, 16, 4, ACTS["relu"], 1e-5, 16, 16, 16
+    nws = _lib.lib().plyolo_gn_workspace(C.byref(d))
+    ws, st, out = torch.empty(nws, dtype=torch.uint8, device=DEV), torch.empty(2, 4, 2, device=DEV), torch.empty(100, 16, device=DEV)
+    call("plyolo_gn_act_fwd", C.byref(d), x.data_ptr(), None, None, None, out.data_ptr(), st.data_ptr(), ws.data_ptr(), nws, hu.stream())
+    assert bool(torch.isnan(st[1, 0, 1])) and bool((out[50:, :4] == 0).all()) and bool(torch.isfinite(out).all())
+
+
+# ------------------------------------------------------------------------------------------------ the rounding of dz
+@pytest.mark.parametrize("m,n,k", [(1, 300, 600), (2, 85, 179), (333, 85, 179), (12900, 264, 248), (11600, 520, 1288)])
+def test_linear_backward_rounds_dz_once_and_nothing_else(m, n, k):
+    """bf16: the products are those of dz rounded to bf16, with fp32 sums: dw in fp32 and db are within the sums' error of that form (db: of
+    the unrounded dz), and dx within it before its own rounding.  What the products lose against an unrounded dz is that one rounding."""
+    t = Linear(0, m, n, k, "silu")
+    dy = Mat(m, n, 0, data=rnd((m, n), 57, scale=0.1))
+    _, z = t.fwd()
+    dx, dw, db = t.bwd(dy, z)
+    u = z.v.double()
+    s = 1.0 / (1.0 + torch.exp(-u))
+    exact = dy.v.double() * (s * (1.0 + u * (1.0 - s)))
+    # the kernel's dz before its rounding is off by 64 E32 |dy| (1 + |z|): a value that close to a border may round to its other side
+    edge = 64 * E32 * dy.v.double().abs() * (1.0 + u.abs())
+    dz = exact.to(torch.bfloat16).double()
+    step = (exact + edge).to(torch.bfloat16).double() - (exact - edge).to(torch.bfloat16).double()
+    w, x = t.w.v.double(), t.x.v.double()
+    assert_close(dw, dz.t() @ x, step.t() @ x.abs() + (min(m, 4096) + 64) * E32 * (dz.abs().t() @ x.abs()) + 1e-30, "dw")
+    want, tol = dz @ w, step @ w.abs() + (n + 4) * E32 * (dz.abs() @ w.abs())
+    assert_close(dx, want, tol + UNIT[0] * (want.abs() + tol) + 1e-30, "dx")
+    assert_close(db, exact.sum(0), edge.sum(0) + 1100 * E32 * exact.abs().sum(0) + 1e-30, "db")
