@@ -215,7 +215,9 @@ class ModuleRunner:
     @staticmethod
     def _act_to_nchw(a, t):
         st = a.storage
-        return t.view(st.rows, st.ld)[:, a.c_off:a.c_off + a.C].float().view(a.N, a.H, a.W, a.C).permute(0, 3, 1, 2).contiguous()
+        # always a copy: a map of one pixel or one channel is contiguous either way, and .contiguous() would hand out the plan's own buffer
+        out = torch.empty(a.N, a.C, a.H, a.W, dtype=torch.float32, device=t.device)
+        return out.copy_(t.view(st.rows, st.ld)[:, a.c_off:a.c_off + a.C].unflatten(0, (a.N, a.H, a.W)).permute(0, 3, 1, 2))
 
     def _outputs(self, s):
         if s.head is not None:
@@ -223,7 +225,7 @@ class ModuleRunner:
             outs = []
             for (h, w), r0 in zip(hd.sizes, hd.lvl_row):
                 blk = hd.raw[r0 * hd.nch:(r0 + B * h * w) * hd.nch].view(B, h, w, hd.nch)
-                outs.append(blk.permute(0, 3, 1, 2).contiguous())
+                outs.append(blk.permute(0, 3, 1, 2).clone(memory_format=torch.contiguous_format))
             return outs
         return [self._act_to_nchw(o, o.storage.tensor) for o in s.outs]
 

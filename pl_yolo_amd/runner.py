@@ -367,7 +367,7 @@ class DetectorRunner:
         outs = []
         for (h, w), r0 in zip(hd.sizes, hd.lvl_row):
             blk = hd.raw[r0 * hd.nch:(r0 + B * h * w) * hd.nch].view(B, h, w, hd.nch)
-            outs.append(blk.permute(0, 3, 1, 2).contiguous())  # API edge: NCHW like the reference
+            outs.append(blk.permute(0, 3, 1, 2).clone(memory_format=torch.contiguous_format))  # API edge: NCHW like the reference (a copy, also of one pixel)
         return (s, outs) if want_grad else outs
 
     def backward_maps(self, s, grads):

@@ -464,3 +464,44 @@ def test_linear_backward_rounds_dz_once_and_nothing_else(m, n, k):
     want, tol = dz @ w, step @ w.abs() + (n + 4) * E32 * (dz.abs() @ w.abs())
     assert_close(dx, want, tol + UNIT[0] * (want.abs() + tol) + 1e-30, "dx")
     assert_close(db, exact.sum(0), edge.sum(0) + 1100 * E32 * exact.abs().sum(0) + 1e-30, "db")
+
+
+# ------------------------------------------------------------------------------------------------ what a call returned stays what it was
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("make,c,hw", [(lambda: BaseConv(16, 32, 1, 1, bias=True, norm=None), 16, (1, 1)), (lambda: BaseConv(16, 1, 1, 1, bias=True, norm=None), 16, (3, 4)),
+                                       (lambda: BaseConv(1, 8, 1, 1, bias=True, norm=None), 1, (3, 4)), (lambda: Dropout(0.5), 8, (1, 1)),
+                                       (lambda: BaseConv(16, 32, 1, 1, norm="gn"), 16, (1, 1))])
+def test_outputs_and_gradients_of_a_call_outlive_the_next(make, c, hw, dtype):
+    """Maps of one pixel or one channel lie in memory alike channels first and last: what is returned must be a copy all the same."""
+    m = make().to(DEV).train()
+    m.compute_dtype = dtype
+    held = []
+    for i in range(3):
+        x = rnd((4, c) + hw, 60 + i).requires_grad_(True)
+        y = m(x)
+        y.backward(rnd(tuple(y.shape), 70 + i))
+        held.append((y.detach(), y.detach().clone(), x.grad, x.grad.clone()))
+    m.eval()
+    with torch.no_grad():
+        for i in range(2):
+            y = m(rnd((4, c) + hw, 80 + i))
+            held.append((y, y.clone(), y, y))
+    for y, y_then, dx, dx_then in held:
+        assert torch.equal(y, y_then) and torch.equal(dx, dx_then)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_maps_of_one_pixel_outlive_the_next_call(dtype):
+    with open(os.path.join(ROOT, "configs", "model", "yolox", "yolox_test.yaml")) as f:
+        m = pl_yolo_amd.build_model(yaml.safe_load(f), 3).to(DEV).eval()
+    m.compute_dtype = dtype
+    with torch.no_grad():
+        maps = m(rnd((2, 3, 32, 32), 90, scale=50.0))
+        then = [t.clone() for t in maps]
+        feats = [rnd((2, 32, 4, 4), 91), rnd((2, 64, 2, 2), 92), rnd((2, 128, 1, 1), 93)]
+        own = m.head(feats)
+        own_then = [t.clone() for t in own]
+        m(rnd((2, 3, 32, 32), 94, scale=50.0))
+        m.head([2.0 * t for t in feats])
+    assert tuple(maps[2].shape[2:]) == (1, 1)
+    assert all(torch.equal(a, b) for a, b in zip(maps + own, then + own_then))
