@@ -89,7 +89,8 @@ def _map_grads(hd, dtypes):
     out = []
     for (h, w), r0, dt in zip(hd.sizes, hd.lvl_row, dtypes):
         n = hd.B * h * w
-        out.append(drawv[r0:r0 + n].view(hd.B, h, w, hd.nch).permute(0, 3, 1, 2).to(dt).contiguous())
+        grad = torch.empty(hd.B, hd.nch, h, w, dtype=dt, device=drawv.device)      # (always a copy: a map of one pixel is contiguous either way)
+        out.append(grad.copy_(drawv[r0:r0 + n].view(hd.B, h, w, hd.nch).permute(0, 3, 1, 2)))
     return out
 
 

@@ -505,3 +505,18 @@ def test_maps_of_one_pixel_outlive_the_next_call(dtype):
         m.head([2.0 * t for t in feats])
     assert tuple(maps[2].shape[2:]) == (1, 1)
     assert all(torch.equal(a, b) for a, b in zip(maps + own, then + own_then))
+
+
+def test_map_gradients_of_one_pixel_outlive_the_next_loss():
+    with open(os.path.join(ROOT, "configs", "model", "yolox", "yolox_test.yaml")) as f:
+        loss = pl_yolo_amd.build_model(yaml.safe_load(f), 3).to(DEV).train().loss
+    labels = torch.zeros(2, 3, 5, device=DEV)
+    labels[:, 0] = torch.tensor([1.0, 16.0, 16.0, 12.0, 10.0], device=DEV)
+
+    def grads(seed):
+        maps = [1.0 * rnd((2, 8, n, n), seed + n).requires_grad_(True) for n in (4, 2, 1)]
+        return torch.autograd.grad(loss(list(maps), labels)["loss"], maps)
+    first = grads(95)
+    then = [g.clone() for g in first]
+    second = grads(105)
+    assert all(torch.equal(a, b) for a, b in zip(first, then)) and not torch.equal(first[2], second[2])
