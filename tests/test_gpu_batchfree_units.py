@@ -8,6 +8,7 @@ import os
 
 import pytest
 import torch
+import torch.nn.functional as F
 import yaml
 
 import hiputil as hu
@@ -520,3 +521,55 @@ def test_map_gradients_of_one_pixel_outlive_the_next_loss():
     then = [g.clone() for g in first]
     second = grads(105)
     assert all(torch.equal(a, b) for a, b in zip(first, then)) and not torch.equal(first[2], second[2])
+
+
+# ------------------------------------------------------------------------------------------------ beside BatchNorm units
+class Mixed(HipModule):
+    """A BatchNorm unit whose output is read by a linear unit (with it as the shortcut), a group-norm unit and a second BatchNorm unit, their
+    sum behind dropout read by a third: every kind of unit is the last to write some BatchNorm unit's gradient."""
+
+    def __init__(self, order):
+        super().__init__()
+        self.a, self.e = BaseConv(16, 32, 3, 1), BaseConv(32, 16, 3, 1)
+        self.lin, self.gn, self.c = BaseConv(32, 32, 1, 1, bias=True, norm=None), BaseConv(32, 32, 3, 1, norm="gn"), BaseConv(32, 32, 1, 1)
+        self.drop, self.order = Dropout(0.25), order
+
+    def emit(self, g, x):
+        t = self.a.emit(g, x)
+        out = {}
+        for k in self.order:
+            out[k] = {"lin": lambda: self.lin.emit(g, t, residual=t), "gn": lambda: self.gn.emit(g, t), "c": lambda: self.c.emit(g, t)}[k]()
+        return self.e.emit(g, self.drop.emit(g, self.drop.emit(g, out["lin"], residual=out["gn"]), residual=out["c"]))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("order", [("lin", "gn", "c"), ("c", "lin", "gn"), ("gn", "c", "lin")])
+def test_units_beside_batch_norm_units(order, dtype):
+    torch.manual_seed(47)
+    m = Mixed(order).to(DEV).train()
+    m.compute_dtype = dtype
+    n, h, w = 4, 24, 20
+    x, r = rnd((n, 16, h, w), 48, dtype), rnd((n, 16, h, w), 49, dtype)
+    p = {k: (hu.rnd_bf16(v) if dtype == "bf16" and k.endswith("conv.weight") else v).detach().double().clone().requires_grad_(True) for k, v in m.named_parameters()}
+    seed = dropout_state(m).tolist()[0]
+    keep = [torch.from_numpy(keep_mask(seed, 0, s, n * h * w, 32, 0.25)).to(DEV).view(n, h, w, 32).permute(0, 3, 1, 2) / 0.75 for s in (0, 1)]
+
+    def bn(t, k):
+        z = F.conv2d(t, p[k + ".conv.weight"], None, 1, p[k + ".conv.weight"].shape[-1] // 2)
+        return act64(F.batch_norm(z, None, None, p[k + ".norm.weight"], p[k + ".norm.bias"], True, 0.0, 1e-3), "silu")
+    x64 = x.double().requires_grad_(True)
+    t = bn(x64, "a")
+    lin = act64(F.conv2d(t, p["lin.conv.weight"], p["lin.conv.bias"]), "silu") + t
+    gn = act64(F.group_norm(F.conv2d(t, p["gn.conv.weight"], None, 1, 1), 32, p["gn.norm.weight"], p["gn.norm.bias"], 1e-5), "silu")
+    y = bn(keep[1] * (keep[0] * lin + gn) + bn(t, "c"), "e")
+    (y * r.double()).sum().backward()
+    xi = x.clone().requires_grad_(True)
+    got = m(xi)
+    (got * r).sum().backward()
+    # the bounds of the single units (test_gpu_batchfree_modules.TOL), of the largest value: a lost or doubled contribution is of its order
+    f, b = ((2e-2, 6e-2), (2e-5, 5e-4))[TYPES[dtype]]
+    assert hu.relerr(got, y) <= 2 * f and hu.relerr(xi.grad, x64.grad) <= b
+    for k, v in m.named_parameters():
+        e = hu.relerr(v.grad, p[k].grad)
+        print(k, e)
+        assert e <= b, k
