@@ -15,6 +15,9 @@
 // The variance is never formed as E[x^2] - E[x]^2: a thread sums deviations from its own first value, (count, mean, M2) triples are joined
 // by Chan's formula, and the means of the triples are kept as distances from the first value of their (image, group): neither a mean of
 // thousands of spreads nor one huge value costs digits.
+//
+// Times in this file are of whole calls in a captured graph that goes over three sets of operands in turn (more than the last-level cache
+// holds comes from HBM); "cached": over one set.  Times of single kernels are the profiler's, over three sets as well.
 #include "common.h"
 
 namespace {
@@ -100,8 +103,8 @@ template <typename A> DEVINL A lane_sum(A v, int lanes) {
 // ------------------------------------------------------------------------------------------------ forward
 // Vector `col` of a row of any C >= V channels (streaming kernels): the last one of a row that V does not divide is the row's last V channels,
 // of which the first `skip` are its neighbour's -- read, never summed or stored.  (Element by element instead: 16 x 6400 x 132 bf16 forward 44,
-// backward 138 us; this way 34 and 47.)
-// RAG: there is such a vector (8 x 25600 x 320 backward 153 us with the test for it, 151 without).
+// backward 138 us; this way 33 and 46.)
+// RAG: there is such a vector (8 x 25600 x 320 backward 149 us with the test for it, 146 without; cached 127 and 124).
 template <int V, bool RAG> struct Col {
   int c, skip;
   DEVINL Col(const GnP& p, int col) : c(RAG ? min(col * V, p.C - V) : col * V), skip(RAG ? col * V - c : 0) {}
@@ -257,7 +260,7 @@ template <typename T, int JOIN_NT> __global__ __launch_bounds__(JOIN_NT) void gn
 
 constexpr int GN_U = 4;    // rows a thread has in flight
 
-// the stream of the forward: GN_U rows requested ahead of the GN_U being formed (statistics, join and this: 32 x 6400 x 256 bf16 78 us, 2.7 TB/s
+// the stream of the forward: GN_U rows requested ahead of the GN_U being formed (statistics, join and this: 32 x 6400 x 256 bf16 75 us, 2.8 TB/s
 // counting x once)
 template <typename T, int V, int ACTC, bool RAG> __global__ __launch_bounds__(256) void gn_apply_kernel(const GnP p) {
   // last chunk first: what the statistics read last is still in the last-level cache
@@ -333,7 +336,8 @@ DEVINL void gn_request(typename Lane<T, V>::raw (&rx)[GN_BU], typename Lane<T, V
     }
 }
 
-// per chunk: (sum du, sum du xh) of every channel, and (sum v, sum v xh) of every group.  HBM: 8 x 25600 x 320 bf16 54 us, 4.8 TB/s of reads
+// per chunk: (sum du, sum du xh) of every channel, and (sum v, sum v xh) of every group.  Reads: 8 x 25600 x 320 bf16 74 us, 3.5 TB/s
+// from HBM (cached 54 us); every byte of x and dout is fetched once
 template <typename T, int V, int ACTC, bool RAG> __global__ __launch_bounds__(256) void gn_bwd_sums_kernel(const GnP p) {
   extern __shared__ float2 chan[];
   __shared__ float2 red[256 * V];
@@ -447,7 +451,7 @@ template <int JOIN_NT> __global__ __launch_bounds__(JOIN_NT) void gn_join_bwd_ke
   }
 }
 
-// the stream of the backward.  HBM: 8 x 25600 x 320 bf16 66 us, 6.0 TB/s (part of what the sums read last is still in the last-level cache)
+// the stream of the backward.  HBM: 8 x 25600 x 320 bf16 67 us, 5.9 TB/s (part of what the sums read last is still in the last-level cache)
 template <typename T, int V, int ACTC, bool RAG> __global__ __launch_bounds__(256) void gn_bwd_dx_kernel(const GnP p) {
   const int act = ACTC >= 0 ? ACTC : p.act;
   const int blk = gridDim.x - 1 - blockIdx.x, n = blk / p.chunks, j = blk % p.chunks;      // last chunk first, as in gn_apply_kernel
@@ -519,8 +523,8 @@ DEVINL int xcd_contiguous(int id, int n) {      // hardware deals workgroup ids 
   return (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + (id >> 3);
 }
 
-// The chip reads, reduces and writes one after the other: 32 x 6400 x 128 bf16 31 us for 105 MB (23 for its reads and writes alone); on one
-// 400 x 256 image it is a chain of latencies, 6.7 us.
+// The chip reads, reduces and writes one after the other: 32 x 6400 x 128 bf16 38 us for 105 MB, cached 29;
+// on one 400 x 256 image it is a chain of latencies, 6.4 us.
 template <typename T, int V, int NV, int ACTC, int NT> __global__ __launch_bounds__(NT) void gn_res_fwd_kernel(const ResP q) {
   const GnP& p = q.g;
   extern __shared__ float2 red[];              // [channel of the vector][thread]: (mean, M2) of the thread's values
@@ -658,7 +662,7 @@ template <typename T, int V, int NV, int ACTC, int NT> __global__ __launch_bound
     }
 }
 
-// x and dout held across the reduction: 32 x 1600 x 256 bf16 31 us for 79 MB
+// x and dout held across the reduction: 32 x 1600 x 256 bf16 29 us for 79 MB
 template <typename T, int V, int NV, int ACTC> __global__ __launch_bounds__(RES_NT) void gn_res_bwd_kernel(const ResP q) {
   const GnP& p = q.g;
   __shared__ float2 red[V * RES_NT];           // (sum du, sum du c) of the thread's rows, then [channel] totals
@@ -843,10 +847,11 @@ GnP gn_params(const plyolo_gn_desc* d, void* ws) {
 // The resident split of the descriptor, or nv = 0 for the streaming launches.  A slice is a multiple of the least run of vectors that holds
 // whole groups; it grows towards 128-byte row pieces as long as the batch still gives every compute unit a workgroup and the rows fit the
 // registers (nv vectors a thread).  Measured, resident / streaming: the forward keeps its lead to the register limit when there are
-// workgroups to fill the chip (32 x 6400 x 128 bf16, nv 25: 38 / 48 us; 32 x 1600 x 256: 19 / 37), one image on a few workgroups loses it
-// beyond 12 vectors (1 x 6400 x 128, nv 13: 20 / 15).  The backward holds two operands and has nothing to hide narrow row pieces behind: 16
-// vectors in pieces of 64 bytes and more (32 x 1600 x 256, sv 4: 31 / 44; 16 x 1600 x 640, sv 5: 39 / 51), 8 in narrower ones
-// (32 x 6400 x 128, sv 1, nv 13: 91 / 72) and on few workgroups.
+// workgroups to fill the chip (32 x 6400 x 128 bf16, 25 vectors in a 512-thread workgroup and so 13 in the 1024-thread one that is launched:
+// 38 / 42 us, cached 29 / 41; 32 x 1600 x 256: 18.5 / 32), one image on a few workgroups loses it beyond 12 vectors (1 x 6400 x 128, 13: 15.1
+// / 14.7).  The backward holds two operands and has nothing to hide narrow row pieces behind: 16 vectors in pieces of 64 bytes and more
+// (32 x 1600 x 256, sv 4: 29 / 42; 16 x 1600 x 640, sv 5: 40 / 49), 8 in narrower ones (32 x 6400 x 128, sv 1, nv 13: 90 / 68) and on few
+// workgroups.
 struct ResPlan { int sv, slices, rpb, nv, nt; };
 ResPlan res_plan(const plyolo_gn_desc* d, int V, bool bwd) {
   ResPlan r{};

@@ -12,6 +12,10 @@
 //
 // dw contracts over the rows of the batch: the rows are split over workgroups, every range leaves a private fp32 slab and the slabs are
 // added in a fixed order.
+//
+// Times in this file are of whole calls in a captured graph that goes over three sets of operands in turn (more than the last-level cache
+// holds comes from HBM), sizes M x K x N, forwards with z; "cached": over one set.  The profiler times kernels one by one, which
+// can come out above their share of a stream (12800 x 2048 x 1024 78 us).
 #include "common.h"
 
 namespace {
@@ -335,7 +339,7 @@ template <int WI, int WJ> DEVINL void slab_out(const LinP& p, int slab, int i0, 
 }
 
 // Any size, pitch and alignment: TI x TJ tile, four waves of TI / 2 x TJ / 2, operands through registers into two LDS images, one barrier per
-// stage: stage s + 1 is requested behind the barrier of stage s and lands under its MFMAs.  12800 x 2047 x 1023 with z 132 us, 405 TFLOP/s.
+// stage: stage s + 1 is requested behind the barrier of stage s and lands under its MFMAs.  12800 x 2047 x 1023 126 us, 427 TFLOP/s.
 template <int MODE, int TI, int TJ, bool HEAVY> DEVINL void any_tile(const LinP& p, int block, int blocks) {
   constexpr bool ARC = MODE == MODE_DW, BRC = MODE != MODE_FWD;
   typedef Tile<ARC, TI, BK, 256, false> TA;
@@ -389,7 +393,8 @@ template <int MODE, int TI, int TJ, bool HEAVY> DEVINL void any_tile(const LinP&
 
 // Aligned operands: NWI x NWJ waves of WI x WJ, ST LDS images of K contraction elements filled by direct loads, ST - 1 stages in flight: a
 // stage's wait leaves the younger stages' loads outstanding.  One barrier per stage: behind it the image that was read in the stage before is
-// free for the youngest request.  12800 x 2048 x 1024 with z 62 us, 860 TFLOP/s: the MFMAs of one round of tiles (48), then 52 MB of stores.
+// free for the youngest request.  12800 x 2048 x 1024 64 us, 840 TFLOP/s (cached 58): the MFMAs of one round of tiles (44 % busy over the
+// kernel), then 52 MB of stores.
 template <int N> DEVINL void wait_and_meet() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory"); }
 
 template <int MODE, int NWI, int NWJ, int WI, int WJ, int K, int ST, bool HEAVY> DEVINL void direct_tile(const LinP& p, int block, int blocks) {
@@ -465,7 +470,7 @@ __global__ __launch_bounds__(64 * NWI * NWJ) void linear_bf16_kernel(const LinP 
   direct_tile<MODE, NWI, NWJ, WI, WJ, K, ST, HEAVY>(p, blockIdx.x, gridDim.x);
 }
 // Both products of the backward in one launch: workgroups [0, nw) form dw (few and long), the others dx (many and short) beside them.  Alone,
-// neither keeps the memory system busy: 51200 x 256 x 256 19 + 20 us one after the other, 30 us together.
+// neither keeps the memory system busy: 51200 x 256 x 256 19 + 20 us one after the other, 30 us together (the kernels alone, cached).
 template <int T, bool DIRECT> __global__ __launch_bounds__(256) void linear_bf16_bwd_kernel(const LinP px, const LinP pw, const int nw) {
   const bool first = (int)blockIdx.x < nw;
   const int block = first ? blockIdx.x : blockIdx.x - nw, blocks = first ? nw : gridDim.x - nw;
@@ -577,7 +582,7 @@ template <int MODE> DEVINL void f32_store(const LinP& p, int slab, int i, int j,
 }
 
 // T x T tile, four waves of T / 2 x T / 2, v_mfma_f32_16x16x4_f32, two LDS images per operand, one barrier per stage, whole operands two stages
-// ahead (12800 x 512 x 512 83 us, 81 TFLOP/s; one ahead 103)
+// ahead (12800 x 512 x 512 82 us, 82 TFLOP/s; one ahead 103)
 template <int MODE, int T, bool WHOLE> __global__ __launch_bounds__(256) void linear_f32_kernel(const LinP p) {
   typedef F32Tile<MODE == MODE_DW, T, WHOLE> TA;
   typedef F32Tile<MODE != MODE_FWD, T, WHOLE> TB;
@@ -735,7 +740,7 @@ struct DzP {
 
 // dz and the column sums of `rows` rows: a thread owns one vector of columns (16 bytes of T, at any element address) and walks down the rows.
 // dz leaves with a pitch of whole vectors and zeros behind column N: the products then take it on their wide path whatever N is.
-// HBM: 51200 x 256 bf16 18 us, 4.4 TB/s.
+// HBM: 51200 x 256 bf16 21 us, 3.7 TB/s (the kernel alone; cached 18).
 template <typename T> __global__ __launch_bounds__(256) void linear_dz_kernel(const DzP p) {
   constexpr int V = Vec<T>::N, U = 4;
   __shared__ float red[256 * V];
@@ -853,8 +858,8 @@ size_t up16(size_t v) { return (v + 15) & ~(size_t)15; }
 
 // Tile of an I x J output: the larger, the fewer LDS reads per MFMA and the fewer re-reads of the operands; the smaller, the more of the chip a
 // small output fills.  256 (x 256, eight waves: one workgroup per compute unit) becomes 224 x 256 where that is still one round of the 256
-// compute units: 12800 x 2048 x 1024 82 -> 77 us, 12800 x 1024 x 1024 45 -> 43 us (M x K x N, z and y written, inputs from HBM).
-// 128 x 128 in place of 256 x 256 costs a sixth there.  fp32 and operands that pass registers (direct false): 128 or 64.
+// compute units: 12800 x 2048 x 1024 67 -> 64 us, 12800 x 1024 x 1024 40 -> 38 us.  128 x 128 in place of 256 x 256: 82 and 47 us.
+// fp32 and operands that pass registers (direct false): 128 or 64.
 int pick_tile(int64_t I, int64_t J, int64_t Kc, bool direct) {
   auto tiles = [&](int a, int b) { return ((I + a - 1) / a) * ((J + b - 1) / b); };
   if (direct && tiles(256, 256) >= 128 && J > 128 && Kc >= 512) return tiles(224, 256) <= 256 ? 224 : 256;
@@ -864,9 +869,11 @@ int pick_tile(int64_t I, int64_t J, int64_t Kc, bool direct) {
 
 // Tile and slabs of dw: enough row ranges to give every compute unit a workgroup, as long as the slabs are not more to move than the operands; a
 // layer that does not get there with 128 x 128 tiles takes small ones, and so does one whose output fills half of them (K <= 64, where dx has
-// small tiles too and the two share a launch: 204800 x 64 x 64 bf16 66 -> 52 us; fp32, N <= 64 also: 204800 x 128 x 64 171 -> 156).  bf16: three quarters of the compute units where dx shares the launch
-// (51200 x 256 x 256 backward 62 us, 64 with all of them, 71 with half or one and a half), two workgroups each where dx has its own large tiles
-// (12800 x 2048 x 1024 196 us, 239 at three quarters, 214 at three; 12800 x 1024 x 1024 120, 157, 140).
+// small tiles too and the two share a launch: 204800 x 64 x 64 bf16 66 -> 52 us; fp32, N <= 64 also: 204800 x 128 x 64 171 -> 151).
+// bf16: three quarters of the compute units where dx shares the launch (backward, three quarters / all / one and a half: 51200 x 256 x 256
+// 59.9 / 59.9 / 67 us, 204800 x 128 x 128 85.6 / 86.8 / 89.5, 25600 x 512 x 256 49 / 51 / 53), two workgroups each where dx has its own large
+// tiles (two / three quarters / three: 12800 x 2048 x 1024 182 / 234 / 200, 12800 x 1024 x 1024 115 / 157 / 127, 25600 x 1024 x 512
+// 118 / 160 / 136).
 void dw_plan(const plyolo_linear_desc* d, int tile, BwdPlan* b) {
   const bool half = d->dtype == PLYOLO_BF16;
   const int64_t tiles = (int64_t)cdiv(d->N, tile) * cdiv(d->K, tile);
@@ -1015,8 +1022,8 @@ int plyolo_linear_fwd(const plyolo_linear_desc* d, const void* x, const void* w,
   plyolo::annotate("linear_fwd", 2.0 * m * n * k, (m * k + n * k + m * n * (1.0 + (z ? 1 : 0) + (res ? 1 : 0))) * es);
   // Blocks of 16 R x 16 R re-read x once per 16 R columns and w once per 16 R rows, out of L2; a tile walks its whole contraction by itself.
   // Estimated microseconds, fitted over M 16 .. 51200, N 16 .. 2048, K 32 .. 2048.  Measured, M x K x N, us with R = 1 / R = 2 / tiles:
-  //   bf16  64 x 2048 x 1024  6.8 / 10.4 / 13.6   256 x 1024 x 1024  10.2 /  7.4 /  9.0   12800 x 64 x 64  6.5 / 5.1 / 4.4
-  //   fp32  64 x 2048 x 1024 11.4 / 22.2 / 53.3   256 x 1024 x 1024  18.5 / 14.1 / 30.8   3200 x 512 x 512  54 / 37 / 27.8
+  //   bf16  64 x 2048 x 1024  6.6 / 10.4 / 13.6   256 x 1024 x 1024  10.2 /  7.2 /  9.0   12800 x 64 x 64  6.5 / 5.1 / 4.4
+  //   fp32  64 x 2048 x 1024 10.7 / 22.2 / 53.3   256 x 1024 x 1024  18.5 / 13.8 / 30.8   3200 x 512 x 512  54 / 37 / 27.0
   const bool half = dtype == PLYOLO_BF16;
   auto again = [&](int e) { return (m * k * cdiv(d->N, e) + n * k * cdiv(d->M, e)) * es; };
   const double one_us = half ? 3.4 + again(16) / 9.6e6 : 6.0 + again(16) / 9.0e6, two_us = half ? 3.6 + again(32) / 8.0e6 : 5.0 + again(32) / 7.5e6;
