@@ -794,8 +794,8 @@ template <typename T, int V, int NV, int ACTC> __global__ __launch_bounds__(RES_
 // ------------------------------------------------------------------------------------------------ host side
 // Row chunks of one image in the streaming launches.  A function of the descriptor's sizes alone, so that the workspace does not depend on
 // addresses: four workgroups per compute unit over the whole batch (eight: 8 x 6400 x 320 bf16 forward 49 instead of 35 us), and at least 8192
-// values per chunk (2048 where that would leave fewer than 128 workgroups).  Beyond 2^29 values (bf16) there are more workgroups instead of
-// longer ones: a thread then sums THREAD_ROWS rows in fp32, and a chunk whose first value dwarfs the rest keeps its M2 to THREAD_ROWS^2 half
+// values per chunk (2048 where that would leave fewer than 128 workgroups).  From 2^28 .. 2^29 values on (bf16, by C; fp32 half) there are more workgroups
+// instead of longer ones: a thread then sums THREAD_ROWS rows in fp32, and a chunk whose first value dwarfs the rest keeps its M2 to THREAD_ROWS^2 half
 // steps at worst (4e-3; with 8208 rows a thread 0.12 was measured).
 constexpr int THREAD_ROWS = 256;
 void gn_chunks(const plyolo_gn_desc* d, int* chunks, int* rows) {

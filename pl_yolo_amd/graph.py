@@ -1485,6 +1485,12 @@ def drop_key(module, units):
     return tuple(u.drop_p() for u in units) if module.training else ()
 
 
+def without_other_drops(sessions, key):
+    """`sessions` (their keys end in drop_key) as a new one of `key` joins them: a training session takes the place of those of other
+    probabilities, so that a schedule does not pile them up; sessions of eval mode, and those beside one, stay."""
+    return {k: v for k, v in sessions.items() if not k[-1] or not key[-1] or k[-1] == key[-1]}
+
+
 def rng_state_of(module, device=None):
     """Device tensor (seed, step) of the dropouts of a traced module (layers.dropout_state)."""
     s = module.__dict__.get("_dropout_state")

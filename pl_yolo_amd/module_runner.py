@@ -238,7 +238,7 @@ class ModuleRunner:
         key = (tuple(tuple(x.shape) for x in xs), image, in_is_list, dtype, training, want_grad, mask, G.drop_key(self.m, G.dropout_units(self.m)))
         s = self.sessions.get(key)
         if s is None:
-            self.sessions = {k: v for k, v in self.sessions.items() if k[-1] in ((), key[-1])}     # a schedule of dropout probabilities does not pile up
+            self.sessions = G.without_other_drops(self.sessions, key)
             s = self._build([tuple(x.shape) for x in xs], image, in_is_list, dtype, training, want_grad, device)
             s.generation = 0
             self.sessions[key] = s

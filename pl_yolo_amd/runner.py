@@ -119,6 +119,7 @@ class DetectorRunner:
         key = (B, H, W, M, mode, self.dtype, self.model_ref.training, bool(getattr(self.model_ref.loss, "use_l1", False)), self.drop_key())
         s = self.sessions.pop(key, None)
         if s is None:
+            self.sessions = G.without_other_drops(self.sessions, key)
             before = torch.cuda.memory_allocated(device)
             s = self._build(B, H, W, M, mode, device)
             s.bytes = max(torch.cuda.memory_allocated(device) - before, 0)

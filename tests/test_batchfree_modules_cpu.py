@@ -100,9 +100,12 @@ def test_a_changed_dropout_probability_is_another_session():
     two.a.drop = 0.5
     assert [op.p for op in dropout_ops(trace(two, (1, 16, 4, 4), runner=r))] == [0.1]
     two.train()
+    two.d.p = 0.1
+    last = trace(two, (1, 16, 4, 4), runner=r)
     two.eval()
     evals = trace(two, (1, 16, 4, 4), want_grad=False, runner=r)
     two.train()
+    assert trace(two, (1, 16, 4, 4), runner=r) is last       # (a call in eval mode costs no training session)
     for i in range(1, 9):        # a schedule leaves one session behind, not one a value; those of eval mode stay
         two.d.p = i / 16
         last = trace(two, (1, 16, 4, 4), runner=r)

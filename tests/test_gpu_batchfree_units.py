@@ -4,6 +4,7 @@ rows, probabilities that change, several streams.
 Tolerances: bf16 stored values are off by half a step, 2^-8 relative (UNIT); the linear unit rounds x and W on their way in (the references
 here start from the rounded ones), z, dz and its outputs once each."""
 import ctypes as C
+import math
 import os
 
 import pytest
@@ -573,3 +574,25 @@ def test_units_beside_batch_norm_units(order, dtype):
         e = hu.relerr(v.grad, p[k].grad)
         print(k, e)
         assert e <= b, k
+
+
+def test_a_group_norm_detector_without_buffers_trains():
+    """No BatchNorm, no buffers at all: trainer, EMA and a schedule of dropout probabilities, which leaves one training session behind."""
+    from pl_yolo_amd.trainer import Trainer
+    m = gn_detector("yolox/yolox_test.yaml", "bf16")
+    assert not list(m.buffers())
+    imgs, labels = odet.synthetic_batch(2, 64, 3, num_gt=3, max_gt=8, seed=5)
+    imgs, labels = imgs.to(DEV), labels.to(DEV)
+    tr = Trainer(m, learning_rate=0.005, total_steps=100, ema=True)
+    before = m.head.stems[0].norm.weight.detach().clone()
+    state = dropout_state(m)
+    unit = m.backbone.stage4[2].conv3
+    for i in range(4):
+        unit.drop = 0.1 * (i + 1)
+        assert math.isfinite(float(tr.train_step(imgs, labels)["loss"].detach()))
+    assert not torch.equal(before, m.head.stems[0].norm.weight.detach()) and state.tolist()[1] == 4
+    assert [k[4] for k in m.runner().sessions] == ["train"]
+    m.eval()
+    with torch.no_grad():
+        assert bool(torch.isfinite(m(imgs, labels)).all())
+    assert sorted(k[4] for k in m.runner().sessions) == ["eval", "train"]
