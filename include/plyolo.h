@@ -512,8 +512,9 @@ int plyolo_lnw_act_bwd(int dtype, int N, int H, int W, int C, const void* dout, 
  * gamma, beta: fp32 [C], NULL = 1 / 0.  Any C, pitch and element-aligned address; rows of at least one 16-byte vector of channels are read
  * and written by vectors, whatever their alignment, and rows of whole vectors may stay in registers between the two passes.
  * Statistics and gradient sums are formed in a fixed order (no atomics): results repeat bit for bit.  A NaN or infinity stays inside its
- * (image, group), whose outputs become NaN; as everywhere in this library relu is u > 0 ? u : 0, so it turns them into 0, and
- * slopes that are chosen by comparisons stay finite (act'(NaN): relu 0, lrelu 0.1, hswish 0).  No operand may overlap another, except out == x and dx == dout (same pitch).
+ * (image, group), whose outputs become NaN; as everywhere in this library relu is u > 0 ? u : 0, so it turns them into 0, and slopes that
+ * are chosen by comparisons stay finite (act'(NaN): relu 0, lrelu 0.1, hswish 0).  No operand may overlap another, except out == x and
+ * dx == dout (same pitch).
  * Workspace: plyolo_gn_workspace(d) bytes, 16-byte aligned, contents need not survive a call; calls that may run at the same time
  * (streams, captured graphs) need one each.  C <= 4096, N*HW and every pitch below 2^31, N * ceil(groups / 32) below 2^22 - 128. */
 typedef struct plyolo_gn_desc {

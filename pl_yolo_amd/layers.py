@@ -206,7 +206,8 @@ class Dropout(HipModule):
 
 
 def dropout_state(module):
-    """The state of `module`'s dropouts: a device int64 tensor (seed, step).  Every training forward of the module advances `step` by one;
+    """The state of `module`'s dropouts: a device int64 tensor (seed, step).  Every training forward of the module that drops advances `step`
+    by one (sub-modules called by themselves have states of their own; the state is no buffer: save it beside a checkpoint to resume it);
     copying a saved tensor back (`dropout_state(m).copy_(saved)`) resumes its masks.  The seed is drawn from torch's default CPU generator
     when the state is first used (torch.manual_seed makes it repeat), with the rank of the process group mixed in."""
     return G.rng_state_of(module)

@@ -249,11 +249,12 @@ def test_a_group_norm_detector_does_not_depend_on_its_batch(path, dtype):
 @pytest.mark.parametrize("path", ["yolox/yolox_test.yaml", "yolov7/yolov7_test.yaml"])
 def test_group_norm_detector_steps_repeat_on_any_lanes(path, monkeypatch):
     """bf16 training steps with group norm everywhere and dropout in two units: loss and every gradient are the same bit for bit on several
-    streams, on one, and again."""
+    streams, on one, and again, and so as captured graphs."""
     imgs, labels = odet.synthetic_batch(2, 96, 3, num_gt=3, max_gt=8, seed=77)
     runs = []
-    for lanes in ("1", "0", "1"):
+    for lanes, graph in (("1", "auto"), ("0", "auto"), ("1", "auto"), ("0", "1"), ("1", "1"), ("0", "0")):
         monkeypatch.setenv("PLYOLO_LANES", lanes)
+        monkeypatch.setenv("PLYOLO_GRAPH", graph)
         m = gn_detector(path, "bf16")
         units = [k for k in m.modules() if isinstance(k, BaseConv)]
         units[5].drop, units[-4].drop = 0.25, 0.5
@@ -262,9 +263,9 @@ def test_group_norm_detector_steps_repeat_on_any_lanes(path, monkeypatch):
             m.zero_grad(set_to_none=True)
             loss = m(imgs.to(DEV), labels.to(DEV))["loss"]
             loss.sum().backward()
-            runs.append((lanes, loss.detach().clone(), {n: p.grad.clone() for n, p in m.named_parameters() if p.grad is not None}))
+            runs.append(((lanes, graph), loss.detach().clone(), {n: p.grad.clone() for n, p in m.named_parameters() if p.grad is not None}))
     assert not torch.equal(runs[0][1], runs[1][1])            # another mask each step
-    for i in range(3, 9):
+    for i in range(3, len(runs)):
         (_, l0, g0), (lanes, l1, g1) = runs[i % 3], runs[i]
         assert torch.equal(l0, l1), (lanes, i)
         off = [n for n in g0 if not torch.equal(g0[n], g1[n])]
